@@ -1,0 +1,255 @@
+// Appending to the paged key/value cache held in 8 bits.
+//
+// One power-of-two scale s per (page, kv head, K or V); a cached value is s times an e4m3 code.  New rows of a page need
+//   need = 2^ceil(log2(amax / 448)), clamped to [2^-24, 2^64],  amax over the finite |x| of the page's new rows;
+//   s'   = need where the page begins with them (slot 0 is among them), else max(s, need).
+// Where s' > s the page's older codes become RN(code * s / s'); the new rows are RN_sat(x / s').  e4m3 is a floating
+// format, so a power-of-two scale costs no precision, dividing by it is exact, and a grown scale moves the exponents of
+// the older codes: only codes that leave the normal range (below 2^-6) lose bits, once per growth.
+//
+// The rows are named by sequence (block table, length, new tokens), so one block owns all rows of a page that a call
+// writes: the page's maximum is taken and its rows are written in one pass over them, with no atomics and no second
+// launch.
+#include <ATen/core/Tensor.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+
+#include "q8.cuh"
+
+using namespace cl;
+using namespace q8;
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct AppendArgs {
+  const void* x[2];              // new keys, new values
+  int64_t row[2], head[2];       // strides in elements
+  uint8_t* codes[2];             // [pages, nkv, bs, D]
+  float* scale[2];               // [pages, nkv]
+  const int* tables;             // [B, width]
+  const int* lens;               // [B] lengths with the new tokens
+  const int* news;               // [B] new tokens (null: one each)
+  int B, width, T, nkv, D, bs;
+  int64_t pages;
+};
+
+// 8 consecutive elements as fp32; `vec`: the address is 16-byte aligned
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, float (&f)[8]) {
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < 8; i += 16 / (int)sizeof(T)) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p + i);
+      const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+      for (int j = 0; j < 16 / (int)sizeof(T); ++j) f[i + j] = to_float(t[j]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_float(p[i]);
+  }
+}
+
+// largest finite magnitude
+__device__ __forceinline__ float finite_max(float m, const float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float a = fabsf(f[i]);
+    m = a < INFINITY ? fmaxf(m, a) : m;
+  }
+  return m;
+}
+
+__device__ __forceinline__ void store8(uint8_t* p, const float (&f)[8], float inv) {
+  uint2 u;
+  u.x = pack_e4m3(f[0] * inv, f[1] * inv) | (uint32_t)pack_e4m3(f[2] * inv, f[3] * inv) << 16;
+  u.y = pack_e4m3(f[4] * inv, f[5] * inv) | (uint32_t)pack_e4m3(f[6] * inv, f[7] * inv) << 16;
+  *reinterpret_cast<uint2*>(p) = u;
+}
+
+// older codes of a page under its grown scale; n is a multiple of 8
+__device__ __forceinline__ void regrade(uint8_t* codes, int n, float ratio, int tid, int step) {
+  for (int i = tid * 8; i < n; i += step * 8) {
+    const uint2 u = *reinterpret_cast<const uint2*>(codes + i);
+    float f[8];
+    unpack_e4m3(u.x, f);
+    unpack_e4m3(u.y, f + 4);
+    store8(codes + i, f, ratio);
+  }
+}
+
+// One token per sequence: a warp per (sequence, kv head, K or V).  The chain length -> table -> scale of dependent
+// loads is all there is to wait for; the row itself is loaded beside it.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs a) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int64_t item = blockIdx.x * (int64_t)(kThreads / 32) + (threadIdx.x >> 5);
+  const int b = (int)(item / (2 * a.nkv)), h = (int)(item / 2 % a.nkv), kv = (int)(item & 1);
+  if (b >= min(a.B, a.T)) return;
+  const T* x = static_cast<const T*>(a.x[kv]) + b * a.row[kv] + h * a.head[kv];
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  float f[2][8], amax = 0.f;                       // D <= 512
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if ((i * 32 + lane) * 8 < a.D) {
+      load8(x + (i * 32 + lane) * 8, vec, f[i]);
+      amax = finite_max(amax, f[i]);
+    }
+  amax = warp_max(amax);
+  const int pos = a.lens[b] - 1;
+  if (pos < 0 || pos / a.bs >= a.width) return;
+  const int page = a.tables[(int64_t)b * a.width + pos / a.bs], off = pos % a.bs;
+  if (page < 0 || page >= a.pages) return;
+  const int64_t ph = (int64_t)page * a.nkv + h;
+  uint8_t* codes = a.codes[kv] + ph * a.bs * a.D;
+  float s = scale_for(amax);
+  if (off > 0) {
+    const float old = a.scale[kv][ph];
+    if (s > old) regrade(codes, off * a.D, old / s, lane, 32);
+    else s = old;
+  }
+  __syncwarp();
+  if (lane == 0) a.scale[kv][ph] = s;
+  const float inv = 1.f / s;
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if ((i * 32 + lane) * 8 < a.D) store8(codes + (int64_t)off * a.D + (i * 32 + lane) * 8, f[i], inv);
+}
+
+// Any number of tokens per sequence: a block per (page that gets new rows, kv head, K or V).  The rows of a page of 64 x
+// 128 fit the block's registers (kKeep vectors of 8 a thread), so they are read once; longer pages read the rest again,
+// out of L2.
+constexpr int kKeep = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) append_pages_kernel(const AppendArgs a) {
+  __shared__ int sh_scan[2][kThreads / 32];
+  __shared__ int sh_found[4];
+  __shared__ float sh_max[kThreads / 32];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // which (sequence, page) is this block's: prefix sums of the pages and rows that the sequences add
+  if (tid == 0) sh_found[0] = -1;
+  int base_pages = 0, base_rows = 0;
+  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
+    const int b = b0 + tid;
+    int n = 0, len = 0, cnt = 0;
+    if (b < a.B) {
+      len = a.lens[b];
+      n = max(0, a.news ? a.news[b] : min(1, len));
+      const int from = max(len - n, 0);
+      cnt = (n > 0 && len > 0) ? (len - 1) / a.bs - from / a.bs + 1 : 0;
+    }
+    int ip = cnt, ir = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int p = __shfl_up_sync(0xffffffffu, ip, o), r = __shfl_up_sync(0xffffffffu, ir, o);
+      if (lane >= o) { ip += p; ir += r; }
+    }
+    __syncthreads();
+    if (lane == 31) { sh_scan[0][warp] = ip; sh_scan[1][warp] = ir; }
+    __syncthreads();
+    int bp = base_pages, br = base_rows;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) { bp += sh_scan[0][w]; br += sh_scan[1][w]; }
+      base_pages += sh_scan[0][w]; base_rows += sh_scan[1][w];
+    }
+    const int first = bp + ip - cnt;
+    if (cnt > 0 && first <= (int)blockIdx.x && (int)blockIdx.x < first + cnt) {
+      const int from = max(len - n, 0), pg = from / a.bs + ((int)blockIdx.x - first);
+      const int lo = max(from, pg * a.bs), hi = min(len, (pg + 1) * a.bs);
+      int row = br + ir - n + (lo - (len - n));               // row of the page's first new token
+      sh_found[1] = lo % a.bs;
+      sh_found[2] = min(hi - lo, a.T - row);                   // rows that the tensors really hold
+      sh_found[3] = row;
+      if (sh_found[2] > 0 && pg < a.width) sh_found[0] = a.tables[(int64_t)b * a.width + pg];
+    }
+    __syncthreads();
+    if (base_pages > (int)blockIdx.x) break;
+  }
+  const int page = sh_found[0], off = sh_found[1], m = sh_found[2], row = sh_found[3];
+  if (page < 0 || page >= a.pages) return;
+  const int h = blockIdx.y, kv = blockIdx.z;
+  const T* x = static_cast<const T*>(a.x[kv]) + row * a.row[kv] + h * a.head[kv];
+  const bool vec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(a.row[kv] * sizeof(T))) & 15) == 0;
+  const int per = a.D / 8, total = m * per;
+  float f[kKeep][8], amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int c = i * kThreads + tid;
+    if (c < total) {
+      load8(x + (c / per) * a.row[kv] + (c % per) * 8, vec, f[i]);
+      amax = finite_max(amax, f[i]);
+    }
+  }
+  for (int c = kKeep * kThreads + tid; c < total; c += kThreads) {
+    float g[8];
+    load8(x + (c / per) * a.row[kv] + (c % per) * 8, vec, g);
+    amax = finite_max(amax, g);
+  }
+  amax = warp_max(amax);
+  if (lane == 0) sh_max[warp] = amax;
+  const int64_t ph = (int64_t)page * a.nkv + h;
+  const float old = off > 0 ? a.scale[kv][ph] : 0.f;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, sh_max[w]);
+  const float s = fmaxf(scale_for(amax), old), inv = 1.f / s;
+  uint8_t* codes = a.codes[kv] + ph * a.bs * a.D;
+  if (off > 0 && s > old) regrade(codes, off * a.D, old / s, tid, kThreads);
+  if (tid == 0) a.scale[kv][ph] = s;               // every thread has read the old scale before the barrier above
+  uint8_t* to = codes + (int64_t)off * a.D;
+#pragma unroll
+  for (int i = 0; i < kKeep; ++i) {
+    const int c = i * kThreads + tid;
+    if (c < total) store8(to + c * 8, f[i], inv);
+  }
+  for (int c = kKeep * kThreads + tid; c < total; c += kThreads) {
+    float g[8];
+    load8(x + (c / per) * a.row[kv] + (c % per) * 8, vec, g);
+    store8(to + c * 8, g, inv);
+  }
+}
+
+template <typename T>
+void launch_append(const AppendArgs& a, cudaStream_t st) {
+  if (!a.news) {
+    const int64_t items = (int64_t)std::min(a.B, a.T) * a.nkv * 2;
+    const int64_t grid = (items + kThreads / 32 - 1) / (kThreads / 32);
+    C10_CUDA_CHECK(launch_pdl(append_step_kernel<T>, dim3((unsigned)grid), dim3(kThreads), 0, st, a));
+  } else {
+    // a sequence with n new tokens adds to at most (n - 1) / bs + 2 pages
+    const int64_t runs = std::min<int64_t>(a.T, a.T / a.bs + 2 * (int64_t)a.B);
+    C10_CUDA_CHECK(launch_pdl(append_pages_kernel<T>, dim3((unsigned)runs, a.nkv, 2), dim3(kThreads), 0, st, a));
+  }
+}
+
+}  // namespace
+
+void kv_append_q8(const at::Tensor& k, const at::Tensor& v, at::Tensor kc, at::Tensor vc, at::Tensor ks, at::Tensor vs,
+                  const at::Tensor& tables, const at::Tensor& lens, const c10::optional<at::Tensor>& news) {
+  const c10::cuda::CUDAGuard guard(k.device());
+  AppendArgs a;
+  a.x[0] = k.data_ptr(); a.x[1] = v.data_ptr();
+  a.row[0] = k.stride(0); a.row[1] = v.stride(0);
+  a.head[0] = k.stride(1); a.head[1] = v.stride(1);
+  a.codes[0] = (uint8_t*)kc.data_ptr(); a.codes[1] = (uint8_t*)vc.data_ptr();
+  a.scale[0] = ks.data_ptr<float>(); a.scale[1] = vs.data_ptr<float>();
+  a.tables = tables.data_ptr<int>(); a.lens = lens.data_ptr<int>();
+  a.news = news.has_value() ? news->data_ptr<int>() : nullptr;
+  a.B = (int)lens.size(0); a.width = (int)tables.size(1); a.T = (int)k.size(0);
+  a.nkv = (int)kc.size(1); a.bs = (int)kc.size(2); a.D = (int)kc.size(3); a.pages = kc.size(0);
+  if (a.B == 0 || a.T == 0 || a.width == 0) return;
+  auto st = at::cuda::getCurrentCUDAStream();
+  if (k.scalar_type() == at::kBFloat16) launch_append<__nv_bfloat16>(a, st);
+  else if (k.scalar_type() == at::kHalf) launch_append<__half>(a, st);
+  else launch_append<float>(a, st);
+}

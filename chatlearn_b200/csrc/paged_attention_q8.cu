@@ -1,0 +1,578 @@
+// Attention over the paged key/value cache held in 8 bits (e4m3 codes, one power-of-two scale per page and kv head).
+//
+//   o = softmax(scale * q (s_k C_k)^T) (s_v C_v)
+//
+// One unit of work is (query row set, kv head): the query heads that share a kv head are the rows of one m16n8k16 tile,
+// so each cached byte is read once per unit and dequantised once.  Codes become halves by one conversion (exact: e4m3
+// is a subset of fp16); the scales are powers of two and stay out of the products: s_k joins the softmax scale, s_v the
+// probabilities.  Queries are rescaled per row by a power of two to 2^10..2^11, so that their fp16 form loses nothing
+// that counts (bf16 has 8 significant bits, fp16 11; what falls below 2^-24 of a row's largest is lost).
+//
+// The bytes of the cache bound it.  The tokens of all units form one line that is cut evenly over the resident blocks
+// (whatever the lengths are), 64 at a time; a unit that a cut divides is written as partial (o, m, l) and joined by a
+// second kernel.  The cut goes by the lengths alone, so results do not depend on timing.  Inside a block each warp owns
+// 16 of the 64 tokens with its own cp.async ring, running maximum and sum: no barrier in the loop; the four streams meet
+// at the end of a unit.
+#include <ATen/core/Tensor.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_pipeline.h>
+
+#include <atomic>
+
+#include "q8.cuh"
+
+using namespace cl;
+using namespace q8;
+
+namespace {
+
+constexpr int kThreads = 128, kWarps = 4;
+constexpr int kTile = 64;                         // tokens of a tile: 16 for each warp
+// probabilities are carried times 2^10: fp16 keeps 11 bits of them down to 2^-24 of the largest
+constexpr float kProbShift = 10.f;
+
+struct Args {
+  const void* q;                 // [T, nq, D], row stride q_row
+  int64_t q_row;
+  const uint8_t *kc, *vc;        // [pages, nkv, bs, D]
+  const float *ks, *vs;          // [pages, nkv]
+  const int* tables;             // [B, width]
+  const int* row_seq;            // [rows] sequence of a query row (null: the row's own number)
+  const int* row_len;            // [rows] tokens it sees
+  void* out;                     // [T, nq, D]
+  float *part_o, *part_ml;       // [2 * grid, 16, D], [2 * grid, 16, 2]
+  int rows, T, width, nq, nkv, bs;
+  int64_t pages;
+  int grid;                      // blocks that the line is cut over
+  float scale;                   // softmax scale times log2 e
+};
+
+__device__ __forceinline__ int tiles_of(const Args& a, int r) {
+  const int len = min(a.row_len[r], a.width * a.bs);
+  return len > 0 ? (len + kTile - 1) / kTile : 0;
+}
+
+// The line is cut into min(blocks, tiles) shares: none is empty, and their bounds go by the lengths alone.
+struct Place {
+  int64_t total;                 // tiles of the line
+  int64_t shares;
+  int64_t pos;                   // where share `index` begins (total, if there is no such share)
+  int row;                       // row set that holds this position
+  int64_t base;                  // where that row set begins
+  __device__ __forceinline__ int64_t begin(int64_t i) const { return i * total / shares; }
+};
+
+// Exclusive prefix sums over the rows' tiles, `per_row` units each.  All threads of the block take part.
+__device__ Place locate(const Args& a, int per_row, int index, int64_t* sh) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (a.rows + kThreads - 1) / kThreads;
+  const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
+  int64_t sum = 0;
+  for (int r = r0; r < r1; ++r) sum += tiles_of(a, r);
+  sum *= per_row;
+  int64_t inc = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t p = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += p;
+  }
+  if (lane == 31) sh[warp] = inc;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += sh[w];
+    total += sh[w];
+  }
+  Place p;
+  p.total = total;
+  p.shares = max((int64_t)1, min((int64_t)a.grid, total));
+  p.pos = index < p.shares ? p.begin(index) : total;
+  const int64_t pos = p.pos;
+  const int64_t first = before + inc - sum;
+  if (first <= pos && pos < first + sum) {
+    int64_t at = first;
+    int r = r0;
+    for (; r < r1; ++r) {
+      const int64_t n = (int64_t)tiles_of(a, r) * per_row;
+      if (pos < at + n) break;
+      at += n;
+    }
+    sh[4] = r;
+    sh[5] = at;
+  }
+  __syncthreads();
+  p.row = (int)sh[4];
+  p.base = sh[5];
+  return p;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16-byte chunk of a row after the swizzle that keeps both reads below free of bank conflicts: eight lanes that read in
+// one phase are two neighbouring rows x four chunks (keys), or rows 0, 2, 4, 6 x the chunks c and c + 4 (values)
+template <int D>
+__device__ __forceinline__ int swizzled(int r, int chunk) {
+  if (D >= 128) return chunk ^ (((r & 1) << 2) | ((r >> 1) & 3));
+  return chunk ^ ((r >> 1) & 3);
+}
+
+// A warp's position on the line.
+struct Cursor {
+  int row, unit, tile, tiles, len;               // row set, unit of it (kv head, row tile), tile, the row's tiles and tokens
+  __device__ __forceinline__ void enter(const Args& a, int r) {
+    row = r;
+    while (row < a.rows && (tiles = tiles_of(a, row)) == 0) ++row;
+    len = row < a.rows ? min(a.row_len[row], a.width * a.bs) : 0;
+  }
+  __device__ __forceinline__ void next(const Args& a, int per_row) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++unit < per_row) return;
+    unit = 0;
+    enter(a, row + 1);
+  }
+};
+
+template <int D, int ST>
+struct WarpRing {
+  uint8_t k[ST][16 * D];
+  uint8_t v[ST][16 * D];
+  float s[ST][4];                                // scales of K and V, validity of the page
+};
+
+template <typename T, int D, int ST>
+__global__ void __launch_bounds__(kThreads)
+paged_q8_kernel(const Args a) {
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ int64_t sh_place[8];
+  __shared__ float sh_m[kWarps][16], sh_l[kWarps][16];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  auto& ring = reinterpret_cast<WarpRing<D, ST>*>(smem)[warp];
+  float* red = reinterpret_cast<float*>(smem + sizeof(WarpRing<D, ST>) * kWarps);   // [2][rows of a unit][D]
+  const int red_rows = min(a.nq / a.nkv, 16);
+  const int rep = a.nq / a.nkv, row_tiles = (rep + 15) / 16, per_row = a.nkv * row_tiles;
+  T* out = static_cast<T*>(a.out);
+
+  // rows that see nothing are zero
+  for (int r = blockIdx.x; r < a.T; r += a.grid)
+    if (r >= a.rows || tiles_of(a, r) == 0)
+      for (int i = tid; i < a.nq * D; i += kThreads) out[(int64_t)r * a.nq * D + i] = from_float<T>(0.f);
+
+  const Place place = locate(a, per_row, blockIdx.x, sh_place);
+  const int64_t pos = place.pos;
+  if (pos >= place.total) return;
+  const int64_t end = place.begin(blockIdx.x + 1);
+  Cursor use;
+  use.enter(a, place.row);
+  use.unit = (int)((pos - place.base) / use.tiles);
+  use.tile = (int)((pos - place.base) % use.tiles);
+  Cursor load = use;
+  int64_t left_load = end - pos;
+  int64_t left = end - pos;
+
+  auto page_of = [&](const Cursor& c) -> int {
+    const int tok = c.tile * kTile + warp * 16;
+    if (tok >= c.len) return -1;
+    const int seq = a.row_seq ? a.row_seq[c.row] : c.row;
+    return a.tables[(int64_t)seq * a.width + tok / a.bs];
+  };
+  int page = left_load > 0 ? page_of(load) : -1;
+  auto issue = [&](int st) {
+    if (left_load > 0) {
+      const int tok = load.tile * kTile + warp * 16;
+      if (tok < load.len) {
+        const bool ok = page >= 0 && page < a.pages;
+        const int64_t ph = (int64_t)(ok ? page : 0) * a.nkv + load.unit / row_tiles;
+        const int64_t at = (ph * a.bs + tok % a.bs) * D;
+        const int valid = ok ? min(16, load.len - tok) : 0;
+        constexpr int CH = D / 16;
+#pragma unroll
+        for (int i = 0; i < 16 * CH / 32; ++i) {
+          const int c = i * 32 + lane, r = c / CH;
+          const int to = r * D + swizzled<D>(r, c % CH) * 16;
+          // rows behind the sequence's end are filled with zeros: 0 * garbage must not be NaN
+          __pipeline_memcpy_async(&ring.k[st][to], a.kc + at + c * 16, 16, r < valid ? 0 : 16);
+          __pipeline_memcpy_async(&ring.v[st][to], a.vc + at + c * 16, 16, r < valid ? 0 : 16);
+        }
+        if (lane < 2) __pipeline_memcpy_async(&ring.s[st][lane], (lane ? a.vs : a.ks) + ph, 4);
+        if (lane == 2) ring.s[st][2] = ok ? 1.f : 0.f;
+      }
+      load.next(a, per_row);
+      --left_load;
+      page = left_load > 0 ? page_of(load) : -1;
+    }
+    __pipeline_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < ST - 1; ++s) issue(s);
+
+  int st = 0;
+  bool first_unit = true;
+  while (left > 0) {
+    // ---------------- a unit, or the part of it in this block's share
+    const int head = use.unit / row_tiles, rt = use.unit % row_tiles;
+    const int rows_here = min(16, rep - rt * 16);
+    const int from_tile = use.tile, n = (int)min((int64_t)(use.tiles - use.tile), left);
+    const int row = use.row, tiles = use.tiles, len = use.len;
+    const T* q = static_cast<const T*>(a.q) + row * a.q_row + (int64_t)(head * rep + rt * 16) * D;
+    // Q fragments: k-step s of chunk i holds elements 16 (t + 4 i) + 4 s .. + 3 of rows g and g + 8 (the order of the
+    // contraction is free as long as K's fragments follow it)
+    constexpr int KI = D / 64;
+    uint32_t qa[KI * 4][4];
+    float sc[2];
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int r = g + 8 * hf;
+      float f[KI][16], big = 0.f;
+#pragma unroll
+      for (int i = 0; i < KI; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; e += 8) {
+          if (r < rows_here) {
+            const uint4 u = *reinterpret_cast<const uint4*>(q + (int64_t)r * D + 16 * (t + 4 * i) + e);
+            const T* x = reinterpret_cast<const T*>(&u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) { f[i][e + j] = to_float(x[j]); big = fmaxf(big, fabsf(f[i][e + j])); }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[i][e + j] = 0.f;
+          }
+        }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // power of two that brings the row's largest to [2^10, 2^11)
+      const int e = big > 0.f ? min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 120) : 0;
+      const float up = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
+      sc[hf] = a.scale * __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+#pragma unroll
+      for (int i = 0; i < KI; ++i)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          qa[i * 4 + s][hf] = half2_bits(f[i][4 * s] * up, f[i][4 * s + 1] * up);
+          qa[i * 4 + s][2 + hf] = half2_bits(f[i][4 * s + 2] * up, f[i][4 * s + 3] * up);
+        }
+    }
+    constexpr int NT = D / 8;
+    float o[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float unit_v = 0.f;                            // o is kept in units of this V scale
+
+    for (int i = 0; i < n; ++i) {
+      __pipeline_wait_prior(ST - 2);
+      __syncwarp();                                // every lane's copies of this stage are in, every lane is done with the last
+      issue(st == 0 ? ST - 1 : st - 1);
+      const int tok = (from_tile + i) * kTile + warp * 16;
+      if (tok < len && ring.s[st][2] != 0.f) {
+        const float k_scale = ring.s[st][0], v_scale = ring.s[st][1];
+        // ---- S = Q K^T: two groups of 8 tokens
+        float s[2][4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+          for (int c = 0; c < KI; ++c) {
+            const int r = j * 8 + g;
+            const uint4 u = *reinterpret_cast<const uint4*>(&ring.k[st][r * D + swizzled<D>(r, t + 4 * c) * 16]);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma_f16(s[j], qa[c * 4 + e], e4m3x2_to_half2(w[e]), e4m3x2_to_half2(w[e] >> 16));
+          }
+        }
+        // ---- running softmax of rows g (h = 0) and g + 8 (h = 1)
+        float alpha[2];
+        bool grown = false;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float f = sc[h] * k_scale;
+          float mx = m[h];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& x = s[j][2 * h + e];
+              x = tok + j * 8 + 2 * t + e < len ? x * f : -INFINITY;
+              mx = fmaxf(mx, x);
+            }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          alpha[h] = mx == m[h] ? 1.f : exp2_approx(m[h] - mx);
+          grown |= mx != m[h];
+          m[h] = mx;
+        }
+        // V's scale joins the probabilities, relative to the unit that o is kept in; the unit follows the scale where
+        // they are far apart, so that the probabilities stay inside fp16's normal range
+        float change = 1.f, ratio = unit_v > 0.f ? v_scale / unit_v : 0.f;
+        if (v_scale > 0.f && !(ratio <= 1.f && ratio >= 0.0625f)) {
+          change = unit_v / v_scale;
+          unit_v = v_scale;
+          ratio = 1.f;
+          grown = true;
+        }
+        if (__any_sync(0xffffffffu, grown)) {
+          l[0] *= alpha[0]; l[1] *= alpha[1];
+          alpha[0] *= change; alpha[1] *= change;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) { o[j][0] *= alpha[0]; o[j][1] *= alpha[0]; o[j][2] *= alpha[1]; o[j][3] *= alpha[1]; }
+        }
+        uint32_t pa[4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float shift = m[h] == -INFINITY ? 0.f : m[h] - kProbShift;
+          float p[2][2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) { p[j][e] = exp2_approx(s[j][2 * h + e] - shift); l[h] += p[j][e]; }
+          pa[h] = half2_bits(p[0][0] * ratio, p[0][1] * ratio);
+          pa[2 + h] = half2_bits(p[1][0] * ratio, p[1][1] * ratio);
+        }
+        // ---- O += P V: lane g holds the columns of its chunk (or half chunk at D = 64)
+        constexpr int VB = D >= 128 ? 16 : 8;      // bytes of a lane's piece of a row
+#pragma unroll
+        for (int c = 0; c < D / (8 * VB); ++c) {
+          uint32_t w[4][VB / 4];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int r = 2 * t + (x & 1) + (x >> 1) * 8;
+            const int piece = ((g & 1) << 2) | (g >> 1);
+            if constexpr (VB == 16) {
+              const uint4 u = *reinterpret_cast<const uint4*>(&ring.v[st][r * D + swizzled<D>(r, piece + 8 * c) * 16]);
+              w[x][0] = u.x; w[x][1] = u.y; w[x][2] = u.z; w[x][3] = u.w;
+            } else {
+              const uint2 u = *reinterpret_cast<const uint2*>(&ring.v[st][r * D + swizzled<D>(r, piece >> 1) * 16 + (piece & 1) * 8]);
+              w[x][0] = u.x; w[x][1] = u.y;
+            }
+          }
+#pragma unroll
+          for (int y = 0; y < VB / 4; ++y) {
+            const uint32_t a01 = __byte_perm(w[0][y], w[1][y], 0x5140), a23 = __byte_perm(w[0][y], w[1][y], 0x7362);
+            const uint32_t b01 = __byte_perm(w[2][y], w[3][y], 0x5140), b23 = __byte_perm(w[2][y], w[3][y], 0x7362);
+            const int j = c * VB + y * 4;
+            mma_f16(o[j], pa, e4m3x2_to_half2(a01), e4m3x2_to_half2(b01));
+            mma_f16(o[j + 1], pa, e4m3x2_to_half2(a01 >> 16), e4m3x2_to_half2(b01 >> 16));
+            mma_f16(o[j + 2], pa, e4m3x2_to_half2(a23), e4m3x2_to_half2(b23));
+            mma_f16(o[j + 3], pa, e4m3x2_to_half2(a23 >> 16), e4m3x2_to_half2(b23 >> 16));
+          }
+        }
+      }
+      st = st + 1 == ST ? 0 : st + 1;
+    }
+    left -= n;
+    use.tile += n - 1;
+    use.next(a, per_row);
+
+    // ---------------- the four streams of the unit meet
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (t == 0) { sh_m[warp][g + 8 * h] = m[h]; sh_l[warp][g + 8 * h] = l[h]; }
+    }
+    __syncthreads();
+    float top[2], w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) top[h] = fmaxf(top[h], sh_m[x][g + 8 * h]);
+      w[h] = m[h] == -INFINITY && l[h] == 0.f ? 0.f : exp2_approx(m[h] - top[h]) * unit_v;
+    }
+    // column of accumulator j: piece of lane 2 t (+ 1), element j
+    constexpr int VB = D >= 128 ? 16 : 8;
+    auto column = [&](int j, int e) { return (j / VB) * (8 * VB) + (e * 4 + t) * VB + j % VB; };
+#pragma unroll
+    for (int pass = 0; pass < 2; ++pass) {
+      if ((warp >> 1) == pass) {
+        float* to = red + (warp & 1) * red_rows * D;
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (g + 8 * h < rows_here)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float& x = to[(g + 8 * h) * D + column(j, e)];
+                const float y = w[h] == 0.f ? 0.f : o[j][2 * h + e] * w[h];
+                x = pass ? x + y : y;
+              }
+      }
+      __syncthreads();
+    }
+    const bool whole = from_tile == 0 && n == tiles;
+    const int slot = 2 * blockIdx.x + (first_unit && from_tile > 0 ? 0 : 1);
+    for (int i = tid; i < rows_here * D; i += kThreads) {
+      const int r = i / D, d = i % D;
+      float big = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x) big = fmaxf(big, sh_m[x][r]);
+#pragma unroll
+      for (int x = 0; x < kWarps; ++x)
+        if (sh_l[x][r] != 0.f) sum += sh_l[x][r] * exp2_approx(sh_m[x][r] - big);
+      const float val = red[i] + red[red_rows * D + i];
+      if (whole) {
+        out[((int64_t)row * a.nq + head * rep + rt * 16 + r) * D + d] = from_float<T>(sum == 0.f ? 0.f : val / sum);
+      } else {
+        a.part_o[((int64_t)slot * 16 + r) * D + d] = val;
+        if (d == 0) {
+          a.part_ml[(slot * 16 + r) * 2] = big;
+          a.part_ml[(slot * 16 + r) * 2 + 1] = sum;
+        }
+      }
+    }
+    first_unit = false;
+    __syncthreads();
+  }
+}
+
+// Joins the parts of the units that the cuts divide: block c looks after the cut in front of block c + 1's share, if it
+// is the first cut inside its unit.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) paged_q8_join_kernel(const Args a) {
+  __shared__ int64_t sh_place[8];
+  pdl_trigger();
+  pdl_wait();
+  const int rep = a.nq / a.nkv, row_tiles = (rep + 15) / 16, per_row = a.nkv * row_tiles;
+  const int c = blockIdx.x + 1;
+  const Place place = locate(a, per_row, c, sh_place);
+  const int64_t pos = place.pos;
+  if (pos >= place.total) return;
+  const int tiles = tiles_of(a, place.row);
+  const int unit = (int)((pos - place.base) / tiles);
+  const int64_t start = place.base + (int64_t)unit * tiles, stop = start + tiles;
+  if (pos == start || place.begin(c - 1) > start) return;
+  int last = c;                                    // last block with a part
+  while (last + 1 < place.shares && place.begin(last + 1) < stop) ++last;
+  const int head = unit / row_tiles, rt = unit % row_tiles, r = blockIdx.y;
+  if (r >= min(16, rep - rt * 16)) return;
+  auto slot = [&](int x) { return x == c - 1 ? 2 * (c - 1) + 1 : 2 * x; };
+  float big = -INFINITY;
+  for (int x = c - 1; x <= last; ++x) big = fmaxf(big, a.part_ml[(slot(x) * 16 + r) * 2]);
+  T* out = static_cast<T*>(a.out) + ((int64_t)place.row * a.nq + head * rep + rt * 16 + r) * D;
+  for (int d = threadIdx.x; d < D; d += kThreads) {
+    float num = 0.f, den = 0.f;
+#pragma unroll 4
+    for (int x = c - 1; x <= last; ++x) {
+      const int s = slot(x) * 16 + r;
+      const float part = a.part_ml[s * 2 + 1];
+      const float w = part == 0.f ? 0.f : exp2_approx(a.part_ml[s * 2] - big);
+      if (w != 0.f) num += w * a.part_o[(int64_t)s * D + d];
+      den += w * part;
+    }
+    out[d] = from_float<T>(den == 0.f ? 0.f : num / den);
+  }
+}
+
+// tokens that every query row sees, and its sequence: trailing q_len tokens of each sequence, causal
+__global__ void __launch_bounds__(kThreads)
+q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B, int T, int* __restrict__ row_seq, int* __restrict__ row_len) {
+  pdl_trigger();
+  pdl_wait();
+  __shared__ int sh[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  // rows before this block's sequence
+  const int b = blockIdx.x;
+  int before = 0;
+  for (int i = tid; i < b; i += kThreads) before += max(news[i], 0);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  if (lane == 0) sh[warp] = before;
+  __syncthreads();
+  before = sh[0] + sh[1] + sh[2] + sh[3];
+  if (b == B) {                                    // rows behind the last sequence
+    for (int r = before + tid; r < T; r += kThreads) { row_seq[r] = 0; row_len[r] = 0; }
+    return;
+  }
+  const int n = max(news[b], 0);
+  for (int i = tid; i < n && before + i < T; i += kThreads) {
+    row_seq[before + i] = b;
+    row_len[before + i] = max(lens[b] - n + 1 + i, 0);
+  }
+}
+
+template <typename T, int D>
+void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
+  constexpr int ST = D == 64 ? 6 : D == 128 ? 4 : 3;
+  const int rep = a.nq / a.nkv, row_tiles = (rep + 15) / 16, red_rows = std::min(rep, 16);
+  auto smem_of = [](int rows) { return sizeof(WarpRing<D, ST>) * kWarps + 2 * rows * D * sizeof(float); };
+  const size_t smem = smem_of(red_rows);
+  static std::atomic<int> residents[64][17] = {};  // blocks that an SM holds, per device and rows of a unit
+  const int dev = q.get_device();
+  TORCH_CHECK(dev >= 0 && dev < 64, "paged_attention_q8: device index out of range");
+  int resident = residents[dev][red_rows].load();
+  if (!resident) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(paged_q8_kernel<T, D, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(16)));
+    C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, paged_q8_kernel<T, D, ST>, kThreads, smem));
+    resident = std::max(resident, 1);
+    residents[dev][red_rows].store(resident);
+  }
+  const int64_t most = (int64_t)a.rows * a.nkv * row_tiles * (((int64_t)a.width * a.bs + kTile - 1) / kTile);
+  a.grid = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)resident * at::cuda::getCurrentDeviceProperties()->multiProcessorCount, most));
+  auto part_o = at::empty({2 * a.grid, 16, D}, q.options().dtype(at::kFloat));
+  auto part_ml = at::empty({2 * a.grid, 16, 2}, q.options().dtype(at::kFloat));
+  a.part_o = part_o.data_ptr<float>();
+  a.part_ml = part_ml.data_ptr<float>();
+  C10_CUDA_CHECK(launch_pdl(paged_q8_kernel<T, D, ST>, dim3(a.grid), dim3(kThreads), smem, st, a));
+  if (a.grid > 1)
+    C10_CUDA_CHECK(launch_pdl(paged_q8_join_kernel<T, D>, dim3(a.grid - 1, std::min(rep, 16)), dim3(kThreads), 0, st, a));
+}
+
+}  // namespace
+
+at::Tensor paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+                              const at::Tensor& vs, const at::Tensor& tables, const at::Tensor& lens,
+                              const c10::optional<at::Tensor>& news, double scale) {
+  const c10::cuda::CUDAGuard guard(q.device());
+  Args a = {};
+  const int D = (int)q.size(2);
+  auto out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
+  if (q.size(0) == 0) return out;
+  a.q = q.data_ptr(); a.q_row = q.stride(0);
+  a.kc = (const uint8_t*)kc.data_ptr(); a.vc = (const uint8_t*)vc.data_ptr();
+  a.ks = ks.data_ptr<float>(); a.vs = vs.data_ptr<float>();
+  a.tables = tables.data_ptr<int>();
+  a.out = out.data_ptr();
+  a.T = (int)q.size(0); a.nq = (int)q.size(1); a.nkv = (int)kc.size(1); a.bs = (int)kc.size(2); a.pages = kc.size(0);
+  a.width = (int)tables.size(1);
+  a.scale = (float)(scale * 1.4426950408889634);
+  auto st = at::cuda::getCurrentCUDAStream();
+  const int B = (int)lens.size(0);
+  at::Tensor row_seq, row_len;
+  if (news.has_value()) {
+    row_seq = at::empty({a.T}, lens.options());
+    row_len = at::empty({a.T}, lens.options());
+    a.rows = a.T;
+    C10_CUDA_CHECK(launch_pdl(q8_rows_kernel, dim3(B + 1), dim3(kThreads), 0, st, (const int*)lens.data_ptr<int>(),
+                              (const int*)news->data_ptr<int>(), B, a.T, row_seq.data_ptr<int>(), row_len.data_ptr<int>()));
+    a.row_seq = row_seq.data_ptr<int>();
+    a.row_len = row_len.data_ptr<int>();
+  } else {
+    a.rows = std::min(a.T, B);
+    a.row_len = lens.data_ptr<int>();
+  }
+  const bool bf = q.scalar_type() == at::kBFloat16;
+  if (D == 64) bf ? launch_q8<__nv_bfloat16, 64>(a, q, st) : launch_q8<__half, 64>(a, q, st);
+  else if (D == 128) bf ? launch_q8<__nv_bfloat16, 128>(a, q, st) : launch_q8<__half, 128>(a, q, st);
+  else bf ? launch_q8<__nv_bfloat16, 256>(a, q, st) : launch_q8<__half, 256>(a, q, st);
+  return out;
+}

@@ -1,0 +1,466 @@
+// Log-probability of given tokens, entropy of their distribution and its n likeliest alternatives, from logits, and the
+// gradient of all three.
+//
+// With M = max z, x_j = (z_j - M) log2(e) / temperature, S = sum 2^x, X = sum 2^x x, everything in one pass:
+//   logprob = (z_tok - M) / temperature - ln S,   entropy = (log2 S - X / S) ln 2
+// (all relative to the maximum: no difference of two large numbers, and no overflow of logits at the type's lowest value).
+//
+// Alternatives without a second pass over the row: a warp notes the maximum of each stretch of the row that it reads
+// (512 or 1024 logits).  At most n stretches hold the n largest logits, namely those with the n largest maxima, and the
+// n-th largest maximum bounds the n-th largest logit from below; so the candidates are the logits of n stretches that
+// reach that bound, about n of them.  Order: larger logit first, then lower index.
+//
+// A row is read by a cluster of 1 to 8 blocks; their sums and lists meet in the first block's shared memory.
+#include <ATen/core/Tensor.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cooperative_groups.h>
+
+#include "q8.cuh"
+
+using namespace cl;
+namespace cg = cooperative_groups;
+
+namespace {
+
+constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kMaxTop = 64;
+constexpr int kUnroll = 4;                        // vectors of 16 bytes a lane loads at once
+constexpr int kMaxStretch = 512;                  // stretches of a block
+constexpr int kCand = 2304;                       // n (n + 1) / 2 candidates when all logits are equal, and room
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kFar = -1000.f;                   // 2^kFar is 0: -inf logits stay out of 0 * inf
+
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+// unique key: larger logit first, then lower index; NaN counts as -inf, -0 as 0
+__device__ __forceinline__ uint64_t key_of(float v, int idx) {
+  v = v == v ? v + 0.f : -INFINITY;
+  const uint32_t b = __float_as_uint(v);
+  return (uint64_t)(b & 0x80000000u ? ~b : b | 0x80000000u) << 32 | (uint32_t)(~idx);
+}
+__device__ __forceinline__ float value_of(uint64_t key) {
+  const uint32_t b = (uint32_t)(key >> 32);
+  return __uint_as_float(b & 0x80000000u ? b & 0x7fffffffu : ~b);
+}
+__device__ __forceinline__ int index_of(uint64_t key) { return (int)~(uint32_t)key; }
+
+template <typename T> struct Wide { static constexpr int N = 16 / sizeof(T); };
+
+template <typename T>
+__device__ __forceinline__ void load16(const T* p, float* f) {
+  const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+  const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int i = 0; i < Wide<T>::N; ++i) f[i] = q8::to_float(t[i]);
+}
+
+struct Sums { float m, s, x; };                   // M, S, X
+__device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
+  Sums r;
+  r.m = fmaxf(a.m, b.m);
+  if (r.m == -INFINITY) { r.s = a.s + b.s; r.x = a.x + b.x; return r; }   // 0, or NaN
+  const float da = fmaxf((a.m - r.m) * c, kFar), db = fmaxf((b.m - r.m) * c, kFar);
+  const float ea = exp2_approx(da), eb = exp2_approx(db);
+  r.s = a.s * ea + b.s * eb;
+  r.x = ea * (a.x + a.s * da) + eb * (b.x + b.s * db);
+  return r;
+}
+
+struct Shared {
+  float stretch[kMaxStretch];
+  uint64_t cand[kCand];
+  uint64_t best[8 * kMaxTop];                     // the cluster's lists, in the first block
+  int chosen[kMaxTop];
+  Sums warp_sums[kWarps];
+  Sums sums;
+  uint64_t round;
+  float bound;
+  int count;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 2)
+token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t* __restrict__ tokens, int V, int n, float c,
+                     float inv_temp, float* __restrict__ lp, float* __restrict__ ent, float* __restrict__ stats, float* __restrict__ top_lp,
+                     int64_t* __restrict__ top_id) {
+  __shared__ Shared sh;
+  constexpr int N = Wide<T>::N;
+  pdl_trigger();
+  pdl_wait();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+  const int64_t row = blockIdx.x / parts;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const T* z = logits + row * stride;
+  // 16-byte vectors from the first aligned element on; what is in front and behind them belongs to the first block
+  const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+  const int head = min(V, mis ? N - mis : 0), vecs = (V - head) / N, tail = head + vecs * N;
+  const T* body = z + head;
+  const int batches = (vecs + 32 * kUnroll - 1) / (32 * kUnroll);
+  const int b0 = (int)((int64_t)part * batches / parts), b1 = (int)((int64_t)(part + 1) * batches / parts);
+  const int per = max(1, (b1 - b0 + kMaxStretch - 1) / kMaxStretch);          // batches of a stretch
+  const int stretches = (b1 - b0 + per - 1) / per;
+
+  // ---- the pass over the row
+  Sums a{-INFINITY, 0.f, 0.f};                     // m is the warp's
+  auto take = [&](const float* f, int count) {
+    const float ref = a.m == -INFINITY ? 0.f : a.m;
+#pragma unroll
+    for (int i = 0; i < N * kUnroll; ++i)
+      if (i < count) {
+        const float x = max_nan((f[i] - ref) * c, kFar), e = exp2_approx(x);
+        a.s += e;
+        a.x = fmaf(e, x, a.x);
+      }
+  };
+  auto raise = [&](float y) {                      // a new warp maximum
+    if (y > a.m) {
+      if (a.m != -INFINITY) {
+        const float d = fmaxf((a.m - y) * c, kFar), e = exp2_approx(d);
+        a.x = e * (a.x + a.s * d);
+        a.s *= e;
+      }
+      a.m = y;
+    }
+  };
+  for (int s = warp; s < stretches; s += kWarps) {
+    float most = -INFINITY;
+    const int e1 = min(b0 + (s + 1) * per, b1);
+    for (int b = b0 + s * per; b < e1; ++b) {
+      float f[N * kUnroll];
+      const int v0 = b * 32 * kUnroll + lane;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        if (v0 + u * 32 < vecs) load16(body + (int64_t)(v0 + u * 32) * N, f + u * N);
+        else
+#pragma unroll
+          for (int i = 0; i < N; ++i) f[u * N + i] = -INFINITY;
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < N * kUnroll; ++i) mx = fmaxf(mx, f[i]);
+      mx = warp_max(mx);
+      raise(mx);
+      most = fmaxf(most, mx);
+      take(f, N * kUnroll);
+    }
+    if (lane == 0) sh.stretch[s] = most;
+  }
+  if (part == 0 && warp == kWarps - 1) {           // the unaligned ends
+    float f[N * kUnroll];
+    f[0] = lane < head ? q8::to_float(z[lane]) : lane >= 16 && tail + lane - 16 < V ? q8::to_float(z[tail + lane - 16]) : -INFINITY;
+    raise(warp_max(f[0]));
+    take(f, 1);
+  }
+  a.s = warp_sum(a.s);
+  a.x = warp_sum(a.x);
+  if (lane == 0) sh.warp_sums[warp] = a;
+  if (tid == 0) { sh.count = 0; sh.bound = -INFINITY; }
+  __syncthreads();
+  if (tid == 0) {
+    Sums t = sh.warp_sums[0];
+    for (int w = 1; w < kWarps; ++w) t = join(t, sh.warp_sums[w], c);
+    sh.sums = t;
+  }
+
+  // ---- the block's n best
+  if (n > 0) {
+    // the n stretches with the largest maxima, and the bound
+    if (tid < stretches) {
+      const float v = sh.stretch[tid];
+      int rank = 0;
+      for (int j = 0; j < stretches; ++j) {
+        const float w = sh.stretch[j];
+        rank += w > v || (w == v && j < tid);
+      }
+      if (rank < n) sh.chosen[rank] = tid;
+      if (rank == n - 1) sh.bound = v;
+    }
+    __syncthreads();
+    const float bound = sh.bound;
+    const int chosen = min(n, stretches);
+    auto push = [&](float v, int idx) {
+      const int at = atomicAdd(&sh.count, 1);
+      if (at < kCand) sh.cand[at] = key_of(v, idx);
+    };
+    for (int r = warp; r < chosen; r += kWarps) {
+      const int s = sh.chosen[r];
+      int equal = 0;                               // logits equal to the bound so far; no more than n - r can matter
+      const int e1 = min(b0 + (s + 1) * per, b1);
+      for (int v = (b0 + s * per) * 32 * kUnroll + lane; v - lane < min(e1 * 32 * kUnroll, vecs); v += 32) {
+        float f[N];
+        int mine = 0;
+        if (v < vecs) {
+          load16(body + (int64_t)v * N, f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            f[i] = f[i] == f[i] ? f[i] : -INFINITY;
+            mine += f[i] == bound;
+            if (f[i] > bound) push(f[i], head + v * N + i);
+          }
+        }
+        if (__any_sync(0xffffffffu, mine > 0)) {
+          int inc = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int p = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += p;
+          }
+          int at = equal + inc - mine;
+          if (mine > 0)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+              if (f[i] == bound) {
+                if (at < n - r) push(f[i], head + v * N + i);
+                ++at;
+              }
+          equal += __shfl_sync(0xffffffffu, inc, 31);
+        }
+      }
+    }
+    if (part == 0 && warp == kWarps - 1) {
+      if (lane < head) push(q8::to_float(z[lane]), lane);
+      if (lane >= 16 && tail + lane - 16 < V) push(q8::to_float(z[tail + lane - 16]), tail + lane - 16);
+    }
+    for (int i = tid; i < n; i += kThreads) sh.best[i] = 0;
+    __syncthreads();
+    const int count = sh.count;
+    if (count <= kCand) {
+      for (int i = tid; i < count; i += kThreads) {
+        const uint64_t k = sh.cand[i];
+        int rank = 0;
+        for (int j = 0; j < count; ++j) rank += sh.cand[j] > k;
+        if (rank < n) sh.best[rank] = k;
+      }
+      __syncthreads();
+    } else {
+      // thousands of logits of few stretches above the bound (ascending rows, for one): n rounds of the largest key
+      // below the last one, over the chosen stretches
+      uint64_t last = ~0ull;
+      for (int k = 0; k < n; ++k) {
+        uint64_t mine = 0;
+        auto see = [&](float v, int idx) {
+          const uint64_t x = key_of(v, idx);
+          if (x < last && x > mine) mine = x;
+        };
+        for (int r = warp; r < chosen; r += kWarps) {
+          const int s = sh.chosen[r], e1 = min(b0 + (s + 1) * per, b1);
+          for (int v = (b0 + s * per) * 32 * kUnroll + lane; v < min(e1 * 32 * kUnroll, vecs); v += 32) {
+            float f[N];
+            load16(body + (int64_t)v * N, f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) see(f[i], head + v * N + i);
+          }
+        }
+        if (part == 0 && warp == kWarps - 1) {
+          if (lane < head) see(q8::to_float(z[lane]), lane);
+          if (lane >= 16 && tail + lane - 16 < V) see(q8::to_float(z[tail + lane - 16]), tail + lane - 16);
+        }
+        if (tid == 0) sh.round = 0;
+        __syncthreads();
+        if (mine) atomicMax(reinterpret_cast<unsigned long long*>(&sh.round), (unsigned long long)mine);
+        __syncthreads();
+        last = sh.round;
+        if (tid == 0) sh.best[k] = last;
+        __syncthreads();
+      }
+    }
+  }
+
+  // ---- the cluster's parts meet in its first block
+  if (parts > 1) {
+    cluster.sync();
+    if (part == 0) {
+      uint64_t k = 0;
+      const int total = parts * n;                 // at most 512: one key a thread
+      if (tid < total) k = cluster.map_shared_rank(&sh, tid / n)->best[tid % n];
+      Sums t = sh.sums;
+      if (tid == 0)
+        for (int p = 1; p < parts; ++p) t = join(t, cluster.map_shared_rank(&sh, p)->sums, c);
+      __syncthreads();                             // the own list has been read
+      if (tid == 0) sh.sums = t;
+      if (tid < total) sh.cand[tid] = k;
+      __syncthreads();
+      if (tid < total && k) {
+        int rank = 0;
+        for (int j = 0; j < total; ++j) rank += sh.cand[j] > k;
+        if (rank < n) sh.best[rank] = k;
+      }
+      __syncthreads();
+    }
+    cluster.sync();                                // the others' shared memory is read no more
+    if (part != 0) return;
+  } else {
+    __syncthreads();
+  }
+  const Sums t = sh.sums;
+  const bool empty = t.m == -INFINITY && t.s == 0.f;                          // nothing but -inf
+  const float ls = log2f(t.s);
+  auto logprob = [&](float v) { return empty ? -INFINITY : fmaf(v - t.m, inv_temp, -ls * kLn2); };
+  if (tid == 0) {
+    const int64_t tok = tokens[row];
+    lp[row] = tok >= 0 && tok < V ? logprob(q8::to_float(z[tok])) : 0.f;
+    ent[row] = empty ? 0.f : (ls - t.x / t.s) * kLn2;
+    stats[2 * row] = t.m;
+    stats[2 * row + 1] = ls;
+  }
+  if (tid < n) {
+    const uint64_t k = sh.best[tid];
+    top_lp[row * n + tid] = logprob(value_of(k));
+    top_id[row * n + tid] = index_of(k);
+  }
+}
+
+// dz_j = 1/temperature [ g_lp d(j = token) + sum_k g_top_k d(j = top_k) - p_j (g_lp + sum_k g_top_k) - g_ent p_j (ln p_j + H) ]
+// One read of the logits, one write of the gradient; the columns of the token and the alternatives are written again
+// after the stretch that holds them.
+constexpr int kGradThreads = 256;
+constexpr int kGradSpan = 16384;                  // bytes of a row that a block handles
+
+template <typename T>
+__global__ void __launch_bounds__(kGradThreads)
+token_logprob_grad_kernel(const T* __restrict__ logits, int64_t stride, const int64_t* __restrict__ tokens, int V, int n,
+                          int spans, float c, float inv_temp, const float* __restrict__ ent, const float* __restrict__ stats,
+                          const int64_t* __restrict__ top_id, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
+                          const float* __restrict__ g_top, T* __restrict__ dz, int64_t dz_stride) {
+  __shared__ float sh_sum;
+  constexpr int N = Wide<T>::N;
+  pdl_trigger();
+  pdl_wait();
+  const int64_t row = blockIdx.x / spans;
+  const int span = (int)(blockIdx.x % spans), tid = threadIdx.x, lane = tid & 31;
+  const T* z = logits + row * stride;
+  T* d = dz + row * dz_stride;
+  const int64_t tok = tokens[row];
+  const float M = stats[2 * row], ls = stats[2 * row + 1], H = ent[row];
+  const bool empty = M == -INFINITY && ls == -INFINITY;                       // log2 of an empty sum
+  const float gl = g_lp && tok >= 0 && tok < V ? g_lp[row] : 0.f, ge = g_ent ? g_ent[row] : 0.f;
+  if (tid < 32) {
+    float s = 0.f;
+    if (g_top)
+      for (int i = lane; i < n; i += 32) s += g_top[row * n + i];
+    s = warp_sum(s);
+    if (lane == 0) sh_sum = s;
+  }
+  __syncthreads();
+  // p (A x + B) with x = log2 p
+  const float A = -inv_temp * ge * kLn2, B = -inv_temp * (gl + sh_sum + ge * H);
+  auto grad = [&](float v) {
+    const float x = max_nan(fmaf(v - M, c, -ls), kFar);
+    return empty ? 0.f : exp2_approx(x) * fmaf(x, A, B);
+  };
+  const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+  const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+  // both rows at the same place inside 16 bytes: vectors; else single elements
+  const int head = same ? min(V, mis ? N - mis : 0) : 0, vecs = same ? (V - head) / N : 0, tail = head + vecs * N;
+  constexpr int kVecs = kGradSpan / 16;
+  const int v0 = span * kVecs, v1 = min(v0 + kVecs, vecs);
+  int lo, hi;                                      // columns of this block
+  if (same) {
+    lo = span == 0 ? 0 : head + v0 * N;
+    hi = span == spans - 1 ? V : min(V, head + (v0 + kVecs) * N);
+    if (span == 0 && tid < head) d[tid] = q8::from_float<T>(grad(q8::to_float(z[tid])));
+    for (int v = v0 + tid; v < v1; v += kGradThreads) {
+      float f[N];
+      load16(z + head + (int64_t)v * N, f);
+      uint4 u;
+      T* o = reinterpret_cast<T*>(&u);
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[i] = q8::from_float<T>(grad(f[i]));
+      *reinterpret_cast<uint4*>(d + head + (int64_t)v * N) = u;
+    }
+    if (span == spans - 1)
+      for (int i = tail + tid; i < V; i += kGradThreads) d[i] = q8::from_float<T>(grad(q8::to_float(z[i])));
+  } else {
+    lo = min(V, span * kVecs * N);
+    hi = span == spans - 1 ? V : min(V, lo + kVecs * N);
+    for (int i = lo + tid; i < hi; i += kGradThreads) d[i] = q8::from_float<T>(grad(q8::to_float(z[i])));
+  }
+  __syncthreads();
+  if (tid <= n && !empty) {                        // thread n: the token; an alternative that is the token is its job
+    const int64_t col = tid < n ? top_id[row * n + tid] : tok;
+    if (col >= lo && col < hi && !(tid < n && col == tok)) {
+      float add = tid < n ? (g_top ? g_top[row * n + tid] : 0.f) : gl;
+      if (tid == n && g_top)
+        for (int i = 0; i < n; ++i)
+          if (top_id[row * n + i] == tok) add += g_top[row * n + i];
+      d[col] = q8::from_float<T>(fmaf(add, inv_temp, grad(q8::to_float(z[col]))));
+    }
+  }
+}
+
+// blocks that share a row
+int cluster_for(int64_t rows) {
+  int parts = 1;
+  while (parts < 8 && rows * parts * 2 <= 2 * 148) parts *= 2;
+  return parts;
+}
+
+}  // namespace
+
+std::vector<at::Tensor> token_logprob_fwd(const at::Tensor& z, const at::Tensor& tokens, int64_t n, double inv_temp) {
+  const c10::cuda::CUDAGuard guard(z.device());
+  TORCH_CHECK(n >= 0 && n <= kMaxTop, "token_logprobs: at most 64 alternatives");
+  const int64_t R = z.size(0), V = z.size(1);
+  auto f = z.options().dtype(at::kFloat);
+  auto lp = at::empty({R}, f), ent = at::empty({R}, f), stats = at::empty({R, 2}, f), top = at::empty({R, n}, f);
+  auto ids = at::empty({R, n}, z.options().dtype(at::kLong));
+  if (R == 0) return {lp, ent, top, ids, stats};
+  const int parts = cluster_for(R);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(R * parts)); cfg.blockDim = dim3(kThreads); cfg.stream = at::cuda::getCurrentCUDAStream();
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  const float c = (float)(inv_temp * 1.4426950408889634);
+#define LAUNCH(T)                                                                                                        \
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, token_logprob_kernel<T>, (const T*)z.data_ptr(), z.stride(0),                   \
+                                    (const int64_t*)tokens.data_ptr<int64_t>(), (int)V, (int)n, c, (float)inv_temp, lp.data_ptr<float>(),  \
+                                    ent.data_ptr<float>(), stats.data_ptr<float>(), top.data_ptr<float>(), ids.data_ptr<int64_t>()))
+  if (z.scalar_type() == at::kFloat) LAUNCH(float);
+  else if (z.scalar_type() == at::kHalf) LAUNCH(__half);
+  else LAUNCH(__nv_bfloat16);
+#undef LAUNCH
+  return {lp, ent, top, ids, stats};
+}
+
+at::Tensor token_logprob_bwd(const at::Tensor& z, const at::Tensor& tokens, const at::Tensor& ent, const at::Tensor& stats,
+                             const at::Tensor& ids, const c10::optional<at::Tensor>& g_lp, const c10::optional<at::Tensor>& g_ent,
+                             const c10::optional<at::Tensor>& g_top, double inv_temp) {
+  const c10::cuda::CUDAGuard guard(z.device());
+  const int64_t R = z.size(0), V = z.size(1), n = ids.size(1);
+  // rows at the places that the logits' rows have inside 16 bytes, so that both go in vectors (a little padding stays)
+  const int64_t stride = z.stride(0) >= V && z.stride(0) - V <= 128 ? z.stride(0) : V;
+  auto dz = at::empty({R, stride}, z.options()).narrow(1, 0, V);
+  if (R == 0 || V == 0) return dz;
+  const int esize = (int)z.element_size();
+  const int spans = (int)((V * esize + kGradSpan - 1) / kGradSpan);
+  auto ptr = [](const c10::optional<at::Tensor>& t) { return t.has_value() && t->numel() ? (const float*)t->data_ptr<float>() : nullptr; };
+  const float c = (float)(inv_temp * 1.4426950408889634);
+  auto st = at::cuda::getCurrentCUDAStream();
+#define LAUNCH(T)                                                                                                          \
+  C10_CUDA_CHECK(launch_pdl(token_logprob_grad_kernel<T>, dim3((unsigned)(R * spans)), dim3(kGradThreads), 0, st,           \
+                            (const T*)z.data_ptr(), z.stride(0), (const int64_t*)tokens.data_ptr<int64_t>(), (int)V, (int)n, \
+                            spans, c, (float)inv_temp, (const float*)ent.data_ptr<float>(), (const float*)stats.data_ptr<float>(), \
+                            (const int64_t*)ids.data_ptr<int64_t>(), ptr(g_lp), ptr(g_ent), ptr(g_top), (T*)dz.data_ptr(), dz.stride(0)))
+  if (z.scalar_type() == at::kFloat) LAUNCH(float);
+  else if (z.scalar_type() == at::kHalf) LAUNCH(__half);
+  else LAUNCH(__nv_bfloat16);
+#undef LAUNCH
+  return dz;
+}

@@ -13,6 +13,7 @@ from collections import Counter
 import torch
 
 from . import reference as ref
+from .q8 import Q8KVCache, TokenLogprobs  # noqa: F401
 
 _MODE = "native"
 _NATIVE = {}
@@ -95,6 +96,9 @@ attention_segments = _dispatch("attention_segments")
 kv_append = _dispatch("kv_append")
 paged_attention = _dispatch("paged_attention")
 mla_paged_decode = _dispatch("mla_paged_decode")
+kv_append_q8 = _dispatch("kv_append_q8")
+paged_attention_q8 = _dispatch("paged_attention_q8")
+token_logprobs = _dispatch("token_logprobs")
 lmhead_logprob_entropy = _dispatch("lmhead_logprob_entropy")
 grpo_loss_fused = _dispatch("grpo_loss_fused")
 gspo_loss_fused = _dispatch("gspo_loss_fused")

@@ -611,3 +611,4 @@ for _name, _fn in (("rmsnorm", rmsnorm), ("add_rmsnorm_", add_rmsnorm_), ("swigl
 
 from . import native_moe  # noqa: E402,F401  (registers the mixture-of-experts ops)
 from . import native_attn  # noqa: E402,F401  (registers the packed attention forward)
+from . import native_q8  # noqa: E402,F401  (registers the 8-bit cache ops and the token statistics)

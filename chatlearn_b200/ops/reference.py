@@ -12,6 +12,8 @@ from typing import Optional, Tuple
 import torch
 import torch.nn.functional as F
 
+from . import q8
+
 
 # ------------------------------------------------------------------ norms / act
 def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float) -> torch.Tensor:
@@ -252,6 +254,102 @@ def paged_attention(q, k_cache, v_cache, block_tables, seq_lens, q_lens=None, sc
     return torch.cat(outs, 0)
 
 
+# ------------------------------------------------------------------ 8-bit KV cache
+def _q8_rows(seq_lens, q_lens, rows):
+    """(sequence, position) of every packed new row."""
+    ql = [min(1, max(n, 0)) for n in seq_lens.tolist()] if q_lens is None else [max(n, 0) for n in q_lens.tolist()]
+    out, at = [], 0
+    for b, (L, n) in enumerate(zip(seq_lens.tolist(), ql)):
+        if q_lens is None:
+            at = b
+        out.append((b, L, n, at))
+        at += n
+    return out
+
+
+def q8_scale(amax):
+    """The smallest power of two s in [2^-24, 2^64] with ``amax <= 448 s``."""
+    m, _ = torch.frexp(amax)                    # amax = m 2^e, 0.5 <= m < 1: amax / m is exact
+    s = torch.where(m > 0, amax / m, torch.zeros_like(amax)) * torch.where(m <= 0.875, 2.0 ** -9, 2.0 ** -8)
+    return s.clamp(q8.SCALE_MIN, q8.SCALE_MAX)
+
+
+@torch.no_grad()
+def kv_append_q8(k, v, cache, block_tables, seq_lens, q_lens=None):
+    """Write the new rows ``k, v [rows, kv heads, head dim]`` of every sequence into the paged 8-bit
+    ``cache`` (``ops.Q8KVCache``, in place); tables and lengths as in ``ops.q8``.
+
+    A page's scale is the smallest power of two that holds its largest finite value; it grows when new
+    rows need it (the page's older codes are then rounded again under the grown scale) and starts over
+    when a page is written from its first token.  Infinite values saturate, NaN stays NaN."""
+    q8.check_append(k, v, cache, block_tables, seq_lens, q_lens)
+    pages, _, bs, _ = cache.k.shape
+    table = block_tables.tolist()
+    for x, codes, scale in ((k, cache.k, cache.k_scale), (v, cache.v, cache.v_scale)):
+        raw = codes.view(torch.uint8)
+        for b, L, n, at in _q8_rows(seq_lens, q_lens, k.shape[0]):
+            pos = max(L - n, 0)
+            at += pos - (L - n)
+            while pos < L:
+                m = min(bs - pos % bs, L - pos, k.shape[0] - at)
+                if m <= 0 or pos // bs >= len(table[b]):
+                    break
+                page, off = table[b][pos // bs], pos % bs
+                if 0 <= page < pages:
+                    part = x[at:at + m].float().transpose(0, 1)                     # [nkv, m, D]
+                    size = part.abs()
+                    s = q8_scale(torch.where(size < math.inf, size, torch.zeros_like(size)).amax((1, 2)))
+                    if off > 0:
+                        s = torch.maximum(s, scale[page])
+                        old = raw[page, :, :off].view(codes.dtype).float()
+                        ratio = (scale[page] / s)[:, None, None]
+                        kept = torch.where(ratio < 1, old * ratio, old)
+                        raw[page, :, :off] = kept.to(codes.dtype).view(torch.uint8)
+                    scale[page] = s
+                    new = (part / s[:, None, None]).clamp(-q8.CODE_MAX, q8.CODE_MAX)
+                    raw[page, :, off:off + m] = new.to(codes.dtype).contiguous().view(torch.uint8)
+                pos, at = pos + m, at + m
+
+
+@torch.no_grad()
+def paged_attention_q8(q, cache, block_tables, seq_lens, q_lens=None, scale=None):
+    """Attention of the new queries ``q [rows, query heads, head dim]`` over the paged 8-bit ``cache``
+    (their keys and values already appended), causal inside a sequence's new tokens; tables and lengths
+    as in ``ops.q8``.  Rows that see nothing, and rows behind the last sequence, are zero.  Inference only."""
+    q8.check_attend(q, cache, block_tables, seq_lens, q_lens)
+    T, nq, D = q.shape
+    pages, nkv, bs, _ = cache.k.shape
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    out = torch.zeros(T, nq, D, dtype=wide, device=q.device)
+    for b, L, n, at in _q8_rows(seq_lens, q_lens, T):
+        n_in = min(n, T - at)
+        seen = min(L, block_tables.shape[1] * bs)
+        if n_in <= 0 or seen <= 0:
+            continue
+        ids = block_tables[b, :(seen + bs - 1) // bs].long()
+        good = ((ids >= 0) & (ids < pages)).repeat_interleave(bs)[:seen]
+        ids = ids.clamp(0, pages - 1)
+        kk = (cache.k.view(torch.uint8)[ids].view(cache.k.dtype).to(wide) * cache.k_scale[ids].to(wide)[:, :, None, None])
+        vv = (cache.v.view(torch.uint8)[ids].view(cache.v.dtype).to(wide) * cache.v_scale[ids].to(wide)[:, :, None, None])
+        kk = kk.transpose(0, 1).reshape(nkv, -1, D)[:, :seen]
+        vv = vv.transpose(0, 1).reshape(nkv, -1, D)[:, :seen]
+        pos = torch.arange(L - n, L - n + n_in, device=q.device)
+        mask = (torch.arange(seen, device=q.device)[None, :] <= pos[:, None]) & good[None, :]      # [n, seen]
+        qq = q[at:at + n_in].to(wide).view(n_in, nkv, nq // nkv, D)
+        # what no query of the row sees may be anything (NaN codes behind the end): it stays out of the products
+        used = mask.any(0)
+        kk = torch.where(used[None, :, None], kk, torch.zeros_like(kk))
+        vv = torch.where(used[None, :, None], vv, torch.zeros_like(vv))
+        s = torch.einsum("nhrd,hld->hrnl", qq, kk) * scale
+        s = s.masked_fill(~mask, -math.inf)
+        some = mask.any(-1)[None, None, :, None]
+        p = torch.where(some, s, torch.zeros_like(s)).softmax(-1)
+        p = torch.where(some & mask, p, torch.zeros_like(p))
+        out[at:at + n_in] = torch.einsum("hrnl,hld->nhrd", p, vv).reshape(n_in, nq, D)
+    return out.to(q.dtype)
+
+
 # ------------------------------------------------------------------ lm head
 class _LMHeadLogprob(torch.autograd.Function):
     """log p(label), entropy without keeping ``[T, V]`` logits: rows are processed
@@ -308,6 +406,32 @@ def entropy_from_logits(logits):
     z = logits.float()
     lse = torch.logsumexp(z, -1)
     return lse - (torch.softmax(z, -1) * z).sum(-1)
+
+
+def token_logprobs(logits, tokens, top_n: int = 0, temperature: float = 1.0):
+    """Log-probability of ``tokens [rows]`` under ``softmax(logits / temperature)``, the entropy, and the
+    ``top_n`` likeliest tokens with their log-probabilities (most likely first, equal logits by the lower
+    index), as ``ops.TokenLogprobs``; fp32, differentiable in the logits.
+
+    A token outside the vocabulary (-1, say) has log-probability 0 and no gradient.  Logits of -inf are
+    tokens that cannot occur; a row of nothing else has entropy 0, log-probabilities of -inf and no
+    gradient.  NaN ranks as -inf."""
+    q8.check_token_logprobs(logits, tokens, top_n, temperature)
+    wide = torch.float64 if logits.dtype == torch.float64 else torch.float32
+    raw = logits.to(wide)
+    order = torch.where(raw.detach().isnan(), torch.full_like(raw, -math.inf), raw.detach())
+    ids = torch.sort(order, dim=1, descending=True, stable=True).indices[:, :top_n].contiguous()
+    empty = (raw.detach() == -math.inf).all(1)
+    z = torch.where(empty[:, None], torch.zeros_like(raw), raw) * (1.0 / temperature)
+    logp = torch.log_softmax(z, -1)
+    safe = logp.masked_fill(z.detach() == -math.inf, 0.0)
+    entropy = -(logp.exp() * safe).sum(-1)
+    has = (tokens >= 0) & (tokens < logits.shape[1])
+    lp = logp.gather(1, tokens.long().clamp(0, logits.shape[1] - 1)[:, None]).squeeze(1)
+    none = torch.full_like(lp, -math.inf)
+    lp = torch.where(has, torch.where(empty, none, lp), torch.zeros_like(lp))
+    top = torch.where(empty[:, None], none[:, None], logp.gather(1, ids))
+    return q8.TokenLogprobs(lp, torch.where(empty, torch.zeros_like(entropy), entropy), top, ids)
 
 
 # ------------------------------------------------------------------ RL losses
