@@ -133,19 +133,36 @@ __device__ __forceinline__ int swizzled(int r, int chunk) {
   return chunk ^ ((r >> 1) & 3);
 }
 
-// A warp's position on the line.
+// A warp's position on the line: row set, kv head and row tile of it, tile; the page that holds the warp's 16 tokens.
 struct Cursor {
-  int row, unit, tile, tiles, len;               // row set, unit of it (kv head, row tile), tile, the row's tiles and tokens
+  int row, head, rt, tile, tiles, len;
+  int page, off;                                 // number in the sequence's table, token inside the page
+  const int* table;
+  __device__ __forceinline__ void rewind(const Args& a, int warp) {      // to token `tile * kTile + 16 * warp`
+    const int tok = tile * kTile + warp * 16;
+    page = tok / a.bs;
+    off = tok - page * a.bs;
+  }
   __device__ __forceinline__ void enter(const Args& a, int r) {
     row = r;
+    tiles = 0;
     while (row < a.rows && (tiles = tiles_of(a, row)) == 0) ++row;
-    len = row < a.rows ? min(a.row_len[row], a.width * a.bs) : 0;
+    if (row >= a.rows) return;
+    len = min(a.row_len[row], a.width * a.bs);
+    table = a.tables + (int64_t)(a.row_seq ? a.row_seq[row] : row) * a.width;
   }
-  __device__ __forceinline__ void next(const Args& a, int per_row) {
-    if (++tile < tiles) return;
+  __device__ __forceinline__ void next(const Args& a, int row_tiles, int warp) {
+    if (++tile < tiles) {
+      off += kTile;
+      while (off >= a.bs) { off -= a.bs; ++page; }
+      return;
+    }
     tile = 0;
-    if (++unit < per_row) return;
-    unit = 0;
+    rewind(a, warp);
+    if (++rt < row_tiles) return;
+    rt = 0;
+    if (++head < a.nkv) return;
+    head = 0;
     enter(a, row + 1);
   }
 };
@@ -154,10 +171,22 @@ template <int D, int ST>
 struct WarpRing {
   uint8_t k[ST][16 * D];
   uint8_t v[ST][16 * D];
-  float s[ST][4];                                // scales of K and V, validity of the page
+  float s[ST][4];                                // scales of K and V
 };
 
-template <typename T, int D, int ST>
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, int bytes) {       // the rest is filled with zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+
+// H: halves of the m16 tile in use (1: units of at most 8 rows)
+template <typename T, int D, int ST, int H>
 __global__ void __launch_bounds__(kThreads)
 paged_q8_kernel(const Args a) {
   extern __shared__ __align__(128) unsigned char smem[];
@@ -168,8 +197,7 @@ paged_q8_kernel(const Args a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   auto& ring = reinterpret_cast<WarpRing<D, ST>*>(smem)[warp];
   float* red = reinterpret_cast<float*>(smem + sizeof(WarpRing<D, ST>) * kWarps);   // [2][rows of a unit][D]
-  const int red_rows = min(a.nq / a.nkv, 16);
-  const int rep = a.nq / a.nkv, row_tiles = (rep + 15) / 16, per_row = a.nkv * row_tiles;
+  const int rep = a.nq / a.nkv, row_tiles = (rep + 15) / 16, per_row = a.nkv * row_tiles, red_rows = min(rep, 16);
   T* out = static_cast<T*>(a.out);
 
   // rows that see nothing are zero
@@ -180,45 +208,61 @@ paged_q8_kernel(const Args a) {
   const Place place = locate(a, per_row, blockIdx.x, sh_place);
   const int64_t pos = place.pos;
   if (pos >= place.total) return;
-  const int64_t end = place.begin(blockIdx.x + 1);
+  int left = (int)(place.begin(blockIdx.x + 1) - pos), left_load = left;
   Cursor use;
   use.enter(a, place.row);
-  use.unit = (int)((pos - place.base) / use.tiles);
-  use.tile = (int)((pos - place.base) % use.tiles);
+  {
+    const int unit = (int)((pos - place.base) / use.tiles);
+    use.tile = (int)((pos - place.base) - (int64_t)unit * use.tiles);
+    use.head = unit / row_tiles;
+    use.rt = unit - use.head * row_tiles;
+  }
+  use.rewind(a, warp);
   Cursor load = use;
-  int64_t left_load = end - pos;
-  int64_t left = end - pos;
 
-  auto page_of = [&](const Cursor& c) -> int {
-    const int tok = c.tile * kTile + warp * 16;
-    if (tok >= c.len) return -1;
-    const int seq = a.row_seq ? a.row_seq[c.row] : c.row;
-    return a.tables[(int64_t)seq * a.width + tok / a.bs];
-  };
-  int page = left_load > 0 ? page_of(load) : -1;
+  // a lane copies the 16-byte chunks lane, lane + 32, ... of the warp's 16 rows, which lie one behind the other
+  constexpr int CH = D / 16, COPIES = 16 * CH / 32;
+  uint32_t k_to[COPIES];
+#pragma unroll
+  for (int i = 0; i < COPIES; ++i) {
+    const int c = i * 32 + lane, r = c / CH;
+    k_to[i] = shared_address(&ring.k[0][0]) + r * D + swizzled<D>(r, c % CH) * 16;
+  }
+  constexpr uint32_t kToV = sizeof(ring.k);
+  const uint32_t s_to = shared_address(&ring.s[0][lane & 1]);
+  const int64_t page_bytes = (int64_t)a.bs * D;
+  auto page_of = [&](const Cursor& c) { return c.tile * kTile + warp * 16 < c.len ? c.table[c.page] : -1; };
+  int page = page_of(load);
+  uint32_t active = 0;                             // stages that hold tokens
   auto issue = [&](int st) {
     if (left_load > 0) {
-      const int tok = load.tile * kTile + warp * 16;
-      if (tok < load.len) {
-        const bool ok = page >= 0 && page < a.pages;
-        const int64_t ph = (int64_t)(ok ? page : 0) * a.nkv + load.unit / row_tiles;
-        const int64_t at = (ph * a.bs + tok % a.bs) * D;
-        const int valid = ok ? min(16, load.len - tok) : 0;
-        constexpr int CH = D / 16;
+      if (page >= 0 && page < a.pages) {
+        active |= 1u << st;
+        const int64_t ph = (int64_t)page * a.nkv + load.head;
+        const int64_t at = ph * page_bytes + load.off * D + lane * 16;
+        const uint8_t *k = a.kc + at, *v = a.vc + at;
+        const int valid = load.len - load.tile * kTile - warp * 16;
+        const uint32_t stage = st * 16 * D;
+        if (valid >= 16) {
 #pragma unroll
-        for (int i = 0; i < 16 * CH / 32; ++i) {
-          const int c = i * 32 + lane, r = c / CH;
-          const int to = r * D + swizzled<D>(r, c % CH) * 16;
-          // rows behind the sequence's end are filled with zeros: 0 * garbage must not be NaN
-          __pipeline_memcpy_async(&ring.k[st][to], a.kc + at + c * 16, 16, r < valid ? 0 : 16);
-          __pipeline_memcpy_async(&ring.v[st][to], a.vc + at + c * 16, 16, r < valid ? 0 : 16);
+          for (int i = 0; i < COPIES; ++i) {
+            copy16(k_to[i] + stage, k + i * 512);
+            copy16(k_to[i] + stage + kToV, v + i * 512);
+          }
+        } else {                                   // rows behind the end become zeros: 0 * garbage must not be NaN
+#pragma unroll
+          for (int i = 0; i < COPIES; ++i) {
+            const int bytes = (i * 32 + lane) / CH < valid ? 16 : 0;
+            copy16(k_to[i] + stage, k + i * 512, bytes);
+            copy16(k_to[i] + stage + kToV, v + i * 512, bytes);
+          }
         }
-        if (lane < 2) __pipeline_memcpy_async(&ring.s[st][lane], (lane ? a.vs : a.ks) + ph, 4);
-        if (lane == 2) ring.s[st][2] = ok ? 1.f : 0.f;
+        if (lane < 2) copy4(s_to + st * 16, (lane ? a.vs : a.ks) + ph);
+      } else {
+        active &= ~(1u << st);
       }
-      load.next(a, per_row);
-      --left_load;
-      page = left_load > 0 ? page_of(load) : -1;
+      load.next(a, row_tiles, warp);
+      if (--left_load > 0) page = page_of(load);
     }
     __pipeline_commit();
   };
@@ -229,40 +273,35 @@ paged_q8_kernel(const Args a) {
   bool first_unit = true;
   while (left > 0) {
     // ---------------- a unit, or the part of it in this block's share
-    const int head = use.unit / row_tiles, rt = use.unit % row_tiles;
-    const int rows_here = min(16, rep - rt * 16);
-    const int from_tile = use.tile, n = (int)min((int64_t)(use.tiles - use.tile), left);
+    const int head = use.head, rt = use.rt, rows_here = min(16, rep - rt * 16);
+    const int from_tile = use.tile, n = min(use.tiles - use.tile, left);
     const int row = use.row, tiles = use.tiles, len = use.len;
     const T* q = static_cast<const T*>(a.q) + row * a.q_row + (int64_t)(head * rep + rt * 16) * D;
     // Q fragments: k-step s of chunk i holds elements 16 (t + 4 i) + 4 s .. + 3 of rows g and g + 8 (the order of the
     // contraction is free as long as K's fragments follow it)
     constexpr int KI = D / 64;
     uint32_t qa[KI * 4][4];
-    float sc[2];
+    float sc[H];
 #pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
+    for (int hf = 0; hf < H; ++hf) {
       const int r = g + 8 * hf;
       float f[KI][16], big = 0.f;
 #pragma unroll
       for (int i = 0; i < KI; ++i)
 #pragma unroll
         for (int e = 0; e < 16; e += 8) {
-          if (r < rows_here) {
-            const uint4 u = *reinterpret_cast<const uint4*>(q + (int64_t)r * D + 16 * (t + 4 * i) + e);
-            const T* x = reinterpret_cast<const T*>(&u);
+          uint4 u = make_uint4(0, 0, 0, 0);
+          if (r < rows_here) u = *reinterpret_cast<const uint4*>(q + (int64_t)r * D + 16 * (t + 4 * i) + e);
+          const T* x = reinterpret_cast<const T*>(&u);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) { f[i][e + j] = to_float(x[j]); big = fmaxf(big, fabsf(f[i][e + j])); }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[i][e + j] = 0.f;
-          }
+          for (int j = 0; j < 8; ++j) { f[i][e + j] = to_float(x[j]); big = fmaxf(big, fabsf(f[i][e + j])); }
         }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // power of two that brings the row's largest to [2^10, 2^11)
+      // power of two that brings the row's largest to [2^10, 2^11); the sign of the softmax scale goes with it
       const int e = big > 0.f ? min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 120) : 0;
-      const float up = __uint_as_float((uint32_t)(127 + 10 - e) << 23);
-      sc[hf] = a.scale * __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+      const float up = copysignf(__uint_as_float((uint32_t)(127 + 10 - e) << 23), a.scale);
+      sc[hf] = fabsf(a.scale) * __uint_as_float((uint32_t)(127 - 10 + e) << 23);
 #pragma unroll
       for (int i = 0; i < KI; ++i)
 #pragma unroll
@@ -271,20 +310,27 @@ paged_q8_kernel(const Args a) {
           qa[i * 4 + s][2 + hf] = half2_bits(f[i][4 * s + 2] * up, f[i][4 * s + 3] * up);
         }
     }
+    if constexpr (H == 1) {
+#pragma unroll
+      for (int i = 0; i < KI * 4; ++i) qa[i][1] = qa[i][3] = 0u;
+    }
     constexpr int NT = D / 8;
     float o[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float m[H], l[H];
+#pragma unroll
+    for (int h = 0; h < H; ++h) { m[h] = -INFINITY; l[h] = 0.f; }
     float unit_v = 0.f;                            // o is kept in units of this V scale
 
     for (int i = 0; i < n; ++i) {
       __pipeline_wait_prior(ST - 2);
       __syncwarp();                                // every lane's copies of this stage are in, every lane is done with the last
+      const bool any = active >> st & 1;
       issue(st == 0 ? ST - 1 : st - 1);
-      const int tok = (from_tile + i) * kTile + warp * 16;
-      if (tok < len && ring.s[st][2] != 0.f) {
+      if (any) {
         const float k_scale = ring.s[st][0], v_scale = ring.s[st][1];
+        const uint8_t *ks = ring.k[st], *vs = ring.v[st];
         // ---- S = Q K^T: two groups of 8 tokens
         float s[2][4];
 #pragma unroll
@@ -293,86 +339,105 @@ paged_q8_kernel(const Args a) {
 #pragma unroll
           for (int c = 0; c < KI; ++c) {
             const int r = j * 8 + g;
-            const uint4 u = *reinterpret_cast<const uint4*>(&ring.k[st][r * D + swizzled<D>(r, t + 4 * c) * 16]);
+            const uint4 u = *reinterpret_cast<const uint4*>(ks + r * D + swizzled<D>(r, t + 4 * c) * 16);
             const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mma_f16(s[j], qa[c * 4 + e], e4m3x2_to_half2(w[e]), e4m3x2_to_half2(w[e] >> 16));
+            for (int e = 0; e < 4; ++e) {
+              uint32_t b0, b1;
+              e4m3x4_to_half2(w[e], b0, b1);
+              mma_f16(s[j], qa[c * 4 + e], b0, b1);
+            }
           }
         }
-        // ---- running softmax of rows g (h = 0) and g + 8 (h = 1)
-        float alpha[2];
-        bool grown = false;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float f = sc[h] * k_scale;
-          float mx = m[h];
+        const int valid = len - (from_tile + i) * kTile - warp * 16;
+        if (valid < 16) {
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float& x = s[j][2 * h + e];
-              x = tok + j * 8 + 2 * t + e < len ? x * f : -INFINITY;
-              mx = fmaxf(mx, x);
-            }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          alpha[h] = mx == m[h] ? 1.f : exp2_approx(m[h] - mx);
-          grown |= mx != m[h];
-          m[h] = mx;
+            for (int e = 0; e < 4; ++e)
+              if (j * 8 + 2 * t + (e & 1) >= valid) s[j][e] = -INFINITY;
+        }
+        // ---- running softmax of rows g (h = 0) and g + 8 (h = 1)
+        float mx[H], f[H];
+        bool grown = false;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          f[h] = fmaxf(sc[h] * k_scale, 1e-37f);   // above 0: masked scores stay -inf at a softmax scale of 0 too
+          mx[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * f[h];
+          grown |= mx[h] > m[h];
         }
         // V's scale joins the probabilities, relative to the unit that o is kept in; the unit follows the scale where
         // they are far apart, so that the probabilities stay inside fp16's normal range
-        float change = 1.f, ratio = unit_v > 0.f ? v_scale / unit_v : 0.f;
-        if (v_scale > 0.f && !(ratio <= 1.f && ratio >= 0.0625f)) {
-          change = unit_v / v_scale;
-          unit_v = v_scale;
-          ratio = 1.f;
-          grown = true;
-        }
-        if (__any_sync(0xffffffffu, grown)) {
-          l[0] *= alpha[0]; l[1] *= alpha[1];
-          alpha[0] *= change; alpha[1] *= change;
+        float ratio = 1.f;
+        const bool moved = v_scale != unit_v;      // the same for the whole warp
+        if (moved || __any_sync(0xffffffffu, grown)) {
+          float change = 1.f;
+          if (moved) {
+            ratio = unit_v > 0.f ? v_scale / unit_v : 0.f;
+            if (v_scale > 0.f && !(ratio <= 1.f && ratio >= 0.0625f)) {
+              change = unit_v / v_scale;
+              unit_v = v_scale;
+              ratio = 1.f;
+            }
+          }
+          float alpha[2] = {1.f, 1.f};
 #pragma unroll
-          for (int j = 0; j < NT; ++j) { o[j][0] *= alpha[0]; o[j][1] *= alpha[0]; o[j][2] *= alpha[1]; o[j][3] *= alpha[1]; }
-        }
-        uint32_t pa[4];
+          for (int h = 0; h < H; ++h) {
+            const float top = fmaxf(m[h], mx[h]);
+            alpha[h] = top == m[h] ? 1.f : exp2_approx(m[h] - top);
+            m[h] = top;
+            l[h] *= alpha[h];
+            alpha[h] *= change;
+          }
+          if (change != 1.f || __any_sync(0xffffffffu, grown)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+            for (int j = 0; j < NT; ++j) {
+              o[j][0] *= alpha[0]; o[j][1] *= alpha[0];
+              if constexpr (H == 2) { o[j][2] *= alpha[1]; o[j][3] *= alpha[1]; }
+            }
+          }
+        }
+        uint32_t pa[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
           const float shift = m[h] == -INFINITY ? 0.f : m[h] - kProbShift;
           float p[2][2];
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) { p[j][e] = exp2_approx(s[j][2 * h + e] - shift); l[h] += p[j][e]; }
+            for (int e = 0; e < 2; ++e) p[j][e] = exp2_approx(fmaf(s[j][2 * h + e], f[h], -shift));
+          l[h] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
           pa[h] = half2_bits(p[0][0] * ratio, p[0][1] * ratio);
           pa[2 + h] = half2_bits(p[1][0] * ratio, p[1][1] * ratio);
         }
         // ---- O += P V: lane g holds the columns of its chunk (or half chunk at D = 64)
         constexpr int VB = D >= 128 ? 16 : 8;      // bytes of a lane's piece of a row
+        const int piece = ((g & 1) << 2) | (g >> 1);
 #pragma unroll
         for (int c = 0; c < D / (8 * VB); ++c) {
           uint32_t w[4][VB / 4];
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const int r = 2 * t + (x & 1) + (x >> 1) * 8;
-            const int piece = ((g & 1) << 2) | (g >> 1);
             if constexpr (VB == 16) {
-              const uint4 u = *reinterpret_cast<const uint4*>(&ring.v[st][r * D + swizzled<D>(r, piece + 8 * c) * 16]);
+              const uint4 u = *reinterpret_cast<const uint4*>(vs + r * D + swizzled<D>(r, piece + 8 * c) * 16);
               w[x][0] = u.x; w[x][1] = u.y; w[x][2] = u.z; w[x][3] = u.w;
             } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(&ring.v[st][r * D + swizzled<D>(r, piece >> 1) * 16 + (piece & 1) * 8]);
+              const uint2 u = *reinterpret_cast<const uint2*>(vs + r * D + swizzled<D>(r, piece >> 1) * 16 + (piece & 1) * 8);
               w[x][0] = u.x; w[x][1] = u.y;
             }
           }
 #pragma unroll
           for (int y = 0; y < VB / 4; ++y) {
-            const uint32_t a01 = __byte_perm(w[0][y], w[1][y], 0x5140), a23 = __byte_perm(w[0][y], w[1][y], 0x7362);
-            const uint32_t b01 = __byte_perm(w[2][y], w[3][y], 0x5140), b23 = __byte_perm(w[2][y], w[3][y], 0x7362);
-            const int j = c * VB + y * 4;
-            mma_f16(o[j], pa, e4m3x2_to_half2(a01), e4m3x2_to_half2(b01));
-            mma_f16(o[j + 1], pa, e4m3x2_to_half2(a01 >> 16), e4m3x2_to_half2(b01 >> 16));
-            mma_f16(o[j + 2], pa, e4m3x2_to_half2(a23), e4m3x2_to_half2(b23));
-            mma_f16(o[j + 3], pa, e4m3x2_to_half2(a23 >> 16), e4m3x2_to_half2(b23 >> 16));
+            uint32_t lo[4], hi[4];
+            e4m3x4_to_half2(__byte_perm(w[0][y], w[1][y], 0x5140), lo[0], lo[1]);
+            e4m3x4_to_half2(__byte_perm(w[0][y], w[1][y], 0x7362), lo[2], lo[3]);
+            e4m3x4_to_half2(__byte_perm(w[2][y], w[3][y], 0x5140), hi[0], hi[1]);
+            e4m3x4_to_half2(__byte_perm(w[2][y], w[3][y], 0x7362), hi[2], hi[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mma_f16(o[c * VB + y * 4 + e], pa, lo[e], hi[e]);
           }
         }
       }
@@ -380,23 +445,23 @@ paged_q8_kernel(const Args a) {
     }
     left -= n;
     use.tile += n - 1;
-    use.next(a, per_row);
+    use.next(a, row_tiles, warp);
 
     // ---------------- the four streams of the unit meet
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < H; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
       if (t == 0) { sh_m[warp][g + 8 * h] = m[h]; sh_l[warp][g + 8 * h] = l[h]; }
     }
     __syncthreads();
-    float top[2], w[2];
+    float w[H];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      top[h] = -INFINITY;
+    for (int h = 0; h < H; ++h) {
+      float top = -INFINITY;
 #pragma unroll
-      for (int x = 0; x < kWarps; ++x) top[h] = fmaxf(top[h], sh_m[x][g + 8 * h]);
-      w[h] = m[h] == -INFINITY && l[h] == 0.f ? 0.f : exp2_approx(m[h] - top[h]) * unit_v;
+      for (int x = 0; x < kWarps; ++x) top = fmaxf(top, sh_m[x][g + 8 * h]);
+      w[h] = m[h] == -INFINITY && l[h] == 0.f ? 0.f : exp2_approx(m[h] - top) * unit_v;
     }
     // column of accumulator j: piece of lane 2 t (+ 1), element j
     constexpr int VB = D >= 128 ? 16 : 8;
@@ -406,22 +471,25 @@ paged_q8_kernel(const Args a) {
       if ((warp >> 1) == pass) {
         float* to = red + (warp & 1) * red_rows * D;
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+        for (int h = 0; h < H; ++h)
+          if (g + 8 * h < rows_here)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            if (g + 8 * h < rows_here)
+            for (int j = 0; j < NT; j += 4)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                float& x = to[(g + 8 * h) * D + column(j, e)];
-                const float y = w[h] == 0.f ? 0.f : o[j][2 * h + e] * w[h];
-                x = pass ? x + y : y;
+                float4& x = *reinterpret_cast<float4*>(&to[(g + 8 * h) * D + column(j, e)]);
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (w[h] != 0.f)
+                  y = make_float4(o[j][2 * h + e] * w[h], o[j + 1][2 * h + e] * w[h], o[j + 2][2 * h + e] * w[h], o[j + 3][2 * h + e] * w[h]);
+                if (pass) { y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w; }
+                x = y;
               }
       }
       __syncthreads();
     }
     const bool whole = from_tile == 0 && n == tiles;
     const int slot = 2 * blockIdx.x + (first_unit && from_tile > 0 ? 0 : 1);
-    for (int i = tid; i < rows_here * D; i += kThreads) {
+    for (int i = tid * 2; i < rows_here * D; i += kThreads * 2) {
       const int r = i / D, d = i % D;
       float big = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -429,11 +497,14 @@ paged_q8_kernel(const Args a) {
 #pragma unroll
       for (int x = 0; x < kWarps; ++x)
         if (sh_l[x][r] != 0.f) sum += sh_l[x][r] * exp2_approx(sh_m[x][r] - big);
-      const float val = red[i] + red[red_rows * D + i];
+      const float2 u = *reinterpret_cast<const float2*>(&red[i]), v = *reinterpret_cast<const float2*>(&red[red_rows * D + i]);
+      const float2 val = make_float2(u.x + v.x, u.y + v.y);
       if (whole) {
-        out[((int64_t)row * a.nq + head * rep + rt * 16 + r) * D + d] = from_float<T>(sum == 0.f ? 0.f : val / sum);
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        T pair[2] = {from_float<T>(val.x * inv), from_float<T>(val.y * inv)};
+        *reinterpret_cast<uint32_t*>(&out[((int64_t)row * a.nq + head * rep + rt * 16 + r) * D + d]) = *reinterpret_cast<const uint32_t*>(pair);
       } else {
-        a.part_o[((int64_t)slot * 16 + r) * D + d] = val;
+        *reinterpret_cast<float2*>(&a.part_o[((int64_t)slot * 16 + r) * D + d]) = val;
         if (d == 0) {
           a.part_ml[(slot * 16 + r) * 2] = big;
           a.part_ml[(slot * 16 + r) * 2 + 1] = sum;
@@ -514,6 +585,7 @@ template <typename T, int D>
 void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
   constexpr int ST = D == 64 ? 6 : D == 128 ? 4 : 3;
   const int rep = a.nq / a.nkv, row_tiles = (rep + 15) / 16, red_rows = std::min(rep, 16);
+  void (*kernel)(const Args) = rep <= 8 ? paged_q8_kernel<T, D, ST, 1> : paged_q8_kernel<T, D, ST, 2>;
   auto smem_of = [](int rows) { return sizeof(WarpRing<D, ST>) * kWarps + 2 * rows * D * sizeof(float); };
   const size_t smem = smem_of(red_rows);
   static std::atomic<int> residents[64][17] = {};  // blocks that an SM holds, per device and rows of a unit
@@ -521,8 +593,8 @@ void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
   TORCH_CHECK(dev >= 0 && dev < 64, "paged_attention_q8: device index out of range");
   int resident = residents[dev][red_rows].load();
   if (!resident) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(paged_q8_kernel<T, D, ST>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(16)));
-    C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, paged_q8_kernel<T, D, ST>, kThreads, smem));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(16)));
+    C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, smem));
     resident = std::max(resident, 1);
     residents[dev][red_rows].store(resident);
   }
@@ -532,7 +604,7 @@ void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
   auto part_ml = at::empty({2 * a.grid, 16, 2}, q.options().dtype(at::kFloat));
   a.part_o = part_o.data_ptr<float>();
   a.part_ml = part_ml.data_ptr<float>();
-  C10_CUDA_CHECK(launch_pdl(paged_q8_kernel<T, D, ST>, dim3(a.grid), dim3(kThreads), smem, st, a));
+  C10_CUDA_CHECK(launch_pdl(kernel, dim3(a.grid), dim3(kThreads), smem, st, a));
   if (a.grid > 1)
     C10_CUDA_CHECK(launch_pdl(paged_q8_join_kernel<T, D>, dim3(a.grid - 1, std::min(rep, 16)), dim3(kThreads), 0, st, a));
 }

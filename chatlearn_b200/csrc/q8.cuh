@@ -23,18 +23,18 @@ __device__ __forceinline__ uint32_t pack_e4m3(float lo, float hi) {
   return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 
-// two codes (low 16 bits) as a pair of halves
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t codes) {
-  const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(codes & 0xffffu), __NV_E4M3);
-  return (uint32_t)r.x | (uint32_t)r.y << 16;
+// four codes as two pairs of halves (exact: e4m3 is a subset of fp16)
+__device__ __forceinline__ void e4m3x4_to_half2(uint32_t codes, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}" : "=r"(lo), "=r"(hi) : "r"(codes));
 }
 
 // four codes as fp32
 __device__ __forceinline__ void unpack_e4m3(uint32_t codes, float* f) {
+  uint32_t h[2];
+  e4m3x4_to_half2(codes, h[0], h[1]);
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const uint32_t h = e4m3x2_to_half2(codes >> (16 * i));
-    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h));
+    const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
     f[2 * i] = v.x;
     f[2 * i + 1] = v.y;
   }
