@@ -2,11 +2,13 @@
 //
 //   o = softmax(scale * q (s_k C_k)^T) (s_v C_v)
 //
-// One unit of work is (query row set, kv head): the query heads that share a kv head are the rows of one m16n8k16 tile,
-// so each cached byte is read once per unit and dequantised once.  Codes become halves by one conversion (exact: e4m3
-// is a subset of fp16); the scales are powers of two and stay out of the products: s_k joins the softmax scale, s_v the
-// probabilities.  Queries are rescaled per row by a power of two to 2^10..2^11, so that their fp16 form loses nothing
-// that counts (bf16 has 8 significant bits, fp16 11; what falls below 2^-24 of a row's largest is lost).
+// One unit of work is (query row set, kv head): the query heads that share a kv head are the columns of m16n8k16 tiles
+// whose rows are cached tokens (S^T = K Q^T) or head elements (O^T = V^T P^T), so that up to 8 heads waste nothing, each
+// cached byte is read once per unit and dequantised once.  Codes become halves by one conversion (exact: e4m3 is a
+// subset of fp16); the scales are powers of two and stay out of the products: s_k joins the softmax scale, s_v the
+// probabilities.  (Products of e4m3 operands are no way around the conversions: mma.sync carries them out in halves.)
+// Queries are rescaled per row by a power of two to 2^10..2^11, so that their fp16 form loses nothing that counts (bf16
+// has 8 significant bits, fp16 11; what falls below 2^-24 of a row's largest is lost).
 //
 // The bytes of the cache bound it.  The tokens of all units form one line that is cut evenly over the resident blocks
 // (whatever the lengths are), 64 at a time; a unit that a cut divides is written as partial (o, m, l) and joined by a
@@ -21,6 +23,7 @@
 #include <cuda_pipeline.h>
 
 #include <atomic>
+#include <type_traits>
 
 #include "q8.cuh"
 
@@ -30,7 +33,9 @@ using namespace q8;
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4;
-constexpr int kTile = 64;                         // tokens of a tile: 16 for each warp
+// tokens that a warp takes at a time: 8 KB of keys and values at head dims 128 and 256
+__host__ __device__ constexpr int warp_tokens(int D) { return D >= 256 ? 16 : 32; }
+__host__ __device__ constexpr int tile_tokens(int D) { return kWarps * warp_tokens(D); }
 // probabilities are carried times 2^10: fp16 keeps 11 bits of them down to 2^-24 of the largest
 constexpr float kProbShift = 10.f;
 
@@ -47,12 +52,14 @@ struct Args {
   int rows, T, width, nq, nkv, bs;
   int64_t pages;
   int grid;                      // blocks that the line is cut over
+  int unit_rows;                 // query heads of a unit: 8 or 16
   float scale;                   // softmax scale times log2 e
 };
 
+template <int TILE>
 __device__ __forceinline__ int tiles_of(const Args& a, int r) {
   const int len = min(a.row_len[r], a.width * a.bs);
-  return len > 0 ? (len + kTile - 1) / kTile : 0;
+  return len > 0 ? (len + TILE - 1) / TILE : 0;
 }
 
 // The line is cut into min(blocks, tiles) shares: none is empty, and their bounds go by the lengths alone.
@@ -66,12 +73,13 @@ struct Place {
 };
 
 // Exclusive prefix sums over the rows' tiles, `per_row` units each.  All threads of the block take part.
+template <int TILE>
 __device__ Place locate(const Args& a, int per_row, int index, int64_t* sh) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per = (a.rows + kThreads - 1) / kThreads;
   const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
   int64_t sum = 0;
-  for (int r = r0; r < r1; ++r) sum += tiles_of(a, r);
+  for (int r = r0; r < r1; ++r) sum += tiles_of<TILE>(a, r);
   sum *= per_row;
   int64_t inc = sum;
 #pragma unroll
@@ -96,7 +104,7 @@ __device__ Place locate(const Args& a, int per_row, int index, int64_t* sh) {
     int64_t at = first;
     int r = r0;
     for (; r < r1; ++r) {
-      const int64_t n = (int64_t)tiles_of(a, r) * per_row;
+      const int64_t n = (int64_t)tiles_of<TILE>(a, r) * per_row;
       if (pos < at + n) break;
       at += n;
     }
@@ -114,6 +122,12 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], u
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// lane (g, t) gives elements 2 t, 2 t + 1 of row g of an 8 x 8 matrix of halves and gets those of column g
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
@@ -133,28 +147,31 @@ __device__ __forceinline__ int swizzled(int r, int chunk) {
   return chunk ^ ((r >> 1) & 3);
 }
 
-// A warp's position on the line: row set, kv head and row tile of it, tile; the page that holds the warp's 16 tokens.
+// A warp's position on the line: row set, kv head and row tile of it, tile; the page that holds the warp's first token.
+template <int TILE, int WT>
 struct Cursor {
   int row, head, rt, tile, tiles, len;
   int page, off;                                 // number in the sequence's table, token inside the page
+  int step_page, step_off;                       // of a tile
   const int* table;
-  __device__ __forceinline__ void rewind(const Args& a, int warp) {      // to token `tile * kTile + 16 * warp`
-    const int tok = tile * kTile + warp * 16;
-    page = tok / a.bs;
-    off = tok - page * a.bs;
+  __device__ __forceinline__ int token(int warp) const { return tile * TILE + warp * WT; }
+  __device__ __forceinline__ void rewind(const Args& a, int warp) {
+    page = token(warp) / a.bs;
+    off = token(warp) - page * a.bs;
   }
   __device__ __forceinline__ void enter(const Args& a, int r) {
     row = r;
     tiles = 0;
-    while (row < a.rows && (tiles = tiles_of(a, row)) == 0) ++row;
+    while (row < a.rows && (tiles = tiles_of<TILE>(a, row)) == 0) ++row;
     if (row >= a.rows) return;
     len = min(a.row_len[row], a.width * a.bs);
     table = a.tables + (int64_t)(a.row_seq ? a.row_seq[row] : row) * a.width;
   }
   __device__ __forceinline__ void next(const Args& a, int row_tiles, int warp) {
     if (++tile < tiles) {
-      off += kTile;
-      while (off >= a.bs) { off -= a.bs; ++page; }
+      page += step_page;
+      off += step_off;
+      if (off >= a.bs) { off -= a.bs; ++page; }
       return;
     }
     tile = 0;
@@ -169,9 +186,9 @@ struct Cursor {
 
 template <int D, int ST>
 struct WarpRing {
-  uint8_t k[ST][16 * D];
-  uint8_t v[ST][16 * D];
-  float s[ST][4];                                // scales of K and V
+  uint8_t k[ST][warp_tokens(D) * D];
+  uint8_t v[ST][warp_tokens(D) * D];
+  float s[ST][4];                                // scales of the 16-token halves: K, V, K, V
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -185,10 +202,11 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 
-// H: halves of the m16 tile in use (1: units of at most 8 rows)
+// H: 1 for units of at most 8 rows, 2 for up to 16
 template <typename T, int D, int ST, int H>
 __global__ void __launch_bounds__(kThreads)
 paged_q8_kernel(const Args a) {
+  constexpr int WT = warp_tokens(D), TILE = tile_tokens(D), PIECES = WT / 16;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int64_t sh_place[8];
   __shared__ float sh_m[kWarps][16], sh_l[kWarps][16];
@@ -197,19 +215,21 @@ paged_q8_kernel(const Args a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   auto& ring = reinterpret_cast<WarpRing<D, ST>*>(smem)[warp];
   float* red = reinterpret_cast<float*>(smem + sizeof(WarpRing<D, ST>) * kWarps);   // [2][rows of a unit][D]
-  const int rep = a.nq / a.nkv, row_tiles = (rep + 15) / 16, per_row = a.nkv * row_tiles, red_rows = min(rep, 16);
+  const int rep = a.nq / a.nkv, row_tiles = (rep + 8 * H - 1) / (8 * H), per_row = a.nkv * row_tiles, red_rows = min(rep, 8 * H);
   T* out = static_cast<T*>(a.out);
 
   // rows that see nothing are zero
   for (int r = blockIdx.x; r < a.T; r += a.grid)
-    if (r >= a.rows || tiles_of(a, r) == 0)
+    if (r >= a.rows || tiles_of<TILE>(a, r) == 0)
       for (int i = tid; i < a.nq * D; i += kThreads) out[(int64_t)r * a.nq * D + i] = from_float<T>(0.f);
 
-  const Place place = locate(a, per_row, blockIdx.x, sh_place);
+  const Place place = locate<TILE>(a, per_row, blockIdx.x, sh_place);
   const int64_t pos = place.pos;
   if (pos >= place.total) return;
   int left = (int)(place.begin(blockIdx.x + 1) - pos), left_load = left;
-  Cursor use;
+  Cursor<TILE, WT> use;
+  use.step_page = TILE / a.bs;
+  use.step_off = TILE % a.bs;
   use.enter(a, place.row);
   {
     const int unit = (int)((pos - place.base) / use.tiles);
@@ -218,10 +238,10 @@ paged_q8_kernel(const Args a) {
     use.rt = unit - use.head * row_tiles;
   }
   use.rewind(a, warp);
-  Cursor load = use;
+  Cursor<TILE, WT> load = use;
 
-  // a lane copies the 16-byte chunks lane, lane + 32, ... of the warp's 16 rows, which lie one behind the other
-  constexpr int CH = D / 16, COPIES = 16 * CH / 32;
+  // a lane copies the 16-byte chunks lane, lane + 32, ... of 16 rows that lie one behind the other
+  constexpr int CH = D / 16, COPIES = 16 * CH / 32, PIECE = 16 * D;
   uint32_t k_to[COPIES];
 #pragma unroll
   for (int i = 0; i < COPIES; ++i) {
@@ -231,38 +251,52 @@ paged_q8_kernel(const Args a) {
   constexpr uint32_t kToV = sizeof(ring.k);
   const uint32_t s_to = shared_address(&ring.s[0][lane & 1]);
   const int64_t page_bytes = (int64_t)a.bs * D;
-  auto page_of = [&](const Cursor& c) { return c.tile * kTile + warp * 16 < c.len ? c.table[c.page] : -1; };
-  int page = page_of(load);
-  uint32_t active = 0;                             // stages that hold tokens
+  // pages of the warp's 16-token pieces (-1: none)
+  struct Pages { int id[PIECES]; };
+  auto pages_of = [&](const Cursor<TILE, WT>& c) {
+    Pages p;
+    const int tok = c.token(warp);
+    p.id[0] = tok < c.len ? c.table[c.page] : -1;
+    if constexpr (PIECES == 2) p.id[1] = tok + 16 >= c.len ? -1 : c.off + 16 < a.bs ? p.id[0] : c.table[c.page + 1];
+    return p;
+  };
+  Pages pages = pages_of(load);
+  uint32_t active = 0;                             // pieces of the stages that hold tokens
+  auto copy_piece = [&](int st, int x, int64_t ph, int off, int valid) {
+    const int64_t at = ph * page_bytes + off * D + lane * 16;
+    const uint8_t *k = a.kc + at, *v = a.vc + at;
+    const uint32_t stage = st * WT * D + x * PIECE;
+    if (valid >= 16) {
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        copy16(k_to[i] + stage, k + i * 512);
+        copy16(k_to[i] + stage + kToV, v + i * 512);
+      }
+    } else {                                       // rows behind the end become zeros: 0 * garbage must not be NaN
+#pragma unroll
+      for (int i = 0; i < COPIES; ++i) {
+        const int bytes = (i * 32 + lane) / CH < valid ? 16 : 0;
+        copy16(k_to[i] + stage, k + i * 512, bytes);
+        copy16(k_to[i] + stage + kToV, v + i * 512, bytes);
+      }
+    }
+    if (lane < 2) copy4(s_to + st * 16 + x * 8, (lane ? a.vs : a.ks) + ph);
+  };
   auto issue = [&](int st) {
     if (left_load > 0) {
-      if (page >= 0 && page < a.pages) {
-        active |= 1u << st;
-        const int64_t ph = (int64_t)page * a.nkv + load.head;
-        const int64_t at = ph * page_bytes + load.off * D + lane * 16;
-        const uint8_t *k = a.kc + at, *v = a.vc + at;
-        const int valid = load.len - load.tile * kTile - warp * 16;
-        const uint32_t stage = st * 16 * D;
-        if (valid >= 16) {
+      constexpr uint32_t kAll = (1u << PIECES) - 1;
+      uint32_t have = 0;
 #pragma unroll
-          for (int i = 0; i < COPIES; ++i) {
-            copy16(k_to[i] + stage, k + i * 512);
-            copy16(k_to[i] + stage + kToV, v + i * 512);
-          }
-        } else {                                   // rows behind the end become zeros: 0 * garbage must not be NaN
-#pragma unroll
-          for (int i = 0; i < COPIES; ++i) {
-            const int bytes = (i * 32 + lane) / CH < valid ? 16 : 0;
-            copy16(k_to[i] + stage, k + i * 512, bytes);
-            copy16(k_to[i] + stage + kToV, v + i * 512, bytes);
-          }
+      for (int x = 0; x < PIECES; ++x)
+        if (pages.id[x] >= 0 && pages.id[x] < a.pages) {
+          have |= 1u << x;
+          int off = load.off + 16 * x;
+          if (x > 0 && off >= a.bs) off -= a.bs;
+          copy_piece(st, x, (int64_t)pages.id[x] * a.nkv + load.head, off, load.len - load.token(warp) - 16 * x);
         }
-        if (lane < 2) copy4(s_to + st * 16, (lane ? a.vs : a.ks) + ph);
-      } else {
-        active &= ~(1u << st);
-      }
+      active = (active & ~(kAll << (st * PIECES))) | have << (st * PIECES);
       load.next(a, row_tiles, warp);
-      if (--left_load > 0) page = page_of(load);
+      if (--left_load > 0) pages = pages_of(load);
     }
     __pipeline_commit();
   };
@@ -273,18 +307,18 @@ paged_q8_kernel(const Args a) {
   bool first_unit = true;
   while (left > 0) {
     // ---------------- a unit, or the part of it in this block's share
-    const int head = use.head, rt = use.rt, rows_here = min(16, rep - rt * 16);
+    const int head = use.head, rt = use.rt, rows_here = min(8 * H, rep - rt * 8 * H);
     const int from_tile = use.tile, n = min(use.tiles - use.tile, left);
     const int row = use.row, tiles = use.tiles, len = use.len;
-    const T* q = static_cast<const T*>(a.q) + row * a.q_row + (int64_t)(head * rep + rt * 16) * D;
-    // Q fragments: k-step s of chunk i holds elements 16 (t + 4 i) + 4 s .. + 3 of rows g and g + 8 (the order of the
-    // contraction is free as long as K's fragments follow it)
+    const T* q = static_cast<const T*>(a.q) + row * a.q_row + (int64_t)(head * rep + rt * 8 * H) * D;
+    // Q fragments: k-step e of chunk i holds elements 16 (t + 4 i) + 4 e .. + 3 of head g (+ 8 h); the order of the
+    // contraction is free as long as K's fragments follow it
     constexpr int KI = D / 64;
-    uint32_t qa[KI * 4][4];
-    float sc[H];
+    uint32_t qb[H][KI * 4][2];
+    float sc[H][2];                                // softmax scale of heads 2 t, 2 t + 1 (+ 8 h) times what q was divided by
 #pragma unroll
-    for (int hf = 0; hf < H; ++hf) {
-      const int r = g + 8 * hf;
+    for (int h = 0; h < H; ++h) {
+      const int r = g + 8 * h;
       float f[KI][16], big = 0.f;
 #pragma unroll
       for (int i = 0; i < KI; ++i)
@@ -301,143 +335,177 @@ paged_q8_kernel(const Args a) {
       // power of two that brings the row's largest to [2^10, 2^11); the sign of the softmax scale goes with it
       const int e = big > 0.f ? min(max((int)(__float_as_uint(big) >> 23) - 127, -100), 120) : 0;
       const float up = copysignf(__uint_as_float((uint32_t)(127 + 10 - e) << 23), a.scale);
-      sc[hf] = fabsf(a.scale) * __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+      const float down = fabsf(a.scale) * __uint_as_float((uint32_t)(127 - 10 + e) << 23);
+      sc[h][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+      sc[h][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
 #pragma unroll
       for (int i = 0; i < KI; ++i)
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          qa[i * 4 + s][hf] = half2_bits(f[i][4 * s] * up, f[i][4 * s + 1] * up);
-          qa[i * 4 + s][2 + hf] = half2_bits(f[i][4 * s + 2] * up, f[i][4 * s + 3] * up);
+          qb[h][i * 4 + s][0] = half2_bits(f[i][4 * s] * up, f[i][4 * s + 1] * up);
+          qb[h][i * 4 + s][1] = half2_bits(f[i][4 * s + 2] * up, f[i][4 * s + 3] * up);
         }
     }
-    if constexpr (H == 1) {
+    // accumulator j: elements 2 j, 2 j + 1 of a lane's piece of the head, heads 2 t, 2 t + 1
+    constexpr int NT = D / 16;
+    float o[H][NT][4];
+    float m[H][2], l[H][2];
 #pragma unroll
-      for (int i = 0; i < KI * 4; ++i) qa[i][1] = qa[i][3] = 0u;
+    for (int h = 0; h < H; ++h) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) o[h][j][0] = o[h][j][1] = o[h][j][2] = o[h][j][3] = 0.f;
+      m[h][0] = m[h][1] = -INFINITY;
+      l[h][0] = l[h][1] = 0.f;
     }
-    constexpr int NT = D / 8;
-    float o[NT][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-    float m[H], l[H];
-#pragma unroll
-    for (int h = 0; h < H; ++h) { m[h] = -INFINITY; l[h] = 0.f; }
     float unit_v = 0.f;                            // o is kept in units of this V scale
 
     for (int i = 0; i < n; ++i) {
       __pipeline_wait_prior(ST - 2);
       __syncwarp();                                // every lane's copies of this stage are in, every lane is done with the last
-      const bool any = active >> st & 1;
+      const uint32_t now = active >> (st * PIECES) & ((1u << PIECES) - 1);
       issue(st == 0 ? ST - 1 : st - 1);
-      if (any) {
-        const float k_scale = ring.s[st][0], v_scale = ring.s[st][1];
+      if (now) {
         const uint8_t *ks = ring.k[st], *vs = ring.v[st];
-        // ---- S = Q K^T: two groups of 8 tokens
-        float s[2][4];
+        const float4 scales = *reinterpret_cast<const float4*>(ring.s[st]);
+        const float k_scale[2] = {scales.x, scales.z}, v_scale[2] = {scales.y, scales.w};
+        // ---- S^T = K Q^T, 16 tokens at a time: tokens g (elements 0, 1) and g + 8 (2, 3), heads 2 t and 2 t + 1
+        float s[H][PIECES][4];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        for (int x = 0; x < PIECES; ++x) {
+#pragma unroll
+          for (int h = 0; h < H; ++h) s[h][x][0] = s[h][x][1] = s[h][x][2] = s[h][x][3] = 0.f;
 #pragma unroll
           for (int c = 0; c < KI; ++c) {
-            const int r = j * 8 + g;
-            const uint4 u = *reinterpret_cast<const uint4*>(ks + r * D + swizzled<D>(r, t + 4 * c) * 16);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+            const int r = x * 16 + g;              // row r + 8 has the same swizzle
+            const uint8_t* at = ks + r * D + swizzled<D>(r, t + 4 * c) * 16;
+            const uint4 u = *reinterpret_cast<const uint4*>(at), v = *reinterpret_cast<const uint4*>(at + 8 * D);
+            const uint32_t lo[4] = {u.x, u.y, u.z, u.w}, hi[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              uint32_t b0, b1;
-              e4m3x4_to_half2(w[e], b0, b1);
-              mma_f16(s[j], qa[c * 4 + e], b0, b1);
+              uint32_t ka[4];
+              e4m3x4_to_half2(lo[e], ka[0], ka[2]);
+              e4m3x4_to_half2(hi[e], ka[1], ka[3]);
+#pragma unroll
+              for (int h = 0; h < H; ++h) mma_f16(s[h][x], ka, qb[h][c * 4 + e][0], qb[h][c * 4 + e][1]);
             }
           }
         }
-        const int valid = len - (from_tile + i) * kTile - warp * 16;
-        if (valid < 16) {
+        const int valid = len - (from_tile + i) * TILE - warp * WT;
+        if (valid < WT || now != (1u << PIECES) - 1) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int x = 0; x < PIECES; ++x) {
+            const bool out0 = x * 16 + g >= valid || !(now >> x & 1), out1 = x * 16 + g + 8 >= valid || !(now >> x & 1);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (j * 8 + 2 * t + (e & 1) >= valid) s[j][e] = -INFINITY;
+            for (int h = 0; h < H; ++h) {
+              if (out0) s[h][x][0] = s[h][x][1] = -INFINITY;
+              if (out1) s[h][x][2] = s[h][x][3] = -INFINITY;
+            }
+          }
         }
-        // ---- running softmax of rows g (h = 0) and g + 8 (h = 1)
-        float mx[H], f[H];
+        // ---- running softmax
+        float f[H][2][PIECES], mx[H][2];
         bool grown = false;
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-          f[h] = fmaxf(sc[h] * k_scale, 1e-37f);   // above 0: masked scores stay -inf at a softmax scale of 0 too
-          mx[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-          mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2)) * f[h];
-          grown |= mx[h] > m[h];
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            mx[h][y] = -INFINITY;
+#pragma unroll
+            for (int x = 0; x < PIECES; ++x) {
+              // above 0: masked scores stay -inf at a softmax scale of 0 too
+              f[h][y][x] = (now >> x & 1) ? fmaxf(sc[h][y] * k_scale[x], 1e-37f) : 1.f;
+              mx[h][y] = fmaxf(mx[h][y], fmaxf(s[h][x][y], s[h][x][2 + y]) * f[h][y][x]);
+            }
+            mx[h][y] = fmaxf(mx[h][y], __shfl_xor_sync(0xffffffffu, mx[h][y], 4));
+            mx[h][y] = fmaxf(mx[h][y], __shfl_xor_sync(0xffffffffu, mx[h][y], 8));
+            mx[h][y] = fmaxf(mx[h][y], __shfl_xor_sync(0xffffffffu, mx[h][y], 16));
+            grown |= mx[h][y] > m[h][y];
+          }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const float top = fmaxf(m[h][y], mx[h][y]);
+              const float alpha = top == m[h][y] ? 1.f : exp2_approx(m[h][y] - top);
+              m[h][y] = top;
+              l[h][y] *= alpha;
+#pragma unroll
+              for (int j = 0; j < NT; ++j) { o[h][j][y] *= alpha; o[h][j][2 + y] *= alpha; }
+            }
         }
-        // V's scale joins the probabilities, relative to the unit that o is kept in; the unit follows the scale where
-        // they are far apart, so that the probabilities stay inside fp16's normal range
-        float ratio = 1.f;
-        const bool moved = v_scale != unit_v;      // the same for the whole warp
-        if (moved || __any_sync(0xffffffffu, grown)) {
-          float change = 1.f;
-          if (moved) {
-            ratio = unit_v > 0.f ? v_scale / unit_v : 0.f;
-            if (v_scale > 0.f && !(ratio <= 1.f && ratio >= 0.0625f)) {
-              change = unit_v / v_scale;
-              unit_v = v_scale;
-              ratio = 1.f;
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const float shift = m[h][y] == -INFINITY ? 0.f : m[h][y] - kProbShift;
+#pragma unroll
+            for (int x = 0; x < PIECES; ++x) {
+              s[h][x][y] = exp2_approx(fmaf(s[h][x][y], f[h][y][x], -shift));
+              s[h][x][2 + y] = exp2_approx(fmaf(s[h][x][2 + y], f[h][y][x], -shift));
+              l[h][y] += s[h][x][y] + s[h][x][2 + y];
             }
           }
-          float alpha[2] = {1.f, 1.f};
-#pragma unroll
-          for (int h = 0; h < H; ++h) {
-            const float top = fmaxf(m[h], mx[h]);
-            alpha[h] = top == m[h] ? 1.f : exp2_approx(m[h] - top);
-            m[h] = top;
-            l[h] *= alpha[h];
-            alpha[h] *= change;
-          }
-          if (change != 1.f || __any_sync(0xffffffffu, grown)) {
-#pragma unroll
-            for (int j = 0; j < NT; ++j) {
-              o[j][0] *= alpha[0]; o[j][1] *= alpha[0];
-              if constexpr (H == 2) { o[j][2] *= alpha[1]; o[j][3] *= alpha[1]; }
-            }
-          }
-        }
-        uint32_t pa[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-          const float shift = m[h] == -INFINITY ? 0.f : m[h] - kProbShift;
-          float p[2][2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) p[j][e] = exp2_approx(fmaf(s[j][2 * h + e], f[h], -shift));
-          l[h] += (p[0][0] + p[0][1]) + (p[1][0] + p[1][1]);
-          pa[h] = half2_bits(p[0][0] * ratio, p[0][1] * ratio);
-          pa[2 + h] = half2_bits(p[1][0] * ratio, p[1][1] * ratio);
-        }
-        // ---- O += P V: lane g holds the columns of its chunk (or half chunk at D = 64)
-        constexpr int VB = D >= 128 ? 16 : 8;      // bytes of a lane's piece of a row
+        // ---- O^T += V^T P^T, 16 tokens at a time: lane g holds the elements of its piece of V's rows
+        constexpr int VB = D >= 128 ? 16 : 8;      // bytes of a piece
         const int piece = ((g & 1) << 2) | (g >> 1);
 #pragma unroll
-        for (int c = 0; c < D / (8 * VB); ++c) {
-          uint32_t w[4][VB / 4];
+        for (int x = 0; x < PIECES; ++x) {
+          if (PIECES == 2 && !(now >> x & 1)) continue;
+          // V's scale joins the probabilities, relative to the unit that o is kept in; the unit follows the scale where
+          // they are far apart, so that the probabilities stay inside fp16's normal range
+          if (v_scale[x] != unit_v) {              // the same for the whole warp
+            float ratio = unit_v > 0.f ? v_scale[x] / unit_v : 0.f;
+            if (v_scale[x] > 0.f && !(ratio <= 1.f && ratio >= 0.0625f)) {
+              const float change = unit_v / v_scale[x];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int r = 2 * t + (x & 1) + (x >> 1) * 8;
-            if constexpr (VB == 16) {
-              const uint4 u = *reinterpret_cast<const uint4*>(vs + r * D + swizzled<D>(r, piece + 8 * c) * 16);
-              w[x][0] = u.x; w[x][1] = u.y; w[x][2] = u.z; w[x][3] = u.w;
-            } else {
-              const uint2 u = *reinterpret_cast<const uint2*>(vs + r * D + swizzled<D>(r, piece >> 1) * 16 + (piece & 1) * 8);
-              w[x][0] = u.x; w[x][1] = u.y;
+              for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[h][j][e] *= change;
+              unit_v = v_scale[x];
+              ratio = 1.f;
             }
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[h][x][e] *= ratio;
+          }
+          uint32_t pb[H][2];
+#pragma unroll
+          for (int h = 0; h < H; ++h) {
+            pb[h][0] = transpose8(half2_bits(s[h][x][0], s[h][x][1]));
+            pb[h][1] = transpose8(half2_bits(s[h][x][2], s[h][x][3]));
           }
 #pragma unroll
-          for (int y = 0; y < VB / 4; ++y) {
-            uint32_t lo[4], hi[4];
-            e4m3x4_to_half2(__byte_perm(w[0][y], w[1][y], 0x5140), lo[0], lo[1]);
-            e4m3x4_to_half2(__byte_perm(w[0][y], w[1][y], 0x7362), lo[2], lo[3]);
-            e4m3x4_to_half2(__byte_perm(w[2][y], w[3][y], 0x5140), hi[0], hi[1]);
-            e4m3x4_to_half2(__byte_perm(w[2][y], w[3][y], 0x7362), hi[2], hi[3]);
+          for (int c = 0; c < D / (8 * VB); ++c) {
+            uint32_t w[4][VB / 4];                 // tokens 2 t, 2 t + 1, 2 t + 8, 2 t + 9
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mma_f16(o[c * VB + y * 4 + e], pa, lo[e], hi[e]);
+            for (int y = 0; y < 4; ++y) {
+              const int r = x * 16 + 2 * t + (y & 1) + (y >> 1) * 8;
+              if constexpr (VB == 16) {
+                const uint4 u = *reinterpret_cast<const uint4*>(vs + r * D + swizzled<D>(r, piece + 8 * c) * 16);
+                w[y][0] = u.x; w[y][1] = u.y; w[y][2] = u.z; w[y][3] = u.w;
+              } else {
+                const uint2 u = *reinterpret_cast<const uint2*>(vs + r * D + swizzled<D>(r, piece >> 1) * 16 + (piece & 1) * 8);
+                w[y][0] = u.x; w[y][1] = u.y;
+              }
+            }
+#pragma unroll
+            for (int y = 0; y < VB / 4; ++y) {
+              uint32_t lo[4], hi[4];
+              e4m3x4_to_half2(__byte_perm(w[0][y], w[1][y], 0x5140), lo[0], lo[1]);
+              e4m3x4_to_half2(__byte_perm(w[0][y], w[1][y], 0x7362), lo[2], lo[3]);
+              e4m3x4_to_half2(__byte_perm(w[2][y], w[3][y], 0x5140), hi[0], hi[1]);
+              e4m3x4_to_half2(__byte_perm(w[2][y], w[3][y], 0x7362), hi[2], hi[3]);
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                const uint32_t va[4] = {lo[e], lo[e + 1], hi[e], hi[e + 1]};
+#pragma unroll
+                for (int h = 0; h < H; ++h) mma_f16(o[h][(c * VB + y * 4 + e) / 2], va, pb[h][0], pb[h][1]);
+              }
+            }
           }
         }
       }
@@ -449,40 +517,43 @@ paged_q8_kernel(const Args a) {
 
     // ---------------- the four streams of the unit meet
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if (t == 0) { sh_m[warp][g + 8 * h] = m[h]; sh_l[warp][g + 8 * h] = l[h]; }
-    }
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[h][y] += __shfl_xor_sync(0xffffffffu, l[h][y], d);
+        if (g == 0) { sh_m[warp][8 * h + 2 * t + y] = m[h][y]; sh_l[warp][8 * h + 2 * t + y] = l[h][y]; }
+      }
     __syncthreads();
-    float w[H];
+    float w[H][2];
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      float top = -INFINITY;
+    for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int x = 0; x < kWarps; ++x) top = fmaxf(top, sh_m[x][g + 8 * h]);
-      w[h] = m[h] == -INFINITY && l[h] == 0.f ? 0.f : exp2_approx(m[h] - top) * unit_v;
-    }
-    // column of accumulator j: piece of lane 2 t (+ 1), element j
+      for (int y = 0; y < 2; ++y) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < kWarps; ++x) top = fmaxf(top, sh_m[x][8 * h + 2 * t + y]);
+        w[h][y] = m[h][y] == -INFINITY && l[h][y] == 0.f ? 0.f : exp2_approx(m[h][y] - top) * unit_v;
+      }
     constexpr int VB = D >= 128 ? 16 : 8;
-    auto column = [&](int j, int e) { return (j / VB) * (8 * VB) + (e * 4 + t) * VB + j % VB; };
+    const int piece = ((g & 1) << 2) | (g >> 1);
 #pragma unroll
     for (int pass = 0; pass < 2; ++pass) {
       if ((warp >> 1) == pass) {
         float* to = red + (warp & 1) * red_rows * D;
 #pragma unroll
         for (int h = 0; h < H; ++h)
-          if (g + 8 * h < rows_here)
 #pragma unroll
-            for (int j = 0; j < NT; j += 4)
+          for (int y = 0; y < 2; ++y)
+            if (8 * h + 2 * t + y < rows_here)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float4& x = *reinterpret_cast<float4*>(&to[(g + 8 * h) * D + column(j, e)]);
-                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (w[h] != 0.f)
-                  y = make_float4(o[j][2 * h + e] * w[h], o[j + 1][2 * h + e] * w[h], o[j + 2][2 * h + e] * w[h], o[j + 3][2 * h + e] * w[h]);
-                if (pass) { y.x += x.x; y.y += x.y; y.z += x.z; y.w += x.w; }
-                x = y;
+              for (int j = 0; j < NT; j += 2) {
+                float4& x = *reinterpret_cast<float4*>(&to[(8 * h + 2 * t + y) * D + (j * 2 / VB) * 8 * VB + piece * VB + j * 2 % VB]);
+                float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (w[h][y] != 0.f)
+                  z = make_float4(o[h][j][y] * w[h][y], o[h][j][2 + y] * w[h][y], o[h][j + 1][y] * w[h][y], o[h][j + 1][2 + y] * w[h][y]);
+                if (pass) { z.x += x.x; z.y += x.y; z.z += x.z; z.w += x.w; }
+                x = z;
               }
       }
       __syncthreads();
@@ -502,7 +573,7 @@ paged_q8_kernel(const Args a) {
       if (whole) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         T pair[2] = {from_float<T>(val.x * inv), from_float<T>(val.y * inv)};
-        *reinterpret_cast<uint32_t*>(&out[((int64_t)row * a.nq + head * rep + rt * 16 + r) * D + d]) = *reinterpret_cast<const uint32_t*>(pair);
+        *reinterpret_cast<uint32_t*>(&out[((int64_t)row * a.nq + head * rep + rt * 8 * H + r) * D + d]) = *reinterpret_cast<const uint32_t*>(pair);
       } else {
         *reinterpret_cast<float2*>(&a.part_o[((int64_t)slot * 16 + r) * D + d]) = val;
         if (d == 0) {
@@ -523,23 +594,23 @@ __global__ void __launch_bounds__(kThreads) paged_q8_join_kernel(const Args a) {
   __shared__ int64_t sh_place[8];
   pdl_trigger();
   pdl_wait();
-  const int rep = a.nq / a.nkv, row_tiles = (rep + 15) / 16, per_row = a.nkv * row_tiles;
+  const int rep = a.nq / a.nkv, row_tiles = (rep + a.unit_rows - 1) / a.unit_rows, per_row = a.nkv * row_tiles;
   const int c = blockIdx.x + 1;
-  const Place place = locate(a, per_row, c, sh_place);
+  const Place place = locate<tile_tokens(D)>(a, per_row, c, sh_place);
   const int64_t pos = place.pos;
   if (pos >= place.total) return;
-  const int tiles = tiles_of(a, place.row);
+  const int tiles = tiles_of<tile_tokens(D)>(a, place.row);
   const int unit = (int)((pos - place.base) / tiles);
   const int64_t start = place.base + (int64_t)unit * tiles, stop = start + tiles;
   if (pos == start || place.begin(c - 1) > start) return;
   int last = c;                                    // last block with a part
   while (last + 1 < place.shares && place.begin(last + 1) < stop) ++last;
   const int head = unit / row_tiles, rt = unit % row_tiles, r = blockIdx.y;
-  if (r >= min(16, rep - rt * 16)) return;
+  if (r >= min(a.unit_rows, rep - rt * a.unit_rows)) return;
   auto slot = [&](int x) { return x == c - 1 ? 2 * (c - 1) + 1 : 2 * x; };
   float big = -INFINITY;
   for (int x = c - 1; x <= last; ++x) big = fmaxf(big, a.part_ml[(slot(x) * 16 + r) * 2]);
-  T* out = static_cast<T*>(a.out) + ((int64_t)place.row * a.nq + head * rep + rt * 16 + r) * D;
+  T* out = static_cast<T*>(a.out) + ((int64_t)place.row * a.nq + head * rep + rt * a.unit_rows + r) * D;
   for (int d = threadIdx.x; d < D; d += kThreads) {
     float num = 0.f, den = 0.f;
 #pragma unroll 4
@@ -583,9 +654,12 @@ q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B
 
 template <typename T, int D>
 void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
-  constexpr int ST = D == 64 ? 6 : D == 128 ? 4 : 3;
-  const int rep = a.nq / a.nkv, row_tiles = (rep + 15) / 16, red_rows = std::min(rep, 16);
-  void (*kernel)(const Args) = rep <= 8 ? paged_q8_kernel<T, D, ST, 1> : paged_q8_kernel<T, D, ST, 2>;
+  constexpr int ST = D == 64 ? 5 : 3;
+  constexpr int kMostH = 2;
+  const int rep = a.nq / a.nkv;
+  a.unit_rows = rep <= 8 || kMostH == 1 ? 8 : 16;
+  const int row_tiles = (rep + a.unit_rows - 1) / a.unit_rows, red_rows = std::min(rep, a.unit_rows);
+  void (*kernel)(const Args) = a.unit_rows == 8 ? paged_q8_kernel<T, D, ST, 1> : paged_q8_kernel<T, D, ST, kMostH>;
   auto smem_of = [](int rows) { return sizeof(WarpRing<D, ST>) * kWarps + 2 * rows * D * sizeof(float); };
   const size_t smem = smem_of(red_rows);
   static std::atomic<int> residents[64][17] = {};  // blocks that an SM holds, per device and rows of a unit
@@ -598,7 +672,7 @@ void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
     resident = std::max(resident, 1);
     residents[dev][red_rows].store(resident);
   }
-  const int64_t most = (int64_t)a.rows * a.nkv * row_tiles * (((int64_t)a.width * a.bs + kTile - 1) / kTile);
+  const int64_t most = (int64_t)a.rows * a.nkv * row_tiles * (((int64_t)a.width * a.bs + tile_tokens(D) - 1) / tile_tokens(D));
   a.grid = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)resident * at::cuda::getCurrentDeviceProperties()->multiProcessorCount, most));
   auto part_o = at::empty({2 * a.grid, 16, D}, q.options().dtype(at::kFloat));
   auto part_ml = at::empty({2 * a.grid, 16, 2}, q.options().dtype(at::kFloat));
@@ -606,7 +680,7 @@ void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
   a.part_ml = part_ml.data_ptr<float>();
   C10_CUDA_CHECK(launch_pdl(kernel, dim3(a.grid), dim3(kThreads), smem, st, a));
   if (a.grid > 1)
-    C10_CUDA_CHECK(launch_pdl(paged_q8_join_kernel<T, D>, dim3(a.grid - 1, std::min(rep, 16)), dim3(kThreads), 0, st, a));
+    C10_CUDA_CHECK(launch_pdl(paged_q8_join_kernel<T, D>, dim3(a.grid - 1, red_rows), dim3(kThreads), 0, st, a));
 }
 
 }  // namespace
