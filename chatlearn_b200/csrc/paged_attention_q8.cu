@@ -50,7 +50,7 @@ struct Args {
   void* out;                     // [T, nq, D]
   float *part_o, *part_ml;       // [2 * grid, 16, D], [2 * grid, 16, 2]
   int rows, T, width, nq, nkv, bs;
-  int64_t pages;
+  int pages;
   int grid;                      // blocks that the line is cut over
   int unit_rows;                 // query heads of a unit: 8 or 16
   float scale;                   // softmax scale times log2 e
@@ -202,11 +202,12 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 
-// H: 1 for units of at most 8 rows, 2 for up to 16
-template <typename T, int D, int ST, int H>
+// H: 1 for units of at most 8 rows, 2 for up to 16.  PG: pages that a warp's tokens can lie in (2: 32 tokens, page length
+// no multiple of 32).
+template <typename T, int D, int ST, int H, int PG>
 __global__ void __launch_bounds__(kThreads)
 paged_q8_kernel(const Args a) {
-  constexpr int WT = warp_tokens(D), TILE = tile_tokens(D), PIECES = WT / 16;
+  constexpr int WT = warp_tokens(D), TILE = tile_tokens(D), PIECES = WT / 16, PT = WT / PG;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int64_t sh_place[8];
   __shared__ float sh_m[kWarps][16], sh_l[kWarps][16];
@@ -240,61 +241,62 @@ paged_q8_kernel(const Args a) {
   use.rewind(a, warp);
   Cursor<TILE, WT> load = use;
 
-  // a lane copies the 16-byte chunks lane, lane + 32, ... of 16 rows that lie one behind the other
-  constexpr int CH = D / 16, COPIES = 16 * CH / 32, PIECE = 16 * D;
-  uint32_t k_to[COPIES];
+  // a lane copies the 16-byte chunks lane, lane + 32, ... of PT rows that lie one behind the other
+  constexpr int CH = D / 16, COPIES = PT * CH / 32;
+  const uint32_t k_base = shared_address(&ring.k[0][0]);
+  uint32_t k_to[16 * CH / 32];                     // of the first 16 rows: the swizzle repeats behind them
 #pragma unroll
-  for (int i = 0; i < COPIES; ++i) {
+  for (int i = 0; i < 16 * CH / 32; ++i) {
     const int c = i * 32 + lane, r = c / CH;
-    k_to[i] = shared_address(&ring.k[0][0]) + r * D + swizzled<D>(r, c % CH) * 16;
+    k_to[i] = k_base + r * D + swizzled<D>(r, c % CH) * 16;
   }
   constexpr uint32_t kToV = sizeof(ring.k);
   const uint32_t s_to = shared_address(&ring.s[0][lane & 1]);
+  const float* s_from = lane & 1 ? a.vs : a.ks;
   const int64_t page_bytes = (int64_t)a.bs * D;
-  // pages of the warp's 16-token pieces (-1: none)
-  struct Pages { int id[PIECES]; };
+  struct Pages { int id[PG]; };                    // -1: none
   auto pages_of = [&](const Cursor<TILE, WT>& c) {
     Pages p;
     const int tok = c.token(warp);
     p.id[0] = tok < c.len ? c.table[c.page] : -1;
-    if constexpr (PIECES == 2) p.id[1] = tok + 16 >= c.len ? -1 : c.off + 16 < a.bs ? p.id[0] : c.table[c.page + 1];
+    if constexpr (PG == 2) p.id[1] = tok + PT >= c.len ? -1 : c.off + PT < a.bs ? p.id[0] : c.table[c.page + 1];
     return p;
   };
   Pages pages = pages_of(load);
-  uint32_t active = 0;                             // pieces of the stages that hold tokens
-  auto copy_piece = [&](int st, int x, int64_t ph, int off, int valid) {
-    const int64_t at = ph * page_bytes + off * D + lane * 16;
-    const uint8_t *k = a.kc + at, *v = a.vc + at;
-    const uint32_t stage = st * WT * D + x * PIECE;
-    if (valid >= 16) {
-#pragma unroll
-      for (int i = 0; i < COPIES; ++i) {
-        copy16(k_to[i] + stage, k + i * 512);
-        copy16(k_to[i] + stage + kToV, v + i * 512);
-      }
-    } else {                                       // rows behind the end become zeros: 0 * garbage must not be NaN
-#pragma unroll
-      for (int i = 0; i < COPIES; ++i) {
-        const int bytes = (i * 32 + lane) / CH < valid ? 16 : 0;
-        copy16(k_to[i] + stage, k + i * 512, bytes);
-        copy16(k_to[i] + stage + kToV, v + i * 512, bytes);
-      }
-    }
-    if (lane < 2) copy4(s_to + st * 16 + x * 8, (lane ? a.vs : a.ks) + ph);
-  };
+  constexpr uint32_t kAll = (1u << PG) - 1;
+  uint32_t active = 0;                             // pages of the stages that hold tokens
   auto issue = [&](int st) {
     if (left_load > 0) {
-      constexpr uint32_t kAll = (1u << PIECES) - 1;
       uint32_t have = 0;
 #pragma unroll
-      for (int x = 0; x < PIECES; ++x)
-        if (pages.id[x] >= 0 && pages.id[x] < a.pages) {
+      for (int x = 0; x < PG; ++x)
+        if ((uint32_t)pages.id[x] < (uint32_t)a.pages) {
           have |= 1u << x;
-          int off = load.off + 16 * x;
+          int off = load.off + PT * x;
           if (x > 0 && off >= a.bs) off -= a.bs;
-          copy_piece(st, x, (int64_t)pages.id[x] * a.nkv + load.head, off, load.len - load.token(warp) - 16 * x);
+          const int ph = pages.id[x] * a.nkv + load.head, valid = load.len - load.token(warp) - PT * x;
+          const int64_t at = ph * page_bytes + off * D + lane * 16;
+          const uint8_t *k = a.kc + at, *v = a.vc + at;
+          const uint32_t stage = (st * WT + x * PT) * D;
+          if (valid >= PT) {
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+              const uint32_t to = k_to[i % (16 * CH / 32)] + stage + i / (16 * CH / 32) * 16 * D;
+              copy16(to, k + i * 512);
+              copy16(to + kToV, v + i * 512);
+            }
+          } else {                                 // rows behind the end become zeros: 0 * garbage must not be NaN
+#pragma unroll
+            for (int i = 0; i < COPIES; ++i) {
+              const uint32_t to = k_to[i % (16 * CH / 32)] + stage + i / (16 * CH / 32) * 16 * D;
+              const int bytes = (i * 32 + lane) / CH < valid ? 16 : 0;
+              copy16(to, k + i * 512, bytes);
+              copy16(to + kToV, v + i * 512, bytes);
+            }
+          }
+          if (lane < 2) copy4(s_to + st * 16 + x * 8, s_from + ph);
         }
-      active = (active & ~(kAll << (st * PIECES))) | have << (st * PIECES);
+      active = (active & ~(kAll << (st * PG))) | have << (st * PG);
       load.next(a, row_tiles, warp);
       if (--left_load > 0) pages = pages_of(load);
     }
@@ -349,25 +351,31 @@ paged_q8_kernel(const Args a) {
     // accumulator j: elements 2 j, 2 j + 1 of a lane's piece of the head, heads 2 t, 2 t + 1
     constexpr int NT = D / 16;
     float o[H][NT][4];
-    float m[H][2], l[H][2];
+    float m[H][2], l[H][2], shift[H][2];
 #pragma unroll
     for (int h = 0; h < H; ++h) {
 #pragma unroll
       for (int j = 0; j < NT; ++j) o[h][j][0] = o[h][j][1] = o[h][j][2] = o[h][j][3] = 0.f;
       m[h][0] = m[h][1] = -INFINITY;
       l[h][0] = l[h][1] = 0.f;
+      shift[h][0] = shift[h][1] = 0.f;
     }
-    float unit_v = 0.f;                            // o is kept in units of this V scale
+    float unit_v = 0.f, per_unit = 0.f;            // o is kept in units of this V scale; 1 / unit_v
 
     for (int i = 0; i < n; ++i) {
       __pipeline_wait_prior(ST - 2);
       __syncwarp();                                // every lane's copies of this stage are in, every lane is done with the last
-      const uint32_t now = active >> (st * PIECES) & ((1u << PIECES) - 1);
+      const uint32_t now = active >> (st * PG) & kAll;
       issue(st == 0 ? ST - 1 : st - 1);
       if (now) {
         const uint8_t *ks = ring.k[st], *vs = ring.v[st];
-        const float4 scales = *reinterpret_cast<const float4*>(ring.s[st]);
-        const float k_scale[2] = {scales.x, scales.z}, v_scale[2] = {scales.y, scales.w};
+        float k_scale[PG], v_scale[PG];
+#pragma unroll
+        for (int x = 0; x < PG; ++x) {
+          const float2 u = *reinterpret_cast<const float2*>(&ring.s[st][2 * x]);
+          k_scale[x] = u.x;
+          v_scale[x] = u.y;
+        }
         // ---- S^T = K Q^T, 16 tokens at a time: tokens g (elements 0, 1) and g + 8 (2, 3), heads 2 t and 2 t + 1
         float s[H][PIECES][4];
 #pragma unroll
@@ -391,10 +399,12 @@ paged_q8_kernel(const Args a) {
           }
         }
         const int valid = len - (from_tile + i) * TILE - warp * WT;
-        if (valid < WT || now != (1u << PIECES) - 1) {
+        if (valid < WT || now != kAll) {
 #pragma unroll
           for (int x = 0; x < PIECES; ++x) {
-            const bool out0 = x * 16 + g >= valid || !(now >> x & 1), out1 = x * 16 + g + 8 >= valid || !(now >> x & 1);
+            const bool page_in = now >> (x * PG / PIECES) & 1;
+            if (!page_in) k_scale[x * PG / PIECES] = 1.f;
+            const bool out0 = x * 16 + g >= valid || !page_in, out1 = x * 16 + g + 8 >= valid || !page_in;
 #pragma unroll
             for (int h = 0; h < H; ++h) {
               if (out0) s[h][x][0] = s[h][x][1] = -INFINITY;
@@ -403,19 +413,24 @@ paged_q8_kernel(const Args a) {
           }
         }
         // ---- running softmax
-        float f[H][2][PIECES], mx[H][2];
+        float f[H][2][PG], mx[H][2];
         bool grown = false;
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            mx[h][y] = -INFINITY;
+            float best[PG];
 #pragma unroll
             for (int x = 0; x < PIECES; ++x) {
-              // above 0: masked scores stay -inf at a softmax scale of 0 too
-              f[h][y][x] = (now >> x & 1) ? fmaxf(sc[h][y] * k_scale[x], 1e-37f) : 1.f;
-              mx[h][y] = fmaxf(mx[h][y], fmaxf(s[h][x][y], s[h][x][2 + y]) * f[h][y][x]);
+              const float b = fmaxf(s[h][x][y], s[h][x][2 + y]);
+              best[x * PG / PIECES] = x * PG % PIECES == 0 ? b : fmaxf(best[x * PG / PIECES], b);
             }
+#pragma unroll
+            for (int x = 0; x < PG; ++x) {
+              f[h][y][x] = fmaxf(sc[h][y] * k_scale[x], 1e-37f);     // above 0: masked scores stay -inf at a softmax scale of 0 too
+              best[x] *= f[h][y][x];
+            }
+            mx[h][y] = PG == 2 ? fmaxf(best[0], best[PG - 1]) : best[0];
             mx[h][y] = fmaxf(mx[h][y], __shfl_xor_sync(0xffffffffu, mx[h][y], 4));
             mx[h][y] = fmaxf(mx[h][y], __shfl_xor_sync(0xffffffffu, mx[h][y], 8));
             mx[h][y] = fmaxf(mx[h][y], __shfl_xor_sync(0xffffffffu, mx[h][y], 16));
@@ -429,6 +444,7 @@ paged_q8_kernel(const Args a) {
               const float top = fmaxf(m[h][y], mx[h][y]);
               const float alpha = top == m[h][y] ? 1.f : exp2_approx(m[h][y] - top);
               m[h][y] = top;
+              shift[h][y] = top == -INFINITY ? 0.f : kProbShift - top;
               l[h][y] *= alpha;
 #pragma unroll
               for (int j = 0; j < NT; ++j) { o[h][j][y] *= alpha; o[h][j][2 + y] *= alpha; }
@@ -437,41 +453,39 @@ paged_q8_kernel(const Args a) {
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const float shift = m[h][y] == -INFINITY ? 0.f : m[h][y] - kProbShift;
+          for (int y = 0; y < 2; ++y)
 #pragma unroll
             for (int x = 0; x < PIECES; ++x) {
-              s[h][x][y] = exp2_approx(fmaf(s[h][x][y], f[h][y][x], -shift));
-              s[h][x][2 + y] = exp2_approx(fmaf(s[h][x][2 + y], f[h][y][x], -shift));
+              s[h][x][y] = exp2_approx(fmaf(s[h][x][y], f[h][y][x * PG / PIECES], shift[h][y]));
+              s[h][x][2 + y] = exp2_approx(fmaf(s[h][x][2 + y], f[h][y][x * PG / PIECES], shift[h][y]));
               l[h][y] += s[h][x][y] + s[h][x][2 + y];
             }
-          }
         // ---- O^T += V^T P^T, 16 tokens at a time: lane g holds the elements of its piece of V's rows
         constexpr int VB = D >= 128 ? 16 : 8;      // bytes of a piece
         const int piece = ((g & 1) << 2) | (g >> 1);
 #pragma unroll
         for (int x = 0; x < PIECES; ++x) {
-          if (PIECES == 2 && !(now >> x & 1)) continue;
+          if (PG == 2 && !(now >> x & 1)) continue;
           // V's scale joins the probabilities, relative to the unit that o is kept in; the unit follows the scale where
           // they are far apart, so that the probabilities stay inside fp16's normal range
-          if (v_scale[x] != unit_v) {              // the same for the whole warp
-            float ratio = unit_v > 0.f ? v_scale[x] / unit_v : 0.f;
-            if (v_scale[x] > 0.f && !(ratio <= 1.f && ratio >= 0.0625f)) {
-              const float change = unit_v / v_scale[x];
-#pragma unroll
-              for (int h = 0; h < H; ++h)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) o[h][j][e] *= change;
-              unit_v = v_scale[x];
-              ratio = 1.f;
-            }
+          const float vs_x = v_scale[x * PG / PIECES];
+          float ratio = vs_x * per_unit;
+          if (vs_x > 0.f && !(ratio <= 1.f && ratio >= 0.0625f)) {             // the same for the whole warp
+            const float change = unit_v / vs_x;
 #pragma unroll
             for (int h = 0; h < H; ++h)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) s[h][x][e] *= ratio;
+              for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[h][j][e] *= change;
+            unit_v = vs_x;
+            per_unit = 1.f / vs_x;
+            ratio = 1.f;
           }
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[h][x][e] *= ratio;
           uint32_t pb[H][2];
 #pragma unroll
           for (int h = 0; h < H; ++h) {
@@ -655,22 +669,24 @@ q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B
 template <typename T, int D>
 void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
   constexpr int ST = D == 64 ? 5 : 3;
-  constexpr int kMostH = 2;
   const int rep = a.nq / a.nkv;
-  a.unit_rows = rep <= 8 || kMostH == 1 ? 8 : 16;
+  a.unit_rows = rep <= 8 ? 8 : 16;
   const int row_tiles = (rep + a.unit_rows - 1) / a.unit_rows, red_rows = std::min(rep, a.unit_rows);
-  void (*kernel)(const Args) = a.unit_rows == 8 ? paged_q8_kernel<T, D, ST, 1> : paged_q8_kernel<T, D, ST, kMostH>;
+  constexpr int kMostPG = warp_tokens(D) / 16;
+  const int pg = a.bs % warp_tokens(D) ? kMostPG : 1;
+  void (*kernel)(const Args) = a.unit_rows == 8 ? (pg == 1 ? paged_q8_kernel<T, D, ST, 1, 1> : paged_q8_kernel<T, D, ST, 1, kMostPG>)
+                                                : (pg == 1 ? paged_q8_kernel<T, D, ST, 2, 1> : paged_q8_kernel<T, D, ST, 2, kMostPG>);
   auto smem_of = [](int rows) { return sizeof(WarpRing<D, ST>) * kWarps + 2 * rows * D * sizeof(float); };
   const size_t smem = smem_of(red_rows);
-  static std::atomic<int> residents[64][17] = {};  // blocks that an SM holds, per device and rows of a unit
+  static std::atomic<int> residents[64][2][17] = {};  // blocks that an SM holds, per device, pages of a warp, rows of a unit
   const int dev = q.get_device();
   TORCH_CHECK(dev >= 0 && dev < 64, "paged_attention_q8: device index out of range");
-  int resident = residents[dev][red_rows].load();
+  int resident = residents[dev][pg - 1][red_rows].load();
   if (!resident) {
     C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(16)));
     C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, smem));
     resident = std::max(resident, 1);
-    residents[dev][red_rows].store(resident);
+    residents[dev][pg - 1][red_rows].store(resident);
   }
   const int64_t most = (int64_t)a.rows * a.nkv * row_tiles * (((int64_t)a.width * a.bs + tile_tokens(D) - 1) / tile_tokens(D));
   a.grid = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)resident * at::cuda::getCurrentDeviceProperties()->multiProcessorCount, most));
@@ -698,7 +714,8 @@ at::Tensor paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const a
   a.ks = ks.data_ptr<float>(); a.vs = vs.data_ptr<float>();
   a.tables = tables.data_ptr<int>();
   a.out = out.data_ptr();
-  a.T = (int)q.size(0); a.nq = (int)q.size(1); a.nkv = (int)kc.size(1); a.bs = (int)kc.size(2); a.pages = kc.size(0);
+  a.T = (int)q.size(0); a.nq = (int)q.size(1); a.nkv = (int)kc.size(1); a.bs = (int)kc.size(2); a.pages = (int)kc.size(0);
+  TORCH_CHECK_VALUE(kc.size(0) * kc.size(1) < (int64_t)1 << 31, "paged_attention_q8: fewer than 2^31 pages times heads");
   a.width = (int)tables.size(1);
   a.scale = (float)(scale * 1.4426950408889634);
   auto st = at::cuda::getCurrentCUDAStream();
