@@ -62,14 +62,16 @@ __device__ __forceinline__ int tiles_of(const Args& a, int r) {
   return len > 0 ? (len + TILE - 1) / TILE : 0;
 }
 
-// The line is cut into min(blocks, tiles) shares: none is empty, and their bounds go by the lengths alone.
+// The line is cut into min(blocks, tiles) shares, the first ones a tile longer where it does not come out even: none is
+// empty, and their bounds go by the lengths alone.
 struct Place {
   int64_t total;                 // tiles of the line
-  int64_t shares;
+  int shares, longer;            // shares, and how many of them have share + 1 tiles
+  int64_t share;
   int64_t pos;                   // where share `index` begins (total, if there is no such share)
   int row;                       // row set that holds this position
   int64_t base;                  // where that row set begins
-  __device__ __forceinline__ int64_t begin(int64_t i) const { return i * total / shares; }
+  __device__ __forceinline__ int64_t begin(int i) const { return i * share + min(i, longer); }
 };
 
 // Exclusive prefix sums over the rows' tiles, `per_row` units each.  All threads of the block take part.
@@ -96,16 +98,22 @@ __device__ Place locate(const Args& a, int per_row, int index, int64_t* sh) {
   }
   Place p;
   p.total = total;
-  p.shares = max((int64_t)1, min((int64_t)a.grid, total));
+  p.shares = (int)max((int64_t)1, min((int64_t)a.grid, total));
+  if (total >> 31) {
+    p.share = total / p.shares;
+    p.longer = (int)(total - p.share * p.shares);
+  } else {
+    p.share = (uint32_t)total / (uint32_t)p.shares;
+    p.longer = (int)((uint32_t)total - (uint32_t)p.share * p.shares);
+  }
   p.pos = index < p.shares ? p.begin(index) : total;
-  const int64_t pos = p.pos;
   const int64_t first = before + inc - sum;
-  if (first <= pos && pos < first + sum) {
+  if (first <= p.pos && p.pos < first + sum) {
     int64_t at = first;
     int r = r0;
     for (; r < r1; ++r) {
       const int64_t n = (int64_t)tiles_of<TILE>(a, r) * per_row;
-      if (pos < at + n) break;
+      if (p.pos < at + n) break;
       at += n;
     }
     sh[4] = r;
@@ -211,21 +219,20 @@ paged_q8_kernel(const Args a) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int64_t sh_place[8];
   __shared__ float sh_m[kWarps][16], sh_l[kWarps][16];
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();                                   // after the wait: the joining kernel reads the lengths before its own
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   auto& ring = reinterpret_cast<WarpRing<D, ST>*>(smem)[warp];
   float* red = reinterpret_cast<float*>(smem + sizeof(WarpRing<D, ST>) * kWarps);   // [2][rows of a unit][D]
   const int rep = a.nq / a.nkv, row_tiles = (rep + 8 * H - 1) / (8 * H), per_row = a.nkv * row_tiles, red_rows = min(rep, 8 * H);
   T* out = static_cast<T*>(a.out);
 
-  // rows that see nothing are zero
-  for (int r = blockIdx.x; r < a.T; r += a.grid)
-    if (r >= a.rows || tiles_of<TILE>(a, r) == 0)
-      for (int i = tid; i < a.nq * D; i += kThreads) out[(int64_t)r * a.nq * D + i] = from_float<T>(0.f);
-
   const Place place = locate<TILE>(a, per_row, blockIdx.x, sh_place);
   const int64_t pos = place.pos;
+  // rows that see nothing are zero
+  for (int r = blockIdx.x * kWarps + warp; r < a.T; r += gridDim.x * kWarps)
+    if (r >= a.rows || tiles_of<TILE>(a, r) == 0)
+      for (int i = lane * 8; i < a.nq * D; i += 256) *reinterpret_cast<uint4*>(&out[(int64_t)r * a.nq * D + i]) = make_uint4(0, 0, 0, 0);
   if (pos >= place.total) return;
   int left = (int)(place.begin(blockIdx.x + 1) - pos), left_load = left;
   Cursor<TILE, WT> use;
@@ -233,8 +240,9 @@ paged_q8_kernel(const Args a) {
   use.step_off = TILE % a.bs;
   use.enter(a, place.row);
   {
-    const int unit = (int)((pos - place.base) / use.tiles);
-    use.tile = (int)((pos - place.base) - (int64_t)unit * use.tiles);
+    const uint32_t in_row = (uint32_t)(pos - place.base);        // a row set has less than 2^31 tiles
+    const int unit = (int)(in_row / (uint32_t)use.tiles);
+    use.tile = (int)in_row - unit * use.tiles;
     use.head = unit / row_tiles;
     use.rt = unit - use.head * row_tiles;
   }
@@ -602,48 +610,74 @@ paged_q8_kernel(const Args a) {
 }
 
 // Joins the parts of the units that the cuts divide: block c looks after the cut in front of block c + 1's share, if it
-// is the first cut inside its unit.
+// is the first cut inside its unit.  A warp joins a query head; where the cut lies is found while the attention kernel
+// still runs (it lets this one start only after the lengths are there).
+constexpr int kMostParts = 64;                    // weights of so many parts at a time
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) paged_q8_join_kernel(const Args a) {
   __shared__ int64_t sh_place[8];
+  __shared__ float sh_w[kWarps][kMostParts];
   pdl_trigger();
-  pdl_wait();
   const int rep = a.nq / a.nkv, row_tiles = (rep + a.unit_rows - 1) / a.unit_rows, per_row = a.nkv * row_tiles;
-  const int c = blockIdx.x + 1;
+  const int c = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Place place = locate<tile_tokens(D)>(a, per_row, c, sh_place);
   const int64_t pos = place.pos;
-  if (pos >= place.total) return;
-  const int tiles = tiles_of<tile_tokens(D)>(a, place.row);
-  const int unit = (int)((pos - place.base) / tiles);
-  const int64_t start = place.base + (int64_t)unit * tiles, stop = start + tiles;
-  if (pos == start || place.begin(c - 1) > start) return;
-  int last = c;                                    // last block with a part
-  while (last + 1 < place.shares && place.begin(last + 1) < stop) ++last;
-  const int head = unit / row_tiles, rt = unit % row_tiles, r = blockIdx.y;
-  if (r >= min(a.unit_rows, rep - rt * a.unit_rows)) return;
-  auto slot = [&](int x) { return x == c - 1 ? 2 * (c - 1) + 1 : 2 * x; };
-  float big = -INFINITY;
-  for (int x = c - 1; x <= last; ++x) big = fmaxf(big, a.part_ml[(slot(x) * 16 + r) * 2]);
-  T* out = static_cast<T*>(a.out) + ((int64_t)place.row * a.nq + head * rep + rt * a.unit_rows + r) * D;
-  for (int d = threadIdx.x; d < D; d += kThreads) {
-    float num = 0.f, den = 0.f;
-#pragma unroll 4
-    for (int x = c - 1; x <= last; ++x) {
-      const int s = slot(x) * 16 + r;
-      const float part = a.part_ml[s * 2 + 1];
-      const float w = part == 0.f ? 0.f : exp2_approx(a.part_ml[s * 2] - big);
-      if (w != 0.f) num += w * a.part_o[(int64_t)s * D + d];
-      den += w * part;
+  bool mine = pos < place.total;
+  int tiles = 1, unit = 0, parts = 0;
+  if (mine) {
+    tiles = tiles_of<tile_tokens(D)>(a, place.row);
+    unit = (int)((uint32_t)(pos - place.base) / (uint32_t)tiles);
+    const int64_t start = place.base + (int64_t)unit * tiles, stop = start + tiles;
+    mine = pos != start && place.begin(c - 1) <= start;
+    if (mine) {                                    // parts: the end of share c - 1 and the shares from c on that begin before `stop`
+      int last = c + (int)((uint32_t)(stop - 1 - pos) / (uint32_t)min(place.share + 1, (int64_t)1 << 31));      // no share is longer
+      while (last + 1 < place.shares && place.begin(last + 1) < stop) ++last;
+      parts = last - c + 2;
     }
-    out[d] = from_float<T>(den == 0.f ? 0.f : num / den);
+  }
+  pdl_wait();
+  if (!mine) return;
+  const int head = unit / row_tiles, rt = unit % row_tiles, rows_here = min(a.unit_rows, rep - rt * a.unit_rows);
+  auto slot = [&](int x) { return (x == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + x)) * 16; };
+  for (int r = warp; r < rows_here; r += kWarps) {
+    float big = -INFINITY;
+    for (int x = lane; x < parts; x += 32) big = fmaxf(big, a.part_ml[(slot(x) + r) * 2]);
+    big = warp_max(big);
+    constexpr int E = D / 32;
+    float num[E], den = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) num[e] = 0.f;
+    for (int x0 = 0; x0 < parts; x0 += kMostParts) {
+      const int here = min(kMostParts, parts - x0);
+      __syncwarp();
+      for (int x = lane; x < here; x += 32) {
+        const float2 ml = *reinterpret_cast<const float2*>(&a.part_ml[(slot(x0 + x) + r) * 2]);
+        const float w = ml.y == 0.f ? 0.f : exp2_approx(ml.x - big);
+        sh_w[warp][x] = w;
+        den += w * ml.y;
+      }
+      __syncwarp();
+#pragma unroll 8
+      for (int x = 0; x < here; ++x) {
+        const float w = sh_w[warp][x];
+        const float* from = a.part_o + (int64_t)(slot(x0 + x) + r) * D + lane;
+#pragma unroll
+        for (int e = 0; e < E; ++e) num[e] += w == 0.f ? 0.f : w * from[32 * e];
+      }
+    }
+    den = warp_sum(den);
+    T* out = static_cast<T*>(a.out) + ((int64_t)place.row * a.nq + head * rep + rt * a.unit_rows + r) * D + lane;
+#pragma unroll
+    for (int e = 0; e < E; ++e) out[32 * e] = from_float<T>(den == 0.f ? 0.f : num[e] / den);
   }
 }
 
 // tokens that every query row sees, and its sequence: trailing q_len tokens of each sequence, causal
 __global__ void __launch_bounds__(kThreads)
 q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B, int T, int* __restrict__ row_seq, int* __restrict__ row_len) {
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();
   __shared__ int sh[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   // rows before this block's sequence
@@ -696,7 +730,7 @@ void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
   a.part_ml = part_ml.data_ptr<float>();
   C10_CUDA_CHECK(launch_pdl(kernel, dim3(a.grid), dim3(kThreads), smem, st, a));
   if (a.grid > 1)
-    C10_CUDA_CHECK(launch_pdl(paged_q8_join_kernel<T, D>, dim3(a.grid - 1, red_rows), dim3(kThreads), 0, st, a));
+    C10_CUDA_CHECK(launch_pdl(paged_q8_join_kernel<T, D>, dim3(a.grid - 1), dim3(kThreads), 0, st, a));
 }
 
 }  // namespace
