@@ -11,10 +11,10 @@
 // has 8 significant bits, fp16 11; what falls below 2^-24 of a row's largest is lost).
 //
 // The bytes of the cache bound it.  The tokens of all units form one line that is cut evenly over the resident blocks
-// (whatever the lengths are), 64 at a time; a unit that a cut divides is written as partial (o, m, l) and joined by a
-// second kernel.  The cut goes by the lengths alone, so results do not depend on timing.  Inside a block each warp owns
-// 16 of the 64 tokens with its own cp.async ring, running maximum and sum: no barrier in the loop; the four streams meet
-// at the end of a unit.
+// (whatever the lengths are) and inside a block over its warps, 32 tokens at a time (16 at head dim 256).  A warp works
+// alone: its own cp.async ring, running maximum and sum, no barrier until its block's share is done.  A unit that lies
+// inside a warp's stretch is finished by the warp; parts of divided units meet at the end of the block, and a second
+// kernel joins what a cut between blocks divides.  The cuts go by the lengths alone, so results do not depend on timing.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/empty.h>
@@ -33,9 +33,8 @@ using namespace q8;
 namespace {
 
 constexpr int kThreads = 128, kWarps = 4;
-// tokens that a warp takes at a time: 8 KB of keys and values at head dims 128 and 256
-__host__ __device__ constexpr int warp_tokens(int D) { return D >= 256 ? 16 : 32; }
-__host__ __device__ constexpr int tile_tokens(int D) { return kWarps * warp_tokens(D); }
+// tokens of a tile, which a warp takes at a time: 8 KB of keys and values at head dims 128 and 256
+__host__ __device__ constexpr int tile_tokens(int D) { return D >= 256 ? 16 : 32; }
 // probabilities are carried times 2^10: fp16 keeps 11 bits of them down to 2^-24 of the largest
 constexpr float kProbShift = 10.f;
 
@@ -48,7 +47,9 @@ struct Args {
   const int* row_seq;            // [rows] sequence of a query row (null: the row's own number)
   const int* row_len;            // [rows] tokens it sees
   void* out;                     // [T, nq, D]
-  float *part_o, *part_ml;       // [2 * grid, 16, D], [2 * grid, 16, 2]
+  // parts of divided units, unit_rows each: 2 of every block (the unit that its share begins in, the one it ends in),
+  // behind them one of every warp (the unit that its stretch begins in)
+  float *part_o, *part_ml;       // [6 * grid, unit_rows, D], [6 * grid, unit_rows, 2]: maximum and sum
   int rows, T, width, nq, nkv, bs;
   int pages;
   int grid;                      // blocks that the line is cut over
@@ -68,19 +69,21 @@ struct Place {
   int64_t total;                 // tiles of the line
   int shares, longer;            // shares, and how many of them have share + 1 tiles
   int64_t share;
-  int64_t pos;                   // where share `index` begins (total, if there is no such share)
-  int row;                       // row set that holds this position
+  int64_t pos, end;              // stretch of the line
+  int row;                       // row set that holds `pos`
   int64_t base;                  // where that row set begins
   __device__ __forceinline__ int64_t begin(int i) const { return i * share + min(i, longer); }
 };
 
-// Exclusive prefix sums over the rows' tiles, `per_row` units each.  All threads of the block take part.
+// Exclusive prefix sums over the rows' tiles, `per_row` units each: the warp's stretch of share `index`, or all of the
+// share where `whole`; pos == end if there is none.  Every warp for itself.
 template <int TILE>
-__device__ Place locate(const Args& a, int per_row, int index, int64_t* sh) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (a.rows + kThreads - 1) / kThreads;
-  const int r0 = min(tid * per, a.rows), r1 = min(r0 + per, a.rows);
+__device__ Place locate(const Args& a, int per_row, int index, bool whole) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = (a.rows + 31) / 32;
+  const int r0 = min(lane * per, a.rows), r1 = min(r0 + per, a.rows);
   int64_t sum = 0;
+#pragma unroll 4
   for (int r = r0; r < r1; ++r) sum += tiles_of<TILE>(a, r);
   sum *= per_row;
   int64_t inc = sum;
@@ -89,39 +92,36 @@ __device__ Place locate(const Args& a, int per_row, int index, int64_t* sh) {
     const int64_t p = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += p;
   }
-  if (lane == 31) sh[warp] = inc;
-  __syncthreads();
-  int64_t before = 0, total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += sh[w];
-    total += sh[w];
-  }
   Place p;
-  p.total = total;
-  p.shares = (int)max((int64_t)1, min((int64_t)a.grid, total));
-  if (total >> 31) {
-    p.share = total / p.shares;
-    p.longer = (int)(total - p.share * p.shares);
+  p.total = __shfl_sync(0xffffffffu, inc, 31);
+  // at least a tile for each warp of a share
+  p.shares = (int)max((int64_t)1, min((int64_t)a.grid, (p.total + kWarps - 1) / kWarps));
+  if (p.total >> 31) {
+    p.share = p.total / p.shares;
+    p.longer = (int)(p.total - p.share * p.shares);
   } else {
-    p.share = (uint32_t)total / (uint32_t)p.shares;
-    p.longer = (int)((uint32_t)total - (uint32_t)p.share * p.shares);
+    p.share = (uint32_t)p.total / (uint32_t)p.shares;
+    p.longer = (int)((uint32_t)p.total - (uint32_t)p.share * p.shares);
   }
-  p.pos = index < p.shares ? p.begin(index) : total;
-  const int64_t first = before + inc - sum;
-  if (first <= p.pos && p.pos < first + sum) {
-    int64_t at = first;
-    int r = r0;
+  p.pos = p.end = p.total;
+  if (index < p.shares) {
+    const int64_t n = p.share + (index < p.longer), first = p.begin(index);
+    p.pos = whole ? first : first + n * warp / kWarps;
+    p.end = whole ? first + n : first + n * (warp + 1) / kWarps;
+  }
+  const int64_t first = inc - sum;
+  const uint32_t mine = __ballot_sync(0xffffffffu, first <= p.pos && p.pos < inc);
+  int r = r0;
+  int64_t at = first;
+  if (mine >> lane & 1)
     for (; r < r1; ++r) {
       const int64_t n = (int64_t)tiles_of<TILE>(a, r) * per_row;
       if (p.pos < at + n) break;
       at += n;
     }
-    sh[4] = r;
-    sh[5] = at;
-  }
-  __syncthreads();
-  p.row = (int)sh[4];
-  p.base = sh[5];
+  const int from = mine ? __ffs(mine) - 1 : 0;
+  p.row = __shfl_sync(0xffffffffu, r, from);
+  p.base = __shfl_sync(0xffffffffu, at, from);
   return p;
 }
 
@@ -155,17 +155,16 @@ __device__ __forceinline__ int swizzled(int r, int chunk) {
   return chunk ^ ((r >> 1) & 3);
 }
 
-// A warp's position on the line: row set, kv head and row tile of it, tile; the page that holds the warp's first token.
-template <int TILE, int WT>
+// A warp's position on the line: row set, kv head and row tile of it, tile; the page that holds the tile's first token.
+template <int TILE>
 struct Cursor {
   int row, head, rt, tile, tiles, len;
   int page, off;                                 // number in the sequence's table, token inside the page
   int step_page, step_off;                       // of a tile
   const int* table;
-  __device__ __forceinline__ int token(int warp) const { return tile * TILE + warp * WT; }
-  __device__ __forceinline__ void rewind(const Args& a, int warp) {
-    page = token(warp) / a.bs;
-    off = token(warp) - page * a.bs;
+  __device__ __forceinline__ void rewind(const Args& a) {
+    page = tile * TILE / a.bs;
+    off = tile * TILE - page * a.bs;
   }
   __device__ __forceinline__ void enter(const Args& a, int r) {
     row = r;
@@ -174,29 +173,40 @@ struct Cursor {
     if (row >= a.rows) return;
     len = min(a.row_len[row], a.width * a.bs);
     table = a.tables + (int64_t)(a.row_seq ? a.row_seq[row] : row) * a.width;
+    // the first 1024 pages' numbers on their way
+    const int line = (threadIdx.x & 31) * 32;
+    if (line < a.width) asm volatile("prefetch.global.L1 [%0];" ::"l"(table + line));
   }
-  __device__ __forceinline__ void next(const Args& a, int row_tiles, int warp) {
+  // whether a new unit begins
+  __device__ __forceinline__ bool next(const Args& a, int row_tiles) {
     if (++tile < tiles) {
       page += step_page;
       off += step_off;
       if (off >= a.bs) { off -= a.bs; ++page; }
-      return;
+      return false;
     }
-    tile = 0;
-    rewind(a, warp);
-    if (++rt < row_tiles) return;
+    tile = page = off = 0;
+    if (++rt < row_tiles) return true;
     rt = 0;
-    if (++head < a.nkv) return;
+    if (++head < a.nkv) return true;
     head = 0;
     enter(a, row + 1);
+    return true;
   }
 };
 
 template <int D, int ST>
 struct WarpRing {
-  uint8_t k[ST][warp_tokens(D) * D];
-  uint8_t v[ST][warp_tokens(D) * D];
+  uint8_t k[ST][tile_tokens(D) * D];
+  uint8_t v[ST][tile_tokens(D) * D];
   float s[ST][4];                                // scales of the 16-token halves: K, V, K, V
+};
+
+// Parts that a warp leaves to its block: of the unit that its stretch begins in (if it ended there), and of the one that
+// it ends in (if it did not).
+struct Left {
+  int head, tail;                                // 1: there is such a part; tail 2: the unit began in an earlier stretch
+  int row[2], col[2], rows[2];                   // row set, first query head, heads of the unit
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -215,39 +225,32 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
 template <typename T, int D, int ST, int H, int PG>
 __global__ void __launch_bounds__(kThreads)
 paged_q8_kernel(const Args a) {
-  constexpr int WT = warp_tokens(D), TILE = tile_tokens(D), PIECES = WT / 16, PT = WT / PG;
+  constexpr int TILE = tile_tokens(D), PIECES = TILE / 16, PT = TILE / PG;
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int64_t sh_place[8];
-  __shared__ float sh_m[kWarps][16], sh_l[kWarps][16];
+  __shared__ float2 sh_ml[kWarps][2][8 * H];       // maximum and sum of the parts left to the block
+  __shared__ Left sh_left[kWarps];
   pdl_wait();
   pdl_trigger();                                   // after the wait: the joining kernel reads the lengths before its own
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   auto& ring = reinterpret_cast<WarpRing<D, ST>*>(smem)[warp];
-  float* red = reinterpret_cast<float*>(smem + sizeof(WarpRing<D, ST>) * kWarps);   // [2][rows of a unit][D]
-  const int rep = a.nq / a.nkv, row_tiles = (rep + 8 * H - 1) / (8 * H), per_row = a.nkv * row_tiles, red_rows = min(rep, 8 * H);
+  const int rep = a.nq / a.nkv, row_tiles = (rep + 8 * H - 1) / (8 * H), per_row = a.nkv * row_tiles;
   T* out = static_cast<T*>(a.out);
 
-  const Place place = locate<TILE>(a, per_row, blockIdx.x, sh_place);
-  const int64_t pos = place.pos;
-  // rows that see nothing are zero
-  for (int r = blockIdx.x * kWarps + warp; r < a.T; r += gridDim.x * kWarps)
-    if (r >= a.rows || tiles_of<TILE>(a, r) == 0)
-      for (int i = lane * 8; i < a.nq * D; i += 256) *reinterpret_cast<uint4*>(&out[(int64_t)r * a.nq * D + i]) = make_uint4(0, 0, 0, 0);
-  if (pos >= place.total) return;
-  int left = (int)(place.begin(blockIdx.x + 1) - pos), left_load = left;
-  Cursor<TILE, WT> use;
+  const Place place = locate<TILE>(a, per_row, blockIdx.x, false);
+  int left = (int)(place.end - place.pos), left_load = left;
+  Cursor<TILE> use;
   use.step_page = TILE / a.bs;
   use.step_off = TILE % a.bs;
-  use.enter(a, place.row);
-  {
-    const uint32_t in_row = (uint32_t)(pos - place.base);        // a row set has less than 2^31 tiles
+  if (left > 0) {
+    use.enter(a, place.row);
+    const uint32_t in_row = (uint32_t)(place.pos - place.base);        // a row set has less than 2^31 tiles
     const int unit = (int)(in_row / (uint32_t)use.tiles);
     use.tile = (int)in_row - unit * use.tiles;
     use.head = unit / row_tiles;
     use.rt = unit - use.head * row_tiles;
+    use.rewind(a);
   }
-  use.rewind(a, warp);
-  Cursor<TILE, WT> load = use;
+  Cursor<TILE> load = use;
 
   // a lane copies the 16-byte chunks lane, lane + 32, ... of PT rows that lie one behind the other
   constexpr int CH = D / 16, COPIES = PT * CH / 32;
@@ -263,14 +266,15 @@ paged_q8_kernel(const Args a) {
   const float* s_from = lane & 1 ? a.vs : a.ks;
   const int64_t page_bytes = (int64_t)a.bs * D;
   struct Pages { int id[PG]; };                    // -1: none
-  auto pages_of = [&](const Cursor<TILE, WT>& c) {
+  auto pages_of = [&](const Cursor<TILE>& c) {
     Pages p;
-    const int tok = c.token(warp);
-    p.id[0] = tok < c.len ? c.table[c.page] : -1;
+    const int tok = c.tile * TILE;
+    p.id[0] = c.table[c.page];
     if constexpr (PG == 2) p.id[1] = tok + PT >= c.len ? -1 : c.off + PT < a.bs ? p.id[0] : c.table[c.page + 1];
     return p;
   };
-  Pages pages = pages_of(load);
+  Pages pages = {};
+  if (left > 0) pages = pages_of(load);
   constexpr uint32_t kAll = (1u << PG) - 1;
   uint32_t active = 0;                             // pages of the stages that hold tokens
   auto issue = [&](int st) {
@@ -282,10 +286,10 @@ paged_q8_kernel(const Args a) {
           have |= 1u << x;
           int off = load.off + PT * x;
           if (x > 0 && off >= a.bs) off -= a.bs;
-          const int ph = pages.id[x] * a.nkv + load.head, valid = load.len - load.token(warp) - PT * x;
+          const int ph = pages.id[x] * a.nkv + load.head, valid = load.len - load.tile * TILE - PT * x;
           const int64_t at = ph * page_bytes + off * D + lane * 16;
           const uint8_t *k = a.kc + at, *v = a.vc + at;
-          const uint32_t stage = (st * WT + x * PT) * D;
+          const uint32_t stage = (st * TILE + x * PT) * D;
           if (valid >= PT) {
 #pragma unroll
             for (int i = 0; i < COPIES; ++i) {
@@ -305,8 +309,15 @@ paged_q8_kernel(const Args a) {
           if (lane < 2) copy4(s_to + st * 16 + x * 8, s_from + ph);
         }
       active = (active & ~(kAll << (st * PG))) | have << (st * PG);
-      load.next(a, row_tiles, warp);
-      if (--left_load > 0) pages = pages_of(load);
+      const bool fresh = load.next(a, row_tiles);
+      if (--left_load > 0) {
+        pages = pages_of(load);
+        if (fresh) {                               // the next unit's queries on their way
+          const int first = load.head * rep + load.rt * 8 * H, bytes = min(8 * H, rep - load.rt * 8 * H) * D * 2;
+          const char* q = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + load.row * a.q_row + (int64_t)first * D);
+          for (int i = lane * 128; i < bytes; i += 32 * 128) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + i));
+        }
+      }
     }
     __pipeline_commit();
   };
@@ -314,9 +325,9 @@ paged_q8_kernel(const Args a) {
   for (int s = 0; s < ST - 1; ++s) issue(s);
 
   int st = 0;
-  bool first_unit = true;
+  if (lane == 0) sh_left[warp].head = sh_left[warp].tail = 0;
   while (left > 0) {
-    // ---------------- a unit, or the part of it in this block's share
+    // ---------------- a unit, or the part of it in this warp's stretch
     const int head = use.head, rt = use.rt, rows_here = min(8 * H, rep - rt * 8 * H);
     const int from_tile = use.tile, n = min(use.tiles - use.tile, left);
     const int row = use.row, tiles = use.tiles, len = use.len;
@@ -406,8 +417,8 @@ paged_q8_kernel(const Args a) {
             }
           }
         }
-        const int valid = len - (from_tile + i) * TILE - warp * WT;
-        if (valid < WT || now != kAll) {
+        const int valid = len - (from_tile + i) * TILE;
+        if (valid < TILE || now != kAll) {
 #pragma unroll
           for (int x = 0; x < PIECES; ++x) {
             const bool page_in = now >> (x * PG / PIECES) & 1;
@@ -535,142 +546,182 @@ paged_q8_kernel(const Args a) {
     }
     left -= n;
     use.tile += n - 1;
-    use.next(a, row_tiles, warp);
+    use.next(a, row_tiles);
 
-    // ---------------- the four streams of the unit meet
+    // ---------------- the end of the unit, or of the stretch
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l[h][y] += __shfl_xor_sync(0xffffffffu, l[h][y], d);
-        if (g == 0) { sh_m[warp][8 * h + 2 * t + y] = m[h][y]; sh_l[warp][8 * h + 2 * t + y] = l[h][y]; }
-      }
-    __syncthreads();
-    float w[H][2];
-#pragma unroll
-    for (int h = 0; h < H; ++h)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        float top = -INFINITY;
-#pragma unroll
-        for (int x = 0; x < kWarps; ++x) top = fmaxf(top, sh_m[x][8 * h + 2 * t + y]);
-        w[h][y] = m[h][y] == -INFINITY && l[h][y] == 0.f ? 0.f : exp2_approx(m[h][y] - top) * unit_v;
-      }
+    // accumulators j and j + 1 of a head: 4 neighbouring elements
     constexpr int VB = D >= 128 ? 16 : 8;
     const int piece = ((g & 1) << 2) | (g >> 1);
+    auto column = [&](int j) { return j * 2 / VB * 8 * VB + piece * VB + j * 2 % VB; };
+    const bool begins = from_tile == 0, ends = from_tile + n == tiles;
+    if (begins && ends) {
 #pragma unroll
-    for (int pass = 0; pass < 2; ++pass) {
-      if ((warp >> 1) == pass) {
-        float* to = red + (warp & 1) * red_rows * D;
+      for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int h = 0; h < H; ++h)
+        for (int y = 0; y < 2; ++y) {
+          const int r = 8 * h + 2 * t + y;
+          if (r >= rows_here) continue;
+          const float w = l[h][y] == 0.f ? 0.f : unit_v / l[h][y];
+          T* to = out + ((int64_t)row * a.nq + head * rep + rt * 8 * H + r) * D;
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-            if (8 * h + 2 * t + y < rows_here)
+          for (int j = 0; j < NT; j += 4) {        // 8 elements
+            T x[8];
 #pragma unroll
-              for (int j = 0; j < NT; j += 2) {
-                float4& x = *reinterpret_cast<float4*>(&to[(8 * h + 2 * t + y) * D + (j * 2 / VB) * 8 * VB + piece * VB + j * 2 % VB]);
-                float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (w[h][y] != 0.f)
-                  z = make_float4(o[h][j][y] * w[h][y], o[h][j][2 + y] * w[h][y], o[h][j + 1][y] * w[h][y], o[h][j + 1][2 + y] * w[h][y]);
-                if (pass) { z.x += x.x; z.y += x.y; z.z += x.z; z.w += x.w; }
-                x = z;
-              }
-      }
-      __syncthreads();
-    }
-    const bool whole = from_tile == 0 && n == tiles;
-    const int slot = 2 * blockIdx.x + (first_unit && from_tile > 0 ? 0 : 1);
-    for (int i = tid * 2; i < rows_here * D; i += kThreads * 2) {
-      const int r = i / D, d = i % D;
-      float big = -INFINITY, sum = 0.f;
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x) big = fmaxf(big, sh_m[x][r]);
-#pragma unroll
-      for (int x = 0; x < kWarps; ++x)
-        if (sh_l[x][r] != 0.f) sum += sh_l[x][r] * exp2_approx(sh_m[x][r] - big);
-      const float2 u = *reinterpret_cast<const float2*>(&red[i]), v = *reinterpret_cast<const float2*>(&red[red_rows * D + i]);
-      const float2 val = make_float2(u.x + v.x, u.y + v.y);
-      if (whole) {
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        T pair[2] = {from_float<T>(val.x * inv), from_float<T>(val.y * inv)};
-        *reinterpret_cast<uint32_t*>(&out[((int64_t)row * a.nq + head * rep + rt * 8 * H + r) * D + d]) = *reinterpret_cast<const uint32_t*>(pair);
-      } else {
-        *reinterpret_cast<float2*>(&a.part_o[((int64_t)slot * 16 + r) * D + d]) = val;
-        if (d == 0) {
-          a.part_ml[(slot * 16 + r) * 2] = big;
-          a.part_ml[(slot * 16 + r) * 2 + 1] = sum;
+            for (int e = 0; e < 4; ++e) {
+              x[2 * e] = from_float<T>(o[h][j + e][y] * w);
+              x[2 * e + 1] = from_float<T>(o[h][j + e][2 + y] * w);
+            }
+            *reinterpret_cast<uint4*>(to + column(j)) = *reinterpret_cast<const uint4*>(x);
+          }
         }
+    } else {
+      // a part: the stretch's first unit goes to memory (the ring is in use), its last one into the ring
+      float* to;
+      if (ends) {
+        to = a.part_o + (int64_t)(2 * a.grid + blockIdx.x * kWarps + warp) * a.unit_rows * D;
+      } else {
+        __pipeline_wait_prior(0);
+        __syncwarp();
+        to = reinterpret_cast<float*>(&ring);
+      }
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int r = 8 * h + 2 * t + y;
+          if (r >= rows_here) continue;
+          if (g == 0) sh_ml[warp][ends ? 0 : 1][r] = make_float2(m[h][y], l[h][y]);
+#pragma unroll
+          for (int j = 0; j < NT; j += 2)
+            *reinterpret_cast<float4*>(&to[r * D + column(j)]) =
+                make_float4(o[h][j][y] * unit_v, o[h][j][2 + y] * unit_v, o[h][j + 1][y] * unit_v, o[h][j + 1][2 + y] * unit_v);
+        }
+      if (lane == 0) {
+        Left& x = sh_left[warp];
+        const int i = ends ? 0 : 1;
+        if (ends) x.head = 1;
+        else x.tail = begins ? 1 : 2;
+        x.row[i] = row;
+        x.col[i] = head * rep + rt * 8 * H;
+        x.rows[i] = rows_here;
       }
     }
-    first_unit = false;
-    __syncthreads();
   }
+  __pipeline_wait_prior(0);
+
+  // ---------------- parts of the block's warps meet; the list is in the order of the line
+  __syncthreads();
+  auto join_parts = [&](int first, int last, bool continued, bool finished) {        // part 2 w: warp w's head, 2 w + 1: its tail
+    const Left& x = sh_left[last >> 1];
+    const int i = last & 1, rows_here = x.rows[i];
+    for (int e = tid * 4; e < rows_here * D; e += kThreads * 4) {
+      const int r = e / D;
+      float big = -INFINITY, den = 0.f;
+      float4 num = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int p = first; p <= last; ++p)
+        if (p & 1 ? sh_left[p >> 1].tail : sh_left[p >> 1].head) big = fmaxf(big, sh_ml[p >> 1][p & 1][r].x);
+      for (int p = first; p <= last; ++p) {
+        if (!(p & 1 ? sh_left[p >> 1].tail : sh_left[p >> 1].head)) continue;
+        const float2 ml = sh_ml[p >> 1][p & 1][r];
+        if (ml.y == 0.f) continue;
+        const float* from = p & 1 ? reinterpret_cast<const float*>(&reinterpret_cast<WarpRing<D, ST>*>(smem)[p >> 1])
+                                  : a.part_o + (int64_t)(2 * a.grid + blockIdx.x * kWarps + (p >> 1)) * a.unit_rows * D;
+        const float4 v = *reinterpret_cast<const float4*>(&from[e]);
+        const float w = exp2_approx(ml.x - big);
+        den += w * ml.y;
+        num.x += w * v.x; num.y += w * v.y; num.z += w * v.z; num.w += w * v.w;
+      }
+      if (finished && !continued) {
+        const float inv = den == 0.f ? 0.f : 1.f / den;
+        const T y[4] = {from_float<T>(num.x * inv), from_float<T>(num.y * inv), from_float<T>(num.z * inv), from_float<T>(num.w * inv)};
+        *reinterpret_cast<uint2*>(&out[((int64_t)x.row[i] * a.nq + x.col[i]) * D + e]) = *reinterpret_cast<const uint2*>(y);
+      } else {
+        const int64_t slot = 2 * blockIdx.x + (continued ? 0 : 1);
+        *reinterpret_cast<float4*>(&a.part_o[slot * a.unit_rows * D + e]) = num;
+        if (e % D == 0) *reinterpret_cast<float2*>(&a.part_ml[(slot * a.unit_rows + r) * 2]) = make_float2(big, den);
+      }
+    }
+  };
+  int first = -1;
+  bool continued = false;
+  for (int w = 0; w < kWarps; ++w) {
+    if (sh_left[w].head) {
+      if (first < 0) { first = 2 * w; continued = true; }
+      join_parts(first, 2 * w, continued, true);
+      first = -1;
+    }
+    if (sh_left[w].tail && first < 0) { first = 2 * w + 1; continued = sh_left[w].tail == 2; }
+  }
+  if (first >= 0) {
+    int last = kWarps - 1;
+    while (!sh_left[last].tail) --last;            // warps behind it have no stretch
+    join_parts(first, 2 * last + 1, continued, false);
+  }
+  // rows that see nothing are zero
+  for (int r = blockIdx.x * kWarps + warp; r < a.T; r += gridDim.x * kWarps)
+    if (r >= a.rows || tiles_of<TILE>(a, r) == 0)
+      for (int i = lane * 8; i < a.nq * D; i += 256) *reinterpret_cast<uint4*>(&out[(int64_t)r * a.nq * D + i]) = make_uint4(0, 0, 0, 0);
 }
 
-// Joins the parts of the units that the cuts divide: block c looks after the cut in front of block c + 1's share, if it
-// is the first cut inside its unit.  A warp joins a query head; where the cut lies is found while the attention kernel
-// still runs (it lets this one start only after the lengths are there).
-constexpr int kMostParts = 64;                    // weights of so many parts at a time
-
+// Joins the parts of the units that the cuts between blocks divide: block (c, r) looks after query head r of the unit that
+// the cut in front of share c + 1 divides, if it is the first cut inside its unit.  Where the cut lies is found while the
+// attention kernel still runs (it lets this one start only after the lengths are there).  Few and short loops: a handful
+// of warps run through here once, and waiting for code to arrive is a good part of what that takes.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) paged_q8_join_kernel(const Args a) {
-  __shared__ int64_t sh_place[8];
-  __shared__ float sh_w[kWarps][kMostParts];
+  __shared__ float sh_num[kWarps][D], sh_den[kWarps];
   pdl_trigger();
   const int rep = a.nq / a.nkv, row_tiles = (rep + a.unit_rows - 1) / a.unit_rows, per_row = a.nkv * row_tiles;
-  const int c = blockIdx.x + 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const Place place = locate<tile_tokens(D)>(a, per_row, c, sh_place);
+  const int c = blockIdx.x + 1, r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Place place = locate<tile_tokens(D)>(a, per_row, c, true);
   const int64_t pos = place.pos;
-  bool mine = pos < place.total;
-  int tiles = 1, unit = 0, parts = 0;
-  if (mine) {
-    tiles = tiles_of<tile_tokens(D)>(a, place.row);
-    unit = (int)((uint32_t)(pos - place.base) / (uint32_t)tiles);
-    const int64_t start = place.base + (int64_t)unit * tiles, stop = start + tiles;
-    mine = pos != start && place.begin(c - 1) <= start;
-    if (mine) {                                    // parts: the end of share c - 1 and the shares from c on that begin before `stop`
-      int last = c + (int)((uint32_t)(stop - 1 - pos) / (uint32_t)min(place.share + 1, (int64_t)1 << 31));      // no share is longer
-      while (last + 1 < place.shares && place.begin(last + 1) < stop) ++last;
-      parts = last - c + 2;
-    }
-  }
+  if (pos >= place.total) return;
+  const int tiles = tiles_of<tile_tokens(D)>(a, place.row);
+  const int unit = (int)((uint32_t)(pos - place.base) / (uint32_t)tiles);
+  const int64_t start = place.base + (int64_t)unit * tiles, stop = start + tiles;
+  const int head = unit / row_tiles, rt = unit - head * row_tiles;
+  if (pos == start || place.begin(c - 1) > start || r >= min(a.unit_rows, rep - rt * a.unit_rows)) return;
+  // parts: the end of share c - 1 and the shares from c on that begin before `stop`
+  int last = c + (int)((uint32_t)(stop - 1 - pos) / (uint32_t)min(place.share + 1, (int64_t)1 << 31));      // no share is longer
+  while (last + 1 < place.shares && place.begin(last + 1) < stop) ++last;
+  const int parts = last - c + 2;
   pdl_wait();
-  if (!mine) return;
-  const int head = unit / row_tiles, rt = unit % row_tiles, rows_here = min(a.unit_rows, rep - rt * a.unit_rows);
-  auto slot = [&](int x) { return (x == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + x)) * 16; };
-  for (int r = warp; r < rows_here; r += kWarps) {
-    float big = -INFINITY;
-    for (int x = lane; x < parts; x += 32) big = fmaxf(big, a.part_ml[(slot(x) + r) * 2]);
-    big = warp_max(big);
-    constexpr int E = D / 32;
-    float num[E], den = 0.f;
+  auto slot = [&](int x) { return (x == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + x)) * a.unit_rows + r; };
+  float big = -INFINITY;
+  for (int x = lane; x < parts; x += 32) big = fmaxf(big, a.part_ml[slot(x) * 2]);
+  big = warp_max(big);
+  constexpr int E = D / 32;                        // neighbouring elements of a lane
+  float num[E], den = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) num[e] = 0.f;
-    for (int x0 = 0; x0 < parts; x0 += kMostParts) {
-      const int here = min(kMostParts, parts - x0);
-      __syncwarp();
-      for (int x = lane; x < here; x += 32) {
-        const float2 ml = *reinterpret_cast<const float2*>(&a.part_ml[(slot(x0 + x) + r) * 2]);
-        const float w = ml.y == 0.f ? 0.f : exp2_approx(ml.x - big);
-        sh_w[warp][x] = w;
-        den += w * ml.y;
-      }
-      __syncwarp();
-#pragma unroll 8
-      for (int x = 0; x < here; ++x) {
-        const float w = sh_w[warp][x];
-        const float* from = a.part_o + (int64_t)(slot(x0 + x) + r) * D + lane;
+  for (int e = 0; e < E; ++e) num[e] = 0.f;
+#pragma unroll 4
+  for (int x = warp; x < parts; x += kWarps) {     // a warp takes every fourth part
+    const float2 ml = *reinterpret_cast<const float2*>(&a.part_ml[slot(x) * 2]);
+    const float* from = a.part_o + (int64_t)slot(x) * D + lane * E;
+    const float w = ml.y == 0.f ? 0.f : exp2_approx(ml.x - big);
+    den = fmaf(w, ml.y, den);
 #pragma unroll
-        for (int e = 0; e < E; ++e) num[e] += w == 0.f ? 0.f : w * from[32 * e];
-      }
+    for (int e = 0; e < E; e += 2) {
+      const float2 v = *reinterpret_cast<const float2*>(from + e);
+      num[e] = fmaf(w, v.x, num[e]);
+      num[e + 1] = fmaf(w, v.y, num[e + 1]);
     }
-    den = warp_sum(den);
-    T* out = static_cast<T*>(a.out) + ((int64_t)place.row * a.nq + head * rep + rt * a.unit_rows + r) * D + lane;
-#pragma unroll
-    for (int e = 0; e < E; ++e) out[32 * e] = from_float<T>(den == 0.f ? 0.f : num[e] / den);
   }
+#pragma unroll
+  for (int e = 0; e < E; ++e) sh_num[warp][lane * E + e] = num[e];
+  if (lane == 0) sh_den[warp] = den;
+  __syncthreads();
+  den = (sh_den[0] + sh_den[1]) + (sh_den[2] + sh_den[3]);
+  const float inv = den == 0.f ? 0.f : 1.f / den;
+  T* out = static_cast<T*>(a.out) + ((int64_t)place.row * a.nq + head * rep + rt * a.unit_rows + r) * D;
+  for (int d = threadIdx.x; d < D; d += kThreads)
+    out[d] = from_float<T>(((sh_num[0][d] + sh_num[1][d]) + (sh_num[2][d] + sh_num[3][d])) * inv);
 }
 
 // tokens that every query row sees, and its sequence: trailing q_len tokens of each sequence, causal
@@ -705,32 +756,34 @@ void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
   constexpr int ST = D == 64 ? 5 : 3;
   const int rep = a.nq / a.nkv;
   a.unit_rows = rep <= 8 ? 8 : 16;
-  const int row_tiles = (rep + a.unit_rows - 1) / a.unit_rows, red_rows = std::min(rep, a.unit_rows);
-  constexpr int kMostPG = warp_tokens(D) / 16;
-  const int pg = a.bs % warp_tokens(D) ? kMostPG : 1;
+  const int row_tiles = (rep + a.unit_rows - 1) / a.unit_rows;
+  constexpr int kMostPG = tile_tokens(D) / 16;
+  const int pg = a.bs % tile_tokens(D) ? kMostPG : 1;
   void (*kernel)(const Args) = a.unit_rows == 8 ? (pg == 1 ? paged_q8_kernel<T, D, ST, 1, 1> : paged_q8_kernel<T, D, ST, 1, kMostPG>)
                                                 : (pg == 1 ? paged_q8_kernel<T, D, ST, 2, 1> : paged_q8_kernel<T, D, ST, 2, kMostPG>);
-  auto smem_of = [](int rows) { return sizeof(WarpRing<D, ST>) * kWarps + 2 * rows * D * sizeof(float); };
-  const size_t smem = smem_of(red_rows);
-  static std::atomic<int> residents[64][2][17] = {};  // blocks that an SM holds, per device, pages of a warp, rows of a unit
+  constexpr size_t smem = sizeof(WarpRing<D, ST>) * kWarps;
+  static_assert(sizeof(WarpRing<D, ST>) >= 16 * D * sizeof(float), "a part fits the ring");
+  static std::atomic<int> residents[64][4] = {};   // blocks that a device holds, per kernel
   const int dev = q.get_device();
   TORCH_CHECK(dev >= 0 && dev < 64, "paged_attention_q8: device index out of range");
-  int resident = residents[dev][pg - 1][red_rows].load();
+  std::atomic<int>& known = residents[dev][(pg - 1) * 2 + a.unit_rows / 16];
+  int resident = known.load();
   if (!resident) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_of(16)));
+    int sms = 0;
+    C10_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
     C10_CUDA_CHECK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, smem));
-    resident = std::max(resident, 1);
-    residents[dev][pg - 1][red_rows].store(resident);
+    resident = std::max(resident, 1) * sms;
+    known.store(resident);
   }
   const int64_t most = (int64_t)a.rows * a.nkv * row_tiles * (((int64_t)a.width * a.bs + tile_tokens(D) - 1) / tile_tokens(D));
-  a.grid = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)resident * at::cuda::getCurrentDeviceProperties()->multiProcessorCount, most));
-  auto part_o = at::empty({2 * a.grid, 16, D}, q.options().dtype(at::kFloat));
-  auto part_ml = at::empty({2 * a.grid, 16, 2}, q.options().dtype(at::kFloat));
-  a.part_o = part_o.data_ptr<float>();
-  a.part_ml = part_ml.data_ptr<float>();
+  a.grid = (int)std::max<int64_t>(1, std::min<int64_t>(resident, (most + kWarps - 1) / kWarps));
+  const int64_t rows = (int64_t)(2 + kWarps) * a.grid * a.unit_rows;
+  auto part = at::empty({rows * (D + 2)}, q.options().dtype(at::kFloat));
+  a.part_o = part.data_ptr<float>();
+  a.part_ml = a.part_o + rows * D;
   C10_CUDA_CHECK(launch_pdl(kernel, dim3(a.grid), dim3(kThreads), smem, st, a));
-  if (a.grid > 1)
-    C10_CUDA_CHECK(launch_pdl(paged_q8_join_kernel<T, D>, dim3(a.grid - 1), dim3(kThreads), 0, st, a));
+  if (a.grid > 1) C10_CUDA_CHECK(launch_pdl(paged_q8_join_kernel<T, D>, dim3(a.grid - 1, std::min(rep, a.unit_rows)), dim3(kThreads), 0, st, a));
 }
 
 }  // namespace
