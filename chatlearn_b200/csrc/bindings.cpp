@@ -127,6 +127,7 @@ void kv_append_q8(const at::Tensor& k, const at::Tensor& v, at::Tensor kc, at::T
 at::Tensor paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
                               const at::Tensor& vs, const at::Tensor& tables, const at::Tensor& lens,
                               const c10::optional<at::Tensor>& news, double scale);
+int64_t paged_attention_q8_last_status();
 std::vector<at::Tensor> token_logprob_fwd(const at::Tensor& z, const at::Tensor& tokens, int64_t n, double inv_temp);
 at::Tensor token_logprob_bwd(const at::Tensor& z, const at::Tensor& tokens, const at::Tensor& ent, const at::Tensor& stats,
                              const at::Tensor& ids, const c10::optional<at::Tensor>& g_lp, const c10::optional<at::Tensor>& g_ent,
@@ -206,6 +207,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attn_bwd_sm100_last_status", &attn_bwd_sm100_last_status);
   m.def("kv_append_q8", &kv_append_q8);
   m.def("paged_attention_q8", &paged_attention_q8);
+  m.def("paged_attention_q8_last_status", &paged_attention_q8_last_status);
   m.def("token_logprob_fwd", &token_logprob_fwd);
   m.def("token_logprob_bwd", &token_logprob_bwd);
   m.def("source_hash", []() { return std::string(clb200_source_hash()); });

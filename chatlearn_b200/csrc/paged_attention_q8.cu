@@ -26,6 +26,7 @@
 #include <type_traits>
 
 #include "q8.cuh"
+#include "q8_attention.h"
 
 using namespace cl;
 using namespace q8;
@@ -45,7 +46,7 @@ struct Args {
   const float *ks, *vs;          // [pages, nkv]
   const int* tables;             // [B, width]
   const int* row_seq;            // [rows] sequence of a query row (null: the row's own number)
-  const int* row_len;            // [rows] tokens it sees
+  const int* row_len;            // [rows] tokens it sees (kElsewhere: another kernel's row)
   void* out;                     // [T, nq, D]
   // parts of divided units, unit_rows each: 2 of every block (the unit that its share begins in, the one it ends in),
   // behind them one of every warp (the unit that its stretch begins in)
@@ -56,6 +57,10 @@ struct Args {
   int unit_rows;                 // query heads of a unit: 8 or 16
   float scale;                   // softmax scale times log2 e
 };
+
+constexpr int kElsewhere = -(1 << 30);
+// sequences with fewer new tokens go row by row; the others in tiles of 128 / rep tokens, which pay from here on
+constexpr int kChunkTokens = 8;
 
 template <int TILE>
 __device__ __forceinline__ int tiles_of(const Args& a, int r) {
@@ -665,7 +670,7 @@ paged_q8_kernel(const Args a) {
   }
   // rows that see nothing are zero
   for (int r = blockIdx.x * kWarps + warp; r < a.T; r += gridDim.x * kWarps)
-    if (r >= a.rows || tiles_of<TILE>(a, r) == 0)
+    if (r >= a.rows || (tiles_of<TILE>(a, r) == 0 && a.row_len[r] != kElsewhere))
       for (int i = lane * 8; i < a.nq * D; i += 256) *reinterpret_cast<uint4*>(&out[(int64_t)r * a.nq * D + i]) = make_uint4(0, 0, 0, 0);
 }
 
@@ -726,7 +731,7 @@ __global__ void __launch_bounds__(kThreads) paged_q8_join_kernel(const Args a) {
 
 // tokens that every query row sees, and its sequence: trailing q_len tokens of each sequence, causal
 __global__ void __launch_bounds__(kThreads)
-q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B, int T, int* __restrict__ row_seq, int* __restrict__ row_len) {
+q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B, int T, int min_chunk, int* __restrict__ row_seq, int* __restrict__ row_len) {
   pdl_wait();
   pdl_trigger();
   __shared__ int sh[kWarps];
@@ -744,10 +749,10 @@ q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B
     for (int r = before + tid; r < T; r += kThreads) { row_seq[r] = 0; row_len[r] = 0; }
     return;
   }
-  const int n = max(news[b], 0);
+  const int n = max(news[b], 0), len = lens[b];
   for (int i = tid; i < n && before + i < T; i += kThreads) {
     row_seq[before + i] = b;
-    row_len[before + i] = max(lens[b] - n + 1 + i, 0);
+    row_len[before + i] = n >= min_chunk ? kElsewhere : max(len - n + 1 + i, 0);
   }
 }
 
@@ -808,19 +813,30 @@ at::Tensor paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const a
   auto st = at::cuda::getCurrentCUDAStream();
   const int B = (int)lens.size(0);
   at::Tensor row_seq, row_len;
+  const bool bf = q.scalar_type() == at::kBFloat16;
   if (news.has_value()) {
     row_seq = at::empty({a.T}, lens.options());
     row_len = at::empty({a.T}, lens.options());
     a.rows = a.T;
+    // (fp16 queries keep to the rows: the tiles' probabilities and outputs are made for bf16)
+    const bool chunks = bf && a.T >= kChunkTokens && q8::chunk_supported(a.nq / a.nkv);
     C10_CUDA_CHECK(launch_pdl(q8_rows_kernel, dim3(B + 1), dim3(kThreads), 0, st, (const int*)lens.data_ptr<int>(),
-                              (const int*)news->data_ptr<int>(), B, a.T, row_seq.data_ptr<int>(), row_len.data_ptr<int>()));
+                              (const int*)news->data_ptr<int>(), B, a.T, chunks ? kChunkTokens : 1 << 30, row_seq.data_ptr<int>(),
+                              row_len.data_ptr<int>()));
     a.row_seq = row_seq.data_ptr<int>();
     a.row_len = row_len.data_ptr<int>();
+    if (chunks) {
+      q8::ChunkArgs c = {};
+      c.q = a.q; c.q_row = a.q_row; c.kc = a.kc; c.vc = a.vc; c.ks = a.ks; c.vs = a.vs; c.tables = a.tables; c.out = a.out;
+      c.lens = lens.data_ptr<int>(); c.news = news->data_ptr<int>();
+      c.B = B; c.T = a.T; c.width = a.width; c.nq = a.nq; c.nkv = a.nkv; c.bs = a.bs; c.pages = a.pages;
+      c.min_new = kChunkTokens; c.scale = a.scale;
+      q8::launch_chunk(c, D, q.get_device(), st);
+    }
   } else {
     a.rows = std::min(a.T, B);
     a.row_len = lens.data_ptr<int>();
   }
-  const bool bf = q.scalar_type() == at::kBFloat16;
   if (D == 64) bf ? launch_q8<__nv_bfloat16, 64>(a, q, st) : launch_q8<__half, 64>(a, q, st);
   else if (D == 128) bf ? launch_q8<__nv_bfloat16, 128>(a, q, st) : launch_q8<__half, 128>(a, q, st);
   else bf ? launch_q8<__nv_bfloat16, 256>(a, q, st) : launch_q8<__half, 256>(a, q, st);

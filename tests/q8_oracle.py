@@ -40,27 +40,34 @@ def make_cache(lens, nkv, D, bs, seed=0, extra=3, device="cpu", width=None):
 
 
 def attend(q, cache, table, lens, news=None, scale=None):
-    """(output, sum p |v|, largest sum |q k| scale) in 64 bits."""
+    """(output, sum p |v| as `attend_bound` wants it, largest sum |q k| scale) in 64 bits.
+
+    fp16 probabilities below 2^-14 are multiples of 2^-24: off by 2^-25 at most, which is 2^-28 of a row's largest (that one
+    stands at 2^7 or 2^10, or at 2^-4 of it where V's scales differ).  Over all tokens that adds 2^-28 sum |v|, here as
+    2^-17 of it to what is multiplied by 2^-11 or more."""
     args = (table.cpu(), lens.cpu(), None if news is None else news.cpu())
     c = cpu(cache)
     q = q.detach().cpu().double()
     scale = scale if scale is not None else 1.0 / math.sqrt(q.shape[2])
     out = ref.paged_attention_q8(q, c, *args, scale)
     raw = c.v.view(torch.uint8) & 0x7f
-    around = ref.paged_attention_q8(q, c._replace(v=raw.view(torch.float8_e4m3fn)), *args, scale)
+    absolute = c._replace(v=raw.view(torch.float8_e4m3fn))
+    around = ref.paged_attention_q8(q, absolute, *args, scale)
+    around += 2.0 ** -17 * max(int(lens.max()), 1) * ref.paged_attention_q8(torch.zeros_like(q), absolute, *args, scale)
     k = c.dequantize()[0].nan_to_num(nan=0.0).abs().amax((0, 2))                 # [nkv, D]
     size = (q.abs() * k.double().repeat_interleave(q.shape[1] // k.shape[0], 0)[None]).sum(-1).max() * scale if q.numel() else torch.tensor(0.0)
-    return out, around, float(size)
+    return out, around, float(size) * (1 if scale >= 0 else -1)
 
 
-def attend_bound(out, around, size, L, D, dtype):
+def attend_bound(out, around, size, L, D, dtype, prob=2.0 ** -11):
     """How far a result may be off.  The output is rounded once (half a step).  Probabilities are rounded to fp16 for
-    the product (2^-11 of each).  A score is a sum of D exact products in fp32 (truncating adds: 2^-23 each) times
+    the product (2^-11 of each; to bf16, 2^-8, by the kernel that takes long chunks, where its tiles of 64 keys hold
+    several pages: ``prob``).  A score is a sum of D exact products in fp32 (truncating adds: 2^-23 each) times
     rounded factors (4 roundings): (D + 8) 2^-23 of sum |q k|; fp16 queries lose 2^-11 of elements below 2^-24 of their
     row's largest: 2^-33 sum |q k|, inside that.  The exponential adds 2^-22, and the maximum it is relative to as much again.
     Numerator and denominator each carry the score's error.  The sums over L tokens: 2^-23 per add."""
     score = (D + 8) * 2.0 ** -23 * size + 2.0 ** -20 + 2.0 ** -22 * 1.5 * size
-    rel = 2.0 ** -11 + 2 * score + 2 * (L / 16 + 32) * 2.0 ** -23
+    rel = prob + 2 * score + 2 * (L / 16 + 32) * 2.0 ** -23
     return HALF_STEP[dtype] * out.abs() * 1.01 + rel * around + 2.0 ** -24 * HALF_STEP[dtype]
 
 
