@@ -379,31 +379,35 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
       const uint32_t b = j & 1;
       if (!mbar_wait(&sm->s_full[b], (j >> 1) & 1)) { ok = false; break; }
       tc_fence_after_sync();
-      uint32_t s0[32], s1[32];
-      tmem_ld_32x32(lane_addr + b * BN, s0);
-      tmem_ld_32x32(lane_addr + b * BN + 32, s1);
-      tmem_ld_wait();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm->s_empty[b]);          // the scores are in registers: the buffer may be overwritten
       const TileInfo info = sm->info[j % kInfo];
       const int k0 = j * BN;
-      if (k0 + BN - 1 > last || (info.seen[0] & info.seen[1]) != 0xffffffffu) {
-        // keys behind the row's own position, and keys without a page
+      // keys behind the row's own position, and keys without a page
+      uint32_t see[2] = {0xffffffffu, 0xffffffffu};
+      const bool partly = k0 + BN - 1 > last || (info.seen[0] & info.seen[1]) != 0xffffffffu;
+      if (partly) {
         const int room = last - k0;                         // keys 0 .. room of the tile are at or before it
-        uint32_t lo = room >= 31 ? 0xffffffffu : room < 0 ? 0u : (2u << room) - 1u;
-        uint32_t hi = room >= 63 ? 0xffffffffu : room < 32 ? 0u : (2u << (room - 32)) - 1u;
-        lo &= info.seen[0];
-        hi &= info.seen[1];
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          if (!(lo >> i & 1)) s0[i] = 0xff800000u;
-          if (!(hi >> i & 1)) s1[i] = 0xff800000u;
-        }
+        see[0] = (room >= 31 ? 0xffffffffu : room < 0 ? 0u : (2u << room) - 1u) & info.seen[0];
+        see[1] = (room >= 63 ? 0xffffffffu : room < 32 ? 0u : (2u << (room - 32)) - 1u) & info.seen[1];
       }
+      // the scores are read twice, 32 at a time, once for the maximum and once for P: 64 of them in registers all the
+      // while were too many beside the addresses (a spill of 30 loads a tile)
+      auto scores = [&](int half, uint32_t (&s)[32]) {
+        tmem_ld_32x32(lane_addr + b * BN + 32 * half, s);
+        tmem_ld_wait();
+        if (partly) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(see[half] >> i & 1)) s[i] = 0xff800000u;
+        }
+      };
       float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) mx = fmaxf(mx, fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
+      for (int half = 0; half < 2; ++half) {
+        uint32_t s[32];
+        scores(half, s);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[i]));
+      }
       const float f = fmaxf(sc * info.ks, 1e-37f);          // above 0: masked scores stay -inf at a softmax scale of 0 too
       mx *= f;
       // P(j-1) must have been consumed before the tile is overwritten, and O must be at rest before it is rescaled
@@ -437,22 +441,31 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
       float sum = 0.f;
       uint8_t* prow = sm->p + row * 128;
 #pragma unroll
-      for (int ch = 0; ch < 8; ++ch) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int e = (ch & 3) * 8 + 2 * i;
-          const float x0 = __uint_as_float(ch < 4 ? s0[e] : s1[e]), x1 = __uint_as_float(ch < 4 ? s0[e + 1] : s1[e + 1]);
-          const float p0 = exp2_approx(fmaf(x0, f, off)), p1 = exp2_approx(fmaf(x1, f, off));
-          sum += p0 + p1;
-          if constexpr (SMALL) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(p0, p1);
-            w[i] = *reinterpret_cast<const uint32_t*>(&b);
-          } else {
-            w[i] = half2_bits(p0, p1);
-          }
+      for (int half = 0; half < 2; ++half) {
+        uint32_t s[32];
+        scores(half, s);
+        if (half == 1) {
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm->s_empty[b]);      // the scores are in registers: the buffer may be overwritten
         }
-        *reinterpret_cast<uint4*>(prow + ((ch ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+        for (int ch = 0; ch < 4; ++ch) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p0 = exp2_approx(fmaf(__uint_as_float(s[ch * 8 + 2 * i]), f, off));
+            const float p1 = exp2_approx(fmaf(__uint_as_float(s[ch * 8 + 2 * i + 1]), f, off));
+            sum += p0 + p1;
+            if constexpr (SMALL) {
+              const __nv_bfloat162 x = __floats2bfloat162_rn(p0, p1);
+              w[i] = *reinterpret_cast<const uint32_t*>(&x);
+            } else {
+              w[i] = half2_bits(p0, p1);
+            }
+          }
+          *reinterpret_cast<uint4*>(prow + (((half * 4 + ch) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
       }
       l += ratio == 1.f ? sum : sum / ratio;
       fence_proxy_async();          // written through the generic proxy, read through the async one

@@ -45,20 +45,20 @@ struct Args {
   const uint8_t *kc, *vc;        // [pages, nkv, bs, D]
   const float *ks, *vs;          // [pages, nkv]
   const int* tables;             // [B, width]
-  const int* row_seq;            // [rows] sequence of a query row (null: the row's own number)
-  const int* row_len;            // [rows] tokens it sees (kElsewhere: another kernel's row)
+  // the query rows: row of q and out (-1: none), its sequence (both null: the row's own number), the tokens that it sees
+  const int *row_id, *row_seq;
+  const int* row_len;
   void* out;                     // [T, nq, D]
   // parts of divided units, unit_rows each: 2 of every block (the unit that its share begins in, the one it ends in),
   // behind them one of every warp (the unit that its stretch begins in)
   float *part_o, *part_ml;       // [6 * grid, unit_rows, D], [6 * grid, unit_rows, 2]: maximum and sum
-  int rows, T, width, nq, nkv, bs;
+  int rows, T, width, nq, nkv, bs;  // T: rows of out that this kernel looks after, the ones behind `rows` being empty
   int pages;
   int grid;                      // blocks that the line is cut over
   int unit_rows;                 // query heads of a unit: 8 or 16
   float scale;                   // softmax scale times log2 e
 };
 
-constexpr int kElsewhere = -(1 << 30);
 // sequences with fewer new tokens go row by row; the others in tiles of 128 / rep tokens, which pay from here on
 constexpr int kChunkTokens = 8;
 
@@ -211,7 +211,7 @@ struct WarpRing {
 // it ends in (if it did not).
 struct Left {
   int head, tail;                                // 1: there is such a part; tail 2: the unit began in an earlier stretch
-  int row[2], col[2], rows[2];                   // row set, first query head, heads of the unit
+  int row[2], col[2], rows[2];                   // row of out, first query head, heads of the unit
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -319,7 +319,8 @@ paged_q8_kernel(const Args a) {
         pages = pages_of(load);
         if (fresh) {                               // the next unit's queries on their way
           const int first = load.head * rep + load.rt * 8 * H, bytes = min(8 * H, rep - load.rt * 8 * H) * D * 2;
-          const char* q = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + load.row * a.q_row + (int64_t)first * D);
+          const int id = a.row_id ? a.row_id[load.row] : load.row;
+          const char* q = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + id * a.q_row + (int64_t)first * D);
           for (int i = lane * 128; i < bytes; i += 32 * 128) asm volatile("prefetch.global.L1 [%0];" ::"l"(q + i));
         }
       }
@@ -336,7 +337,8 @@ paged_q8_kernel(const Args a) {
     const int head = use.head, rt = use.rt, rows_here = min(8 * H, rep - rt * 8 * H);
     const int from_tile = use.tile, n = min(use.tiles - use.tile, left);
     const int row = use.row, tiles = use.tiles, len = use.len;
-    const T* q = static_cast<const T*>(a.q) + row * a.q_row + (int64_t)(head * rep + rt * 8 * H) * D;
+    const int id = a.row_id ? a.row_id[row] : row;
+    const T* q = static_cast<const T*>(a.q) + id * a.q_row + (int64_t)(head * rep + rt * 8 * H) * D;
     // Q fragments: k-step e of chunk i holds elements 16 (t + 4 i) + 4 e .. + 3 of head g (+ 8 h); the order of the
     // contraction is free as long as K's fragments follow it
     constexpr int KI = D / 64;
@@ -573,7 +575,7 @@ paged_q8_kernel(const Args a) {
           const int r = 8 * h + 2 * t + y;
           if (r >= rows_here) continue;
           const float w = l[h][y] == 0.f ? 0.f : unit_v / l[h][y];
-          T* to = out + ((int64_t)row * a.nq + head * rep + rt * 8 * H + r) * D;
+          T* to = out + ((int64_t)id * a.nq + head * rep + rt * 8 * H + r) * D;
 #pragma unroll
           for (int j = 0; j < NT; j += 4) {        // 8 elements
             T x[8];
@@ -612,7 +614,7 @@ paged_q8_kernel(const Args a) {
         const int i = ends ? 0 : 1;
         if (ends) x.head = 1;
         else x.tail = begins ? 1 : 2;
-        x.row[i] = row;
+        x.row[i] = id;
         x.col[i] = head * rep + rt * 8 * H;
         x.rows[i] = rows_here;
       }
@@ -670,8 +672,10 @@ paged_q8_kernel(const Args a) {
   }
   // rows that see nothing are zero
   for (int r = blockIdx.x * kWarps + warp; r < a.T; r += gridDim.x * kWarps)
-    if (r >= a.rows || (tiles_of<TILE>(a, r) == 0 && a.row_len[r] != kElsewhere))
-      for (int i = lane * 8; i < a.nq * D; i += 256) *reinterpret_cast<uint4*>(&out[(int64_t)r * a.nq * D + i]) = make_uint4(0, 0, 0, 0);
+    if (r >= a.rows || tiles_of<TILE>(a, r) == 0) {
+      const int to = a.row_id ? a.row_id[r] : r;
+      for (int i = lane * 8; to >= 0 && i < a.nq * D; i += 256) *reinterpret_cast<uint4*>(&out[(int64_t)to * a.nq * D + i]) = make_uint4(0, 0, 0, 0);
+    }
 }
 
 // Joins the parts of the units that the cuts between blocks divide: block (c, r) looks after query head r of the unit that
@@ -724,35 +728,49 @@ __global__ void __launch_bounds__(kThreads) paged_q8_join_kernel(const Args a) {
   __syncthreads();
   den = (sh_den[0] + sh_den[1]) + (sh_den[2] + sh_den[3]);
   const float inv = den == 0.f ? 0.f : 1.f / den;
-  T* out = static_cast<T*>(a.out) + ((int64_t)place.row * a.nq + head * rep + rt * a.unit_rows + r) * D;
+  const int id = a.row_id ? a.row_id[place.row] : place.row;
+  T* out = static_cast<T*>(a.out) + ((int64_t)id * a.nq + head * rep + rt * a.unit_rows + r) * D;
   for (int d = threadIdx.x; d < D; d += kThreads)
     out[d] = from_float<T>(((sh_num[0][d] + sh_num[1][d]) + (sh_num[2][d] + sh_num[3][d])) * inv);
 }
 
-// tokens that every query row sees, and its sequence: trailing q_len tokens of each sequence, causal
+// The rows that go one by one: those of sequences with fewer than `min_chunk` new tokens, packed one behind the other,
+// `room` places in all.  A block per sequence; the last one empties the places behind them and the rows of out behind the
+// last sequence.
 __global__ void __launch_bounds__(kThreads)
-q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B, int T, int min_chunk, int* __restrict__ row_seq, int* __restrict__ row_len) {
+q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B, int T, int min_chunk, int room, int* __restrict__ row_id,
+               int* __restrict__ row_seq, int* __restrict__ row_len, uint4* __restrict__ out, int out_row) {
   pdl_wait();
   pdl_trigger();
-  __shared__ int sh[kWarps];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  // rows before this block's sequence
-  const int b = blockIdx.x;
-  int before = 0;
-  for (int i = tid; i < b; i += kThreads) before += max(news[i], 0);
+  __shared__ int sh[2][kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
+  int rows = 0, at = 0;                            // rows before this sequence, and those of them that are in the list
+  for (int i = tid; i < b; i += kThreads) {
+    const int n = max(news[i], 0);
+    rows += n;
+    at += n < min_chunk ? n : 0;
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
-  if (lane == 0) sh[warp] = before;
+  for (int o = 16; o > 0; o >>= 1) {
+    rows += __shfl_xor_sync(0xffffffffu, rows, o);
+    at += __shfl_xor_sync(0xffffffffu, at, o);
+  }
+  if (lane == 0) { sh[0][warp] = rows; sh[1][warp] = at; }
   __syncthreads();
-  before = sh[0] + sh[1] + sh[2] + sh[3];
-  if (b == B) {                                    // rows behind the last sequence
-    for (int r = before + tid; r < T; r += kThreads) { row_seq[r] = 0; row_len[r] = 0; }
+  rows = sh[0][0] + sh[0][1] + sh[0][2] + sh[0][3];
+  at = sh[1][0] + sh[1][1] + sh[1][2] + sh[1][3];
+  if (b == B) {
+    for (int r = at + tid; r < room; r += kThreads) { row_id[r] = -1; row_seq[r] = 0; row_len[r] = 0; }
+    for (int64_t i = (int64_t)rows * out_row + tid; i < (int64_t)T * out_row; i += kThreads) out[i] = make_uint4(0, 0, 0, 0);
     return;
   }
   const int n = max(news[b], 0), len = lens[b];
-  for (int i = tid; i < n && before + i < T; i += kThreads) {
-    row_seq[before + i] = b;
-    row_len[before + i] = n >= min_chunk ? kElsewhere : max(len - n + 1 + i, 0);
+  if (n >= min_chunk) return;
+  for (int i = tid; i < n && at + i < room; i += kThreads) {
+    const bool held = rows + i < T;                // there is such a row
+    row_id[at + i] = held ? rows + i : -1;
+    row_seq[at + i] = b;
+    row_len[at + i] = held ? max(len - n + 1 + i, 0) : 0;
   }
 }
 
@@ -812,19 +830,21 @@ at::Tensor paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const a
   a.scale = (float)(scale * 1.4426950408889634);
   auto st = at::cuda::getCurrentCUDAStream();
   const int B = (int)lens.size(0);
-  at::Tensor row_seq, row_len;
+  at::Tensor row_list;
   const bool bf = q.scalar_type() == at::kBFloat16;
   if (news.has_value()) {
-    row_seq = at::empty({a.T}, lens.options());
-    row_len = at::empty({a.T}, lens.options());
-    a.rows = a.T;
-    // (fp16 queries keep to the rows: the tiles' probabilities and outputs are made for bf16)
+    // (fp16 queries keep to the rows: the tiles' outputs are bf16)
     const bool chunks = bf && a.T >= kChunkTokens && q8::chunk_supported(a.nq / a.nkv);
+    a.rows = chunks ? (int)std::min<int64_t>(a.T, (int64_t)B * (kChunkTokens - 1)) : a.T;
+    row_list = at::empty({3, std::max(a.rows, 1)}, lens.options());
+    int* list = row_list.data_ptr<int>();
+    const int room = (int)row_list.size(1);
     C10_CUDA_CHECK(launch_pdl(q8_rows_kernel, dim3(B + 1), dim3(kThreads), 0, st, (const int*)lens.data_ptr<int>(),
-                              (const int*)news->data_ptr<int>(), B, a.T, chunks ? kChunkTokens : 1 << 30, row_seq.data_ptr<int>(),
-                              row_len.data_ptr<int>()));
-    a.row_seq = row_seq.data_ptr<int>();
-    a.row_len = row_len.data_ptr<int>();
+                              (const int*)news->data_ptr<int>(), B, a.T, chunks ? kChunkTokens : 1 << 30, room, list, list + room,
+                              list + 2 * room, (uint4*)a.out, (int)(a.nq * D / 8)));
+    a.row_id = list;
+    a.row_seq = list + room;
+    a.row_len = list + 2 * room;
     if (chunks) {
       q8::ChunkArgs c = {};
       c.q = a.q; c.q_row = a.q_row; c.kc = a.kc; c.vc = a.vc; c.ks = a.ks; c.vs = a.vs; c.tables = a.tables; c.out = a.out;
@@ -833,6 +853,8 @@ at::Tensor paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const a
       c.min_new = kChunkTokens; c.scale = a.scale;
       q8::launch_chunk(c, D, q.get_device(), st);
     }
+    a.T = a.rows;
+    if (a.rows == 0) return out;
   } else {
     a.rows = std::min(a.T, B);
     a.row_len = lens.data_ptr<int>();
