@@ -122,16 +122,14 @@ std::vector<at::Tensor> attn_bwd_sm100(const at::Tensor& q, const at::Tensor& k,
 int64_t attn_sm100_last_status();
 std::vector<at::Tensor> attn_fwd_sm100(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                        const at::Tensor& cu_seqlens, double scale, bool causal);
-void kv_append_q8(const at::Tensor& k, const at::Tensor& v, at::Tensor kc, at::Tensor vc, at::Tensor ks, at::Tensor vs,
+bool kv_append_q8(const at::Tensor& k, const at::Tensor& v, at::Tensor kc, at::Tensor vc, at::Tensor ks, at::Tensor vs,
                   const at::Tensor& tables, const at::Tensor& lens, const c10::optional<at::Tensor>& news);
-at::Tensor paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+c10::optional<at::Tensor> paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
                               const at::Tensor& vs, const at::Tensor& tables, const at::Tensor& lens,
                               const c10::optional<at::Tensor>& news, double scale);
 int64_t paged_attention_q8_last_status();
 std::vector<at::Tensor> token_logprob_fwd(const at::Tensor& z, const at::Tensor& tokens, int64_t n, double inv_temp);
-at::Tensor token_logprob_bwd(const at::Tensor& z, const at::Tensor& tokens, const at::Tensor& ent, const at::Tensor& stats,
-                             const at::Tensor& ids, const c10::optional<at::Tensor>& g_lp, const c10::optional<at::Tensor>& g_ent,
-                             const c10::optional<at::Tensor>& g_top, double inv_temp);
+std::vector<at::Tensor> token_logprob_apply(const at::Tensor& z, const at::Tensor& tokens, int64_t n, double inv_temp);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rmsnorm_fwd", &rmsnorm_fwd);
@@ -209,6 +207,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("paged_attention_q8", &paged_attention_q8);
   m.def("paged_attention_q8_last_status", &paged_attention_q8_last_status);
   m.def("token_logprob_fwd", &token_logprob_fwd);
-  m.def("token_logprob_bwd", &token_logprob_bwd);
+  m.def("token_logprob_apply", &token_logprob_apply);
   m.def("source_hash", []() { return std::string(clb200_source_hash()); });
 }

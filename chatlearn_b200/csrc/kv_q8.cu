@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 
 #include "q8.cuh"
+#include "q8_attention.h"
 
 using namespace cl;
 using namespace q8;
@@ -234,8 +235,16 @@ void launch_append(const AppendArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-void kv_append_q8(const at::Tensor& k, const at::Tensor& v, at::Tensor kc, at::Tensor vc, at::Tensor ks, at::Tensor vs,
+// False, and nothing done, where the arguments are not as the kernels take them.
+bool kv_append_q8(const at::Tensor& k, const at::Tensor& v, at::Tensor kc, at::Tensor vc, at::Tensor ks, at::Tensor vs,
                   const at::Tensor& tables, const at::Tensor& lens, const c10::optional<at::Tensor>& news) {
+  const auto type = k.scalar_type();
+  const bool fits = k.dim() == 3 && v.dim() == 3 && k.sizes() == v.sizes() && v.scalar_type() == type && v.device() == k.device() &&
+                    (type == at::kBFloat16 || type == at::kHalf || type == at::kFloat) && k.stride(2) == 1 && v.stride(2) == 1 &&
+                    q8::cache_fits(kc, vc, ks, vs, tables, lens, news, k.device()) && kc.size(1) == k.size(1) && kc.size(3) == k.size(2) &&
+                    (k.size(2) == 64 || k.size(2) == 128 || k.size(2) == 256) && k.size(0) < (int64_t)1 << 31 &&
+                    (news.has_value() || k.size(0) >= lens.size(0));
+  if (!fits) return false;
   const c10::cuda::CUDAGuard guard(k.device());
   AppendArgs a;
   a.x[0] = k.data_ptr(); a.x[1] = v.data_ptr();
@@ -247,9 +256,10 @@ void kv_append_q8(const at::Tensor& k, const at::Tensor& v, at::Tensor kc, at::T
   a.news = news.has_value() ? news->data_ptr<int>() : nullptr;
   a.B = (int)lens.size(0); a.width = (int)tables.size(1); a.T = (int)k.size(0);
   a.nkv = (int)kc.size(1); a.bs = (int)kc.size(2); a.D = (int)kc.size(3); a.pages = kc.size(0);
-  if (a.B == 0 || a.T == 0 || a.width == 0) return;
+  if (a.B == 0 || a.T == 0 || a.width == 0) return true;
   auto st = at::cuda::getCurrentCUDAStream();
   if (k.scalar_type() == at::kBFloat16) launch_append<__nv_bfloat16>(a, st);
   else if (k.scalar_type() == at::kHalf) launch_append<__half>(a, st);
   else launch_append<float>(a, st);
+  return true;
 }

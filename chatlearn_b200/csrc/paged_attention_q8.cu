@@ -811,12 +811,34 @@ void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
 
 }  // namespace
 
-at::Tensor paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+bool q8::cache_fits(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& tables,
+                    const at::Tensor& lens, const c10::optional<at::Tensor>& news, c10::Device dev) {
+  auto codes = [&](const at::Tensor& x) {
+    return x.scalar_type() == at::kFloat8_e4m3fn && x.device() == dev && x.is_contiguous() && (uintptr_t)x.data_ptr() % 16 == 0;
+  };
+  auto scales = [&](const at::Tensor& x) {
+    return x.scalar_type() == at::kFloat && x.dim() == 2 && x.size(0) == kc.size(0) && x.size(1) == kc.size(1) && x.device() == dev && x.is_contiguous();
+  };
+  auto ints = [&](const at::Tensor& x, int64_t dims) { return x.scalar_type() == at::kInt && x.dim() == dims && x.device() == dev && x.is_contiguous(); };
+  return dev.is_cuda() && kc.dim() == 4 && codes(kc) && codes(vc) && vc.sizes() == kc.sizes() && kc.size(1) > 0 && kc.size(2) > 0 &&
+         kc.size(2) % 16 == 0 && scales(ks) && scales(vs) && ints(tables, 2) && ints(lens, 1) && tables.size(0) == lens.size(0) &&
+         (!news.has_value() || (ints(*news, 1) && news->size(0) == lens.size(0))) && kc.size(0) * kc.size(1) < (int64_t)1 << 31;
+}
+
+// No tensor where the arguments are not as the kernels take them (the caller then says what is wrong, or lays them out).
+c10::optional<at::Tensor> paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
                               const at::Tensor& vs, const at::Tensor& tables, const at::Tensor& lens,
                               const c10::optional<at::Tensor>& news, double scale) {
+  const int64_t D64 = q.dim() == 3 ? q.size(2) : 0;
+  const bool fits =
+      (D64 == 64 || D64 == 128 || D64 == 256) && (q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf) && q.stride(2) == 1 &&
+      (q.size(1) == 1 || q.stride(1) == D64) && (q.size(0) <= 1 || q.stride(0) % 8 == 0) && (uintptr_t)q.data_ptr() % 16 == 0 &&
+      cache_fits(kc, vc, ks, vs, tables, lens, news, q.device()) && kc.size(3) == D64 && q.size(1) > 0 && q.size(1) % kc.size(1) == 0 &&
+      q.size(0) < (int64_t)1 << 31 && (news.has_value() || q.size(0) >= lens.size(0));
+  if (!fits) return c10::nullopt;
   const c10::cuda::CUDAGuard guard(q.device());
   Args a = {};
-  const int D = (int)q.size(2);
+  const int D = (int)D64;
   auto out = at::empty({q.size(0), q.size(1), q.size(2)}, q.options());
   if (q.size(0) == 0) return out;
   a.q = q.data_ptr(); a.q_row = q.stride(0);
@@ -825,7 +847,6 @@ at::Tensor paged_attention_q8(const at::Tensor& q, const at::Tensor& kc, const a
   a.tables = tables.data_ptr<int>();
   a.out = out.data_ptr();
   a.T = (int)q.size(0); a.nq = (int)q.size(1); a.nkv = (int)kc.size(1); a.bs = (int)kc.size(2); a.pages = (int)kc.size(0);
-  TORCH_CHECK_VALUE(kc.size(0) * kc.size(1) < (int64_t)1 << 31, "paged_attention_q8: fewer than 2^31 pages times heads");
   a.width = (int)tables.size(1);
   a.scale = (float)(scale * 1.4426950408889634);
   auto st = at::cuda::getCurrentCUDAStream();

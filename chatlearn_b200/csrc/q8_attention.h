@@ -1,5 +1,6 @@
-// Attention over the paged 8-bit cache: what the decode and the chunk kernels share on the host.
+// The paged 8-bit cache: what its kernels share on the host.
 #pragma once
+#include <ATen/core/Tensor.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -17,6 +18,10 @@ struct ChunkArgs {
   int min_new;                   // sequences with fewer new tokens are left out
   float scale;                   // softmax scale times log2 e
 };
+
+// whether the cache and the tables are as the kernels take them
+bool cache_fits(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks, const at::Tensor& vs, const at::Tensor& tables,
+                const at::Tensor& lens, const c10::optional<at::Tensor>& news, c10::Device dev);
 
 bool chunk_supported(int rep);
 void launch_chunk(const ChunkArgs& a, int D, int dev, cudaStream_t st);

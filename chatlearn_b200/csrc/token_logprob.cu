@@ -6,7 +6,7 @@
 // (all relative to the maximum: no difference of two large numbers, and no overflow of logits at the type's lowest value).
 //
 // Alternatives without a second pass over the row: a warp notes the maximum of each stretch of the row that it reads
-// (512 or 1024 logits).  At most n stretches hold the n largest logits, namely those with the n largest maxima, and the
+// (512 or 1024 logits, a quarter of that where the row is short).  At most n stretches hold the n largest logits, namely those with the n largest maxima, and the
 // n-th largest maximum bounds the n-th largest logit from below; so the candidates are the logits of n stretches that
 // reach that bound, about n of them.  Order: larger logit first, then lower index.
 //
@@ -17,6 +17,8 @@
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cooperative_groups.h>
+
+#include <type_traits>
 
 #include "q8.cuh"
 
@@ -29,7 +31,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kMaxTop = 64;
 constexpr int kUnroll = 4;                        // vectors of 16 bytes a lane loads at once
 constexpr int kMaxStretch = 512;                  // stretches of a block
-constexpr int kCand = 2304;                       // n (n + 1) / 2 candidates when all logits are equal, and room
+constexpr int kCand = 4096;                       // n (n + 1) / 2 candidates when all logits are equal, and room; a power of two
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1000.f;                   // 2^kFar is 0: -inf logits stay out of 0 * inf
 
@@ -65,6 +67,39 @@ __device__ __forceinline__ void load16(const T* p, float* f) {
   for (int i = 0; i < Wide<T>::N; ++i) f[i] = q8::to_float(t[i]);
 }
 
+// maximum over the warp, NaN left out
+__device__ __forceinline__ float warp_max_f32(float v) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(v));
+  return y;
+}
+// two fp32 in one register pair
+__device__ __forceinline__ uint64_t pair(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
 struct Sums { float m, s, x; };                   // M, S, X
 __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
   Sums r;
@@ -77,7 +112,26 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
   return r;
 }
 
-struct Shared {
+constexpr int kSmall = 96;                        // candidates that are ranked by counting; more are sorted
+
+// The block sorts `count` keys, largest first (bitonic; zeros fill up to a power of two).
+__device__ __forceinline__ void sort_keys(uint64_t* keys, int count) {
+  int size = 64;
+  while (size < count) size *= 2;
+  for (int i = count + threadIdx.x; i < size; i += kThreads) keys[i] = 0;
+  __syncthreads();
+  for (int k = 2; k <= size; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      for (int i = threadIdx.x; i < size / 2; i += kThreads) {
+        const int lo = 2 * i - (i & (j - 1)), hi = lo + j;
+        const uint64_t x = keys[lo], y = keys[hi];
+        if ((x < y) == ((lo & k) == 0)) { keys[lo] = y; keys[hi] = x; }
+      }
+      __syncthreads();
+    }
+}
+
+struct __align__(16) Shared {
   float stretch[kMaxStretch];
   uint64_t cand[kCand];
   uint64_t best[8 * kMaxTop];                     // the cluster's lists, in the first block
@@ -109,32 +163,42 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
   const T* body = z + head;
   const int batches = (vecs + 32 * kUnroll - 1) / (32 * kUnroll);
   const int b0 = (int)((int64_t)part * batches / parts), b1 = (int)((int64_t)(part + 1) * batches / parts);
-  const int per = max(1, (b1 - b0 + kMaxStretch - 1) / kMaxStretch);          // batches of a stretch
-  const int stretches = (b1 - b0 + per - 1) / per;
+  // a stretch is `per` batches, or one vector of each lane where there are few
+  const bool fine = (b1 - b0) * kUnroll <= kMaxStretch;
+  const int per = fine ? 1 : max(1, (b1 - b0 + kMaxStretch - 1) / kMaxStretch);
+  const int runs = (b1 - b0 + per - 1) / per, stretches = fine ? runs * kUnroll : runs;
+  const int length = fine ? 32 : per * 32 * kUnroll;                          // of a stretch, in vectors
+  const int v_end = min(b1 * 32 * kUnroll, vecs);
 
   // ---- the pass over the row
   Sums a{-INFINITY, 0.f, 0.f};                     // m is the warp's
-  auto take = [&](const float* f, int count) {
-    const float ref = a.m == -INFINITY ? 0.f : a.m;
+  // two logits at a time: S and X of the even and the odd ones
+  uint64_t s2 = 0, x2 = 0;
+  const uint64_t c2 = pair(c, c);
+  auto take = [&](const float* f, auto count) {
+    const float ref = a.m == -INFINITY ? 0.f : -a.m;
+    const uint64_t ref2 = pair(ref, ref);
 #pragma unroll
-    for (int i = 0; i < N * kUnroll; ++i)
-      if (i < count) {
-        const float x = max_nan((f[i] - ref) * c, kFar), e = exp2_approx(x);
-        a.s += e;
-        a.x = fmaf(e, x, a.x);
-      }
+    for (int i = 0; i < decltype(count)::value; i += 2) {
+      const float2 y = unpair(mul2(add2(pair(f[i], f[i + 1]), ref2), c2));
+      const float x0 = max_nan(y.x, kFar), x1 = max_nan(y.y, kFar);
+      const uint64_t e = pair(exp2_approx(x0), exp2_approx(x1));
+      s2 = add2(s2, e);
+      x2 = fma2(e, pair(x0, x1), x2);
+    }
   };
   auto raise = [&](float y) {                      // a new warp maximum
     if (y > a.m) {
       if (a.m != -INFINITY) {
         const float d = fmaxf((a.m - y) * c, kFar), e = exp2_approx(d);
-        a.x = e * (a.x + a.s * d);
-        a.s *= e;
+        const uint64_t e2 = pair(e, e);
+        x2 = mul2(e2, fma2(s2, pair(d, d), x2));
+        s2 = mul2(s2, e2);
       }
       a.m = y;
     }
   };
-  for (int s = warp; s < stretches; s += kWarps) {
+  for (int s = warp; s < runs; s += kWarps) {
     float most = -INFINITY;
     const int e1 = min(b0 + (s + 1) * per, b1);
     for (int b = b0 + s * per; b < e1; ++b) {
@@ -147,26 +211,42 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
 #pragma unroll
           for (int i = 0; i < N; ++i) f[u * N + i] = -INFINITY;
       }
-      float mx = -INFINITY;
+      float mx[kUnroll];
 #pragma unroll
-      for (int i = 0; i < N * kUnroll; ++i) mx = fmaxf(mx, f[i]);
-      mx = warp_max(mx);
-      raise(mx);
-      most = fmaxf(most, mx);
-      take(f, N * kUnroll);
+      for (int u = 0; u < kUnroll; ++u) {
+        mx[u] = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < N; ++i) mx[u] = fmaxf(mx[u], f[u * N + i]);
+      }
+      if (fine && n > 0) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) mx[u] = warp_max_f32(mx[u]);
+        if (lane < kUnroll) sh.stretch[s * kUnroll + lane] = lane == 0 ? mx[0] : lane == 1 ? mx[1] : lane == 2 ? mx[2] : mx[3];
+      }
+      const float all = warp_max_f32(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+      raise(all);
+      most = fmaxf(most, all);
+      take(f, std::integral_constant<int, N * kUnroll>{});
     }
-    if (lane == 0) sh.stretch[s] = most;
+    if (!fine && lane == 0) sh.stretch[s] = most;
   }
   if (part == 0 && warp == kWarps - 1) {           // the unaligned ends
-    float f[N * kUnroll];
-    f[0] = lane < head ? q8::to_float(z[lane]) : lane >= 16 && tail + lane - 16 < V ? q8::to_float(z[tail + lane - 16]) : -INFINITY;
+    float f[2] = {-INFINITY, -INFINITY};
+    if (lane < head) f[0] = q8::to_float(z[lane]);
+    if (lane >= 16 && tail + lane - 16 < V) f[0] = q8::to_float(z[tail + lane - 16]);
     raise(warp_max(f[0]));
-    take(f, 1);
+    take(f, std::integral_constant<int, 2>{});
+  }
+  {
+    const float2 s = unpair(s2), x = unpair(x2);
+    a.s = s.x + s.y;
+    a.x = x.x + x.y;
   }
   a.s = warp_sum(a.s);
   a.x = warp_sum(a.x);
   if (lane == 0) sh.warp_sums[warp] = a;
   if (tid == 0) { sh.count = 0; sh.bound = -INFINITY; }
+  if (tid < 4 && stretches + tid < kMaxStretch) sh.stretch[stretches + tid] = -INFINITY;
   __syncthreads();
   if (tid == 0) {
     Sums t = sh.warp_sums[0];
@@ -180,9 +260,10 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
     if (tid < stretches) {
       const float v = sh.stretch[tid];
       int rank = 0;
-      for (int j = 0; j < stretches; ++j) {
-        const float w = sh.stretch[j];
-        rank += w > v || (w == v && j < tid);
+      for (int j = 0; j < stretches; j += 4) {     // (what lies behind the last one is -inf and not in front of anything)
+        const float4 w = *reinterpret_cast<const float4*>(&sh.stretch[j]);
+        rank += (w.x > v || (w.x == v && j < tid)) + (w.y > v || (w.y == v && j + 1 < tid)) + (w.z > v || (w.z == v && j + 2 < tid)) +
+                (w.w > v || (w.w == v && j + 3 < tid));
       }
       if (rank < n) sh.chosen[rank] = tid;
       if (rank == n - 1) sh.bound = v;
@@ -197,11 +278,11 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
     for (int r = warp; r < chosen; r += kWarps) {
       const int s = sh.chosen[r];
       int equal = 0;                               // logits equal to the bound so far; no more than n - r can matter
-      const int e1 = min(b0 + (s + 1) * per, b1);
-      for (int v = (b0 + s * per) * 32 * kUnroll + lane; v - lane < min(e1 * 32 * kUnroll, vecs); v += 32) {
+      const int v0 = b0 * 32 * kUnroll + s * length, v1 = min(v0 + length, v_end);
+      for (int v = v0 + lane; v - lane < v1; v += 32) {
         float f[N];
         int mine = 0;
-        if (v < vecs) {
+        if (v < v1) {
           load16(body + (int64_t)v * N, f);
 #pragma unroll
           for (int i = 0; i < N; ++i) {
@@ -236,13 +317,17 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
     for (int i = tid; i < n; i += kThreads) sh.best[i] = 0;
     __syncthreads();
     const int count = sh.count;
-    if (count <= kCand) {
-      for (int i = tid; i < count; i += kThreads) {
-        const uint64_t k = sh.cand[i];
+    if (count <= kSmall) {
+      if (tid < count) {
+        const uint64_t k = sh.cand[tid];
         int rank = 0;
         for (int j = 0; j < count; ++j) rank += sh.cand[j] > k;
         if (rank < n) sh.best[rank] = k;
       }
+      __syncthreads();
+    } else if (count <= kCand) {
+      sort_keys(sh.cand, count);
+      if (tid < n && tid < count) sh.best[tid] = sh.cand[tid];
       __syncthreads();
     } else {
       // thousands of logits of few stretches above the bound (ascending rows, for one): n rounds of the largest key
@@ -255,8 +340,8 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
           if (x < last && x > mine) mine = x;
         };
         for (int r = warp; r < chosen; r += kWarps) {
-          const int s = sh.chosen[r], e1 = min(b0 + (s + 1) * per, b1);
-          for (int v = (b0 + s * per) * 32 * kUnroll + lane; v < min(e1 * 32 * kUnroll, vecs); v += 32) {
+          const int v0 = b0 * 32 * kUnroll + sh.chosen[r] * length, v1 = min(v0 + length, v_end);
+          for (int v = v0 + lane; v < v1; v += 32) {
             float f[N];
             load16(body + (int64_t)v * N, f);
 #pragma unroll
@@ -409,9 +494,16 @@ int cluster_for(int64_t rows) {
 
 }  // namespace
 
+// {log-prob, entropy, alternatives' log-probs, their ids, statistics for the gradient}; empty where the arguments are not as
+// the kernel takes them.
 std::vector<at::Tensor> token_logprob_fwd(const at::Tensor& z, const at::Tensor& tokens, int64_t n, double inv_temp) {
+  const auto type = z.scalar_type();
+  const bool fits = z.is_cuda() && z.dim() == 2 && (type == at::kBFloat16 || type == at::kHalf || type == at::kFloat) && z.size(1) > 0 &&
+                    (z.size(1) == 1 || z.stride(1) == 1) && z.size(0) < (int64_t)1 << 28 && z.size(1) < (int64_t)1 << 30 && n >= 0 &&
+                    n <= std::min<int64_t>(kMaxTop, z.size(1)) && inv_temp > 0.0 && tokens.scalar_type() == at::kLong && tokens.dim() == 1 &&
+                    tokens.size(0) == z.size(0) && tokens.is_contiguous() && tokens.device() == z.device();
+  if (!fits) return {};
   const c10::cuda::CUDAGuard guard(z.device());
-  TORCH_CHECK(n >= 0 && n <= kMaxTop, "token_logprobs: at most 64 alternatives");
   const int64_t R = z.size(0), V = z.size(1);
   auto f = z.options().dtype(at::kFloat);
   auto lp = at::empty({R}, f), ent = at::empty({R}, f), stats = at::empty({R, 2}, f), top = at::empty({R, n}, f);
