@@ -100,6 +100,37 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+// 16 bytes of logits
+template <typename T>
+__device__ __forceinline__ uint4 load_raw(const T* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+template <typename T>
+__device__ __forceinline__ uint4 raw_lowest() {  // -inf everywhere
+  const uint32_t x = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+  return make_uint4(x, x, x, x);
+}
+template <typename T>
+__device__ __forceinline__ void expand(const uint4& u, float* f) {
+  const T* t = reinterpret_cast<const T*>(&u);
+#pragma unroll
+  for (int i = 0; i < Wide<T>::N; ++i) f[i] = q8::to_float(t[i]);
+}
+// largest of a vector, NaN left out
+template <typename T>
+__device__ __forceinline__ float raw_max(const uint4& u) {
+  if constexpr (sizeof(T) == 4) {
+    const float* f = reinterpret_cast<const float*>(&u);
+    return fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  } else {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+}
+
 struct Sums { float m, s, x; };                   // M, S, X
 __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
   Sums r;
@@ -198,37 +229,50 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
       a.m = y;
     }
   };
-  for (int s = warp; s < runs; s += kWarps) {
-    float most = -INFINITY;
-    const int e1 = min(b0 + (s + 1) * per, b1);
-    for (int b = b0 + s * per; b < e1; ++b) {
-      float f[N * kUnroll];
-      const int v0 = b * 32 * kUnroll + lane;
+  // the warp's batches in order, the next one on its way while this one is summed up
+  auto fetch = [&](int b, uint4 (&raw)[kUnroll]) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (v0 + u * 32 < vecs) load16(body + (int64_t)(v0 + u * 32) * N, f + u * N);
-        else
-#pragma unroll
-          for (int i = 0; i < N; ++i) f[u * N + i] = -INFINITY;
-      }
-      float mx[kUnroll];
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        mx[u] = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < N; ++i) mx[u] = fmaxf(mx[u], f[u * N + i]);
-      }
-      if (fine && n > 0) {
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) mx[u] = warp_max_f32(mx[u]);
-        if (lane < kUnroll) sh.stretch[s * kUnroll + lane] = lane == 0 ? mx[0] : lane == 1 ? mx[1] : lane == 2 ? mx[2] : mx[3];
-      }
-      const float all = warp_max_f32(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-      raise(all);
-      most = fmaxf(most, all);
-      take(f, std::integral_constant<int, N * kUnroll>{});
+    for (int u = 0; u < kUnroll; ++u) {
+      const int v = (b * kUnroll + u) * 32 + lane;
+      raw[u] = v < v_end ? load_raw(body + (int64_t)v * N) : raw_lowest<T>();
     }
-    if (!fine && lane == 0) sh.stretch[s] = most;
+  };
+  int run = warp, b = b0 + warp * per;
+  uint4 next[kUnroll];
+  fetch(b, next);                                  // (behind the end: nothing is loaded)
+  float most = -INFINITY;
+  while (run < runs) {
+    uint4 raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) raw[u] = next[u];
+    const int here = run;
+    const bool last = b + 1 >= min(b0 + (run + 1) * per, b1);
+    if (last) { run += kWarps; b = b0 + run * per; } else ++b;
+    if (run < runs) fetch(b, next);
+    float mx[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) mx[u] = raw_max<T>(raw[u]);
+    float all;
+    if (fine && n > 0) {
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) mx[u] = warp_max_f32(mx[u]);
+      if (lane < kUnroll) sh.stretch[here * kUnroll + lane] = lane == 0 ? mx[0] : lane == 1 ? mx[1] : lane == 2 ? mx[2] : mx[3];
+      all = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    } else {
+      all = warp_max_f32(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+    }
+    raise(all);
+    most = fmaxf(most, all);
+    if (last) {
+      if (!fine && lane == 0) sh.stretch[here] = most;
+      most = -INFINITY;
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      float f[N];
+      expand<T>(raw[u], f);
+      take(f, std::integral_constant<int, N>{});
+    }
   }
   if (part == 0 && warp == kWarps - 1) {           // the unaligned ends
     float f[2] = {-INFINITY, -INFINITY};
@@ -248,10 +292,14 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
   if (tid == 0) { sh.count = 0; sh.bound = -INFINITY; }
   if (tid < 4 && stretches + tid < kMaxStretch) sh.stretch[stretches + tid] = -INFINITY;
   __syncthreads();
-  if (tid == 0) {
-    Sums t = sh.warp_sums[0];
-    for (int w = 1; w < kWarps; ++w) t = join(t, sh.warp_sums[w], c);
-    sh.sums = t;
+  if (warp == kWarps - 1) {                        // (the warp with the least to do below)
+    Sums t = lane < kWarps ? sh.warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+#pragma unroll 1
+    for (int o = kWarps / 2; o > 0; o /= 2) {
+      const Sums y{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o), __shfl_xor_sync(0xffffffffu, t.x, o)};
+      t = lane & o ? join(y, t, c) : join(t, y, c);
+    }
+    if (lane == 0) sh.sums = t;
   }
 
   // ---- the block's n best
@@ -370,11 +418,17 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
       uint64_t k = 0;
       const int total = parts * n;                 // at most 512: one key a thread
       if (tid < total) k = cluster.map_shared_rank(&sh, tid / n)->best[tid % n];
-      Sums t = sh.sums;
-      if (tid == 0)
-        for (int p = 1; p < parts; ++p) t = join(t, cluster.map_shared_rank(&sh, p)->sums, c);
+      Sums t{-INFINITY, 0.f, 0.f};
+      if (warp == kWarps - 1) {
+        if (lane < parts) t = cluster.map_shared_rank(&sh, lane)->sums;
+#pragma unroll 1
+        for (int o = 4; o > 0; o /= 2) {
+          const Sums y{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o), __shfl_xor_sync(0xffffffffu, t.x, o)};
+          t = lane & o ? join(y, t, c) : join(t, y, c);
+        }
+      }
       __syncthreads();                             // the own list has been read
-      if (tid == 0) sh.sums = t;
+      if (warp == kWarps - 1 && lane == 0) sh.sums = t;
       if (tid < total) sh.cand[tid] = k;
       __syncthreads();
       if (tid < total && k) {
