@@ -5,12 +5,14 @@
 //   logprob = (z_tok - M) / temperature - ln S,   entropy = (log2 S - X / S) ln 2
 // (all relative to the maximum: no difference of two large numbers, and no overflow of logits at the type's lowest value).
 //
-// Alternatives without a second pass over the row: a warp notes the maximum of each stretch of the row that it reads
-// (512 or 1024 logits, a quarter of that where the row is short).  At most n stretches hold the n largest logits, namely those with the n largest maxima, and the
-// n-th largest maximum bounds the n-th largest logit from below; so the candidates are the logits of n stretches that
-// reach that bound, about n of them.  Order: larger logit first, then lower index.
+// Alternatives without a second pass over the row: a warp notes the maximum of each stretch of the row that it reads (512
+// or 1024 logits; where the block reads little, each thread that of its own logits).  The n-th largest of the warps' few
+// largest maxima is reached by n logits, so it bounds the n-th largest logit from below; the stretches whose maximum
+// reaches it, hardly more than n, are looked at again, and what reaches it there is ranked.  Where those are too many (rows
+// of equal or rising logits): at most n stretches hold the n largest logits, those with the n largest maxima, and of equal
+// logits no more than n have to be looked at.  Order: larger logit first, then lower index.
 //
-// A row is read by a cluster of 1 to 8 blocks; their sums and lists meet in the first block's shared memory.
+// A row is read by a cluster of 1 to 8 blocks, which write their sums and lists into the first block's shared memory.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/empty.h>
@@ -167,7 +169,8 @@ struct __align__(16) Shared {
   uint64_t cand[kCand];
   uint64_t best[8 * kMaxTop];                     // the cluster's lists, in the first block
   int chosen[kMaxTop];
-  Sums warp_sums[kWarps];
+  float firsts[2 * kMaxTop + kWarps];
+  Sums warp_sums[kWarps], part_sums[8];
   Sums sums;
   uint64_t round;
   float bound;
@@ -194,12 +197,16 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
   const T* body = z + head;
   const int batches = (vecs + 32 * kUnroll - 1) / (32 * kUnroll);
   const int b0 = (int)((int64_t)part * batches / parts), b1 = (int)((int64_t)(part + 1) * batches / parts);
-  // a stretch is `per` batches, or one vector of each lane where there are few
-  const bool fine = (b1 - b0) * kUnroll <= kMaxStretch;
-  const int per = fine ? 1 : max(1, (b1 - b0 + kMaxStretch - 1) / kMaxStretch);
-  const int runs = (b1 - b0 + per - 1) / per, stretches = fine ? runs * kUnroll : runs;
-  const int length = fine ? 32 : per * 32 * kUnroll;                          // of a stretch, in vectors
+  const int per = max(1, (b1 - b0 + kMaxStretch - 1) / kMaxStretch);          // batches of a stretch: a lane for each of a warp's
+  const int stretches = (b1 - b0 + per - 1) / per, length = per * 32 * kUnroll;      // length in vectors
   const int v_end = min(b1 * 32 * kUnroll, vecs);
+  const bool little = b1 - b0 <= 2 * kWarps;       // at most two batches of a warp
+  if (parts > 1) cluster.barrier_arrive();         // the first block has begun, for the writes into its shared memory
+  // the token's logit on its way
+  const int64_t tok = tokens[row];
+  const bool real = tok >= 0 && tok < V;
+  float z_tok = 0.f;
+  if (tid == 0 && part == 0 && real) z_tok = q8::to_float(z[tok]);
 
   // ---- the pass over the row
   Sums a{-INFINITY, 0.f, 0.f};                     // m is the warp's
@@ -241,30 +248,23 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
   uint4 next[kUnroll];
   fetch(b, next);                                  // (behind the end: nothing is loaded)
   float most = -INFINITY;
-  while (run < runs) {
+  float maxima = -INFINITY;                        // lane i: of the warp's i-th stretch (where `little`: of the lane's logits)
+  int nth = 0;
+  while (run < stretches) {
     uint4 raw[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) raw[u] = next[u];
-    const int here = run;
     const bool last = b + 1 >= min(b0 + (run + 1) * per, b1);
     if (last) { run += kWarps; b = b0 + run * per; } else ++b;
-    if (run < runs) fetch(b, next);
-    float mx[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) mx[u] = raw_max<T>(raw[u]);
-    float all;
-    if (fine && n > 0) {
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) mx[u] = warp_max_f32(mx[u]);
-      if (lane < kUnroll) sh.stretch[here * kUnroll + lane] = lane == 0 ? mx[0] : lane == 1 ? mx[1] : lane == 2 ? mx[2] : mx[3];
-      all = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-    } else {
-      all = warp_max_f32(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-    }
+    if (run < stretches) fetch(b, next);
+    const float mine = fmaxf(fmaxf(raw_max<T>(raw[0]), raw_max<T>(raw[1])), fmaxf(raw_max<T>(raw[2]), raw_max<T>(raw[3])));
+    const float all = warp_max_f32(mine);
+    if (little) maxima = fmaxf(maxima, mine);
     raise(all);
     most = fmaxf(most, all);
     if (last) {
-      if (!fine && lane == 0) sh.stretch[here] = most;
+      if (!little && lane == nth) maxima = most;
+      ++nth;
       most = -INFINITY;
     }
 #pragma unroll
@@ -289,8 +289,19 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
   a.s = warp_sum(a.s);
   a.x = warp_sum(a.x);
   if (lane == 0) sh.warp_sums[warp] = a;
+  // maxima that a warp contributes to the bound: twice n in all
+  const int warps = max(1, min(kWarps, stretches)), firsts = min(32, (2 * n + warps - 1) / warps);
+  if (n > 0) {
+    float rest = maxima;
+    for (int k = 0; k < firsts; ++k) {
+      const float top = warp_max_f32(rest);
+      if (lane == 0 && warp < warps) sh.firsts[warp * firsts + k] = top;
+      const uint32_t at = __ballot_sync(0xffffffffu, rest == top);
+      if (lane == __ffs(at) - 1) rest = -INFINITY;
+    }
+  }
   if (tid == 0) { sh.count = 0; sh.bound = -INFINITY; }
-  if (tid < 4 && stretches + tid < kMaxStretch) sh.stretch[stretches + tid] = -INFINITY;
+  for (int i = tid; i < n; i += kThreads) sh.best[i] = 0;
   __syncthreads();
   if (warp == kWarps - 1) {                        // (the warp with the least to do below)
     Sums t = lane < kWarps ? sh.warp_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
@@ -304,67 +315,141 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
 
   // ---- the block's n best
   if (n > 0) {
-    // the n stretches with the largest maxima, and the bound
-    if (tid < stretches) {
-      const float v = sh.stretch[tid];
-      int rank = 0;
-      for (int j = 0; j < stretches; j += 4) {     // (what lies behind the last one is -inf and not in front of anything)
-        const float4 w = *reinterpret_cast<const float4*>(&sh.stretch[j]);
-        rank += (w.x > v || (w.x == v && j < tid)) + (w.y > v || (w.y == v && j + 1 < tid)) + (w.z > v || (w.z == v && j + 2 < tid)) +
-                (w.w > v || (w.w == v && j + 3 < tid));
+    // the bound, by every warp for itself
+    float bound = -INFINITY;
+    for (int i0 = 0; i0 < warps * firsts; i0 += 32) {
+      const int i = i0 + lane;
+      const float v = i < warps * firsts ? sh.firsts[i] : -INFINITY;
+      int rank = i < warps * firsts ? 0 : kMaxStretch;
+#pragma unroll 4
+      for (int j = 0; j < warps * firsts; ++j) {
+        const float w = sh.firsts[j];
+        rank += w > v || (w == v && j < i);
       }
-      if (rank < n) sh.chosen[rank] = tid;
-      if (rank == n - 1) sh.bound = v;
+      const uint32_t hit = __ballot_sync(0xffffffffu, rank == n - 1);
+      if (hit) bound = __shfl_sync(0xffffffffu, v, __ffs(hit) - 1);
     }
-    __syncthreads();
-    const float bound = sh.bound;
-    const int chosen = min(n, stretches);
     auto push = [&](float v, int idx) {
       const int at = atomicAdd(&sh.count, 1);
       if (at < kCand) sh.cand[at] = key_of(v, idx);
     };
-    for (int r = warp; r < chosen; r += kWarps) {
-      const int s = sh.chosen[r];
-      int equal = 0;                               // logits equal to the bound so far; no more than n - r can matter
-      const int v0 = b0 * 32 * kUnroll + s * length, v1 = min(v0 + length, v_end);
-      for (int v = v0 + lane; v - lane < v1; v += 32) {
+    auto ends = [&](auto take_one) {
+      if (part == 0 && warp == kWarps - 1) {
+        if (lane < head) take_one(q8::to_float(z[lane]), lane);
+        if (lane >= 16 && tail + lane - 16 < V) take_one(q8::to_float(z[tail + lane - 16]), tail + lane - 16);
+      }
+    };
+    // what reaches it
+    auto look = [&](const uint4& u, int v) {
+      if (raw_max<T>(u) >= bound) {
         float f[N];
-        int mine = 0;
-        if (v < v1) {
-          load16(body + (int64_t)v * N, f);
+        expand<T>(u, f);
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            f[i] = f[i] == f[i] ? f[i] : -INFINITY;
-            mine += f[i] == bound;
-            if (f[i] > bound) push(f[i], head + v * N + i);
-          }
+        for (int e = 0; e < N; ++e)
+          if (f[e] >= bound || (bound == -INFINITY && f[e] != f[e])) push(f[e], head + v * N + e);
+      }
+    };
+    if (little) {
+      if (maxima >= bound) {                       // the lane's own logits again
+        for (int b = b0 + warp; b < b1; b += kWarps) {
+          uint4 u[kUnroll];
+          fetch(b, u);
+#pragma unroll
+          for (int x = 0; x < kUnroll; ++x)
+            if ((b * kUnroll + x) * 32 + lane < v_end) look(u[x], (b * kUnroll + x) * 32 + lane);
         }
-        if (__any_sync(0xffffffffu, mine > 0)) {
-          int inc = mine;
+      }
+    } else {
+      uint32_t todo = __ballot_sync(0xffffffffu, lane < nth && maxima >= bound);
+      while (todo) {                               // two stretches at a time: their loads overlap
+        const int i = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const int j = todo ? __ffs(todo) - 1 : i;
+        const bool two = todo != 0;
+        todo &= todo - 1;
+        const int v0 = b0 * 32 * kUnroll + (warp + i * kWarps) * length, v1 = b0 * 32 * kUnroll + (warp + j * kWarps) * length;
+        for (int at = lane; at < length; at += 32 * kUnroll) {
+          uint4 u[2][kUnroll];
 #pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int p = __shfl_up_sync(0xffffffffu, inc, o);
-            if (lane >= o) inc += p;
+          for (int x = 0; x < kUnroll; ++x) {
+            u[0][x] = v0 + at + 32 * x < v_end ? load_raw(body + (int64_t)(v0 + at + 32 * x) * N) : raw_lowest<T>();
+            u[1][x] = two && v1 + at + 32 * x < v_end ? load_raw(body + (int64_t)(v1 + at + 32 * x) * N) : raw_lowest<T>();
           }
-          int at = equal + inc - mine;
-          if (mine > 0)
 #pragma unroll
-            for (int i = 0; i < N; ++i)
-              if (f[i] == bound) {
-                if (at < n - r) push(f[i], head + v * N + i);
-                ++at;
-              }
-          equal += __shfl_sync(0xffffffffu, inc, 31);
+          for (int x = 0; x < kUnroll; ++x) {
+            if (v0 + at + 32 * x < v_end) look(u[0][x], v0 + at + 32 * x);
+            if (two && v1 + at + 32 * x < v_end) look(u[1][x], v1 + at + 32 * x);
+          }
         }
       }
     }
-    if (part == 0 && warp == kWarps - 1) {
-      if (lane < head) push(q8::to_float(z[lane]), lane);
-      if (lane >= 16 && tail + lane - 16 < V) push(q8::to_float(z[tail + lane - 16]), tail + lane - 16);
-    }
-    for (int i = tid; i < n; i += kThreads) sh.best[i] = 0;
+    ends(push);
     __syncthreads();
-    const int count = sh.count;
+    int count = sh.count, chosen = 0;
+    if (count > kCand) {                           // too many: the n stretches with the largest maxima, equal logits counted
+      if (little) {
+        for (int i = 0; i < nth; ++i) {            // a stretch is one batch
+          uint4 u[kUnroll];
+          fetch(b0 + warp + i * kWarps, u);
+          const float m = warp_max_f32(fmaxf(fmaxf(raw_max<T>(u[0]), raw_max<T>(u[1])), fmaxf(raw_max<T>(u[2]), raw_max<T>(u[3]))));
+          if (lane == 0) sh.stretch[warp + i * kWarps] = m;
+        }
+      } else if (lane < nth) {
+        sh.stretch[warp + lane * kWarps] = maxima;
+      }
+      __syncthreads();
+      for (int i = tid; i < stretches; i += kThreads) {
+        const float v = sh.stretch[i];
+        int rank = 0;
+        for (int j = 0; j < stretches; ++j) {
+          const float w = sh.stretch[j];
+          rank += w > v || (w == v && j < i);
+        }
+        if (rank < n) sh.chosen[rank] = i;
+        if (rank == n - 1) sh.bound = v;
+      }
+      if (tid == 0) sh.count = 0;
+      __syncthreads();
+      bound = sh.bound;
+      chosen = min(n, stretches);
+      for (int r = warp; r < chosen; r += kWarps) {
+        int equal = 0;                             // logits equal to the bound so far; no more than n - r can matter
+        const int v0 = b0 * 32 * kUnroll + sh.chosen[r] * length, v1 = min(v0 + length, v_end);
+        for (int v = v0 + lane; v - lane < v1; v += 32) {
+          float f[N];
+          int mine = 0;
+          if (v < v1) {
+            load16(body + (int64_t)v * N, f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+              f[i] = f[i] == f[i] ? f[i] : -INFINITY;
+              mine += f[i] == bound;
+              if (f[i] > bound) push(f[i], head + v * N + i);
+            }
+          }
+          if (__any_sync(0xffffffffu, mine > 0)) {
+            int inc = mine;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              const int p = __shfl_up_sync(0xffffffffu, inc, o);
+              if (lane >= o) inc += p;
+            }
+            int to = equal + inc - mine;
+            if (mine > 0)
+#pragma unroll
+              for (int i = 0; i < N; ++i)
+                if (f[i] == bound) {
+                  if (to < n - r) push(f[i], head + v * N + i);
+                  ++to;
+                }
+            equal += __shfl_sync(0xffffffffu, inc, 31);
+          }
+        }
+      }
+      ends(push);
+      __syncthreads();
+      count = sh.count;
+    }
     if (count <= kSmall) {
       if (tid < count) {
         const uint64_t k = sh.cand[tid];
@@ -396,10 +481,7 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
             for (int i = 0; i < N; ++i) see(f[i], head + v * N + i);
           }
         }
-        if (part == 0 && warp == kWarps - 1) {
-          if (lane < head) see(q8::to_float(z[lane]), lane);
-          if (lane >= 16 && tail + lane - 16 < V) see(q8::to_float(z[tail + lane - 16]), tail + lane - 16);
-        }
+        ends(see);
         if (tid == 0) sh.round = 0;
         __syncthreads();
         if (mine) atomicMax(reinterpret_cast<unsigned long long*>(&sh.round), (unsigned long long)mine);
@@ -413,49 +495,48 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
 
   // ---- the cluster's parts meet in its first block
   if (parts > 1) {
-    cluster.sync();
-    if (part == 0) {
-      uint64_t k = 0;
-      const int total = parts * n;                 // at most 512: one key a thread
-      if (tid < total) k = cluster.map_shared_rank(&sh, tid / n)->best[tid % n];
-      Sums t{-INFINITY, 0.f, 0.f};
-      if (warp == kWarps - 1) {
-        if (lane < parts) t = cluster.map_shared_rank(&sh, lane)->sums;
-#pragma unroll 1
-        for (int o = 4; o > 0; o /= 2) {
-          const Sums y{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o), __shfl_xor_sync(0xffffffffu, t.x, o)};
-          t = lane & o ? join(y, t, c) : join(t, y, c);
-        }
-      }
-      __syncthreads();                             // the own list has been read
-      if (warp == kWarps - 1 && lane == 0) sh.sums = t;
-      if (tid < total) sh.cand[tid] = k;
-      __syncthreads();
-      if (tid < total && k) {
-        int rank = 0;
-        for (int j = 0; j < total; ++j) rank += sh.cand[j] > k;
-        if (rank < n) sh.best[rank] = k;
-      }
-      __syncthreads();
-    }
-    cluster.sync();                                // the others' shared memory is read no more
-    if (part != 0) return;
-  } else {
     __syncthreads();
+    cluster.barrier_wait();
+    if (part > 0) {
+      Shared* to = cluster.map_shared_rank(&sh, 0);
+      if (tid < n) to->best[part * n + tid] = sh.best[tid];
+      if (tid == 0) to->part_sums[part] = sh.sums;
+    }
+    cluster.barrier_arrive();                      // what was written is there for those who wait
+    if (part > 0) return;
+    cluster.barrier_wait();
+    const int total = parts * n;                   // at most 512: one key a thread
+    const uint64_t k = tid < total ? sh.best[tid] : 0;
+    if (k) {
+      int rank = 0;
+#pragma unroll 4
+      for (int j = 0; j < total; ++j) rank += sh.best[j] > k;
+      if (rank < n) sh.cand[rank] = k;
+    }
+    if (warp == kWarps - 1) {
+      Sums t = lane == 0 ? sh.sums : lane < parts ? sh.part_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
+#pragma unroll 1
+      for (int o = 4; o > 0; o /= 2) {
+        const Sums y{__shfl_xor_sync(0xffffffffu, t.m, o), __shfl_xor_sync(0xffffffffu, t.s, o), __shfl_xor_sync(0xffffffffu, t.x, o)};
+        t = lane & o ? join(y, t, c) : join(t, y, c);
+      }
+      if (lane == 0) sh.sums = t;
+    }
   }
+  const uint64_t* best = parts > 1 ? sh.cand : sh.best;
+  __syncthreads();
   const Sums t = sh.sums;
   const bool empty = t.m == -INFINITY && t.s == 0.f;                          // nothing but -inf
   const float ls = log2f(t.s);
   auto logprob = [&](float v) { return empty ? -INFINITY : fmaf(v - t.m, inv_temp, -ls * kLn2); };
   if (tid == 0) {
-    const int64_t tok = tokens[row];
-    lp[row] = tok >= 0 && tok < V ? logprob(q8::to_float(z[tok])) : 0.f;
+    lp[row] = real ? logprob(z_tok) : 0.f;
     ent[row] = empty ? 0.f : (ls - t.x / t.s) * kLn2;
     stats[2 * row] = t.m;
     stats[2 * row + 1] = ls;
   }
   if (tid < n) {
-    const uint64_t k = sh.best[tid];
+    const uint64_t k = best[tid];
     top_lp[row * n + tid] = logprob(value_of(k));
     top_id[row * n + tid] = index_of(k);
   }
@@ -539,10 +620,11 @@ token_logprob_grad_kernel(const T* __restrict__ logits, int64_t stride, const in
   }
 }
 
-// blocks that share a row
-int cluster_for(int64_t rows) {
+// blocks that share a row: as many as the GPU holds at a time (two an SM), each with some to read
+constexpr int kLeast = 32768;
+int cluster_for(int64_t rows, int64_t row_bytes) {
   int parts = 1;
-  while (parts < 8 && rows * parts * 2 <= 2 * 148) parts *= 2;
+  while (parts < 8 && rows * parts * 2 <= 2 * 148 && row_bytes >= parts * 2 * kLeast) parts *= 2;
   return parts;
 }
 
@@ -563,7 +645,7 @@ std::vector<at::Tensor> token_logprob_fwd(const at::Tensor& z, const at::Tensor&
   auto lp = at::empty({R}, f), ent = at::empty({R}, f), stats = at::empty({R, 2}, f), top = at::empty({R, n}, f);
   auto ids = at::empty({R, n}, z.options().dtype(at::kLong));
   if (R == 0) return {lp, ent, top, ids, stats};
-  const int parts = cluster_for(R);
+  const int parts = cluster_for(R, V * (int64_t)z.element_size());
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(R * parts)); cfg.blockDim = dim3(kThreads); cfg.stream = at::cuda::getCurrentCUDAStream();
   cudaLaunchAttribute attr[2];
