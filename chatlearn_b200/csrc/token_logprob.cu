@@ -29,10 +29,9 @@ namespace cg = cooperative_groups;
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kSmThreads = 1024;                  // threads that an SM holds of it: 2 blocks of 512, or 4 of 256
 constexpr int kMaxTop = 64;
 constexpr int kUnroll = 4;                        // vectors of 16 bytes a lane loads at once
-constexpr int kMaxStretch = 512;                  // stretches of a block
 constexpr int kCand = 4096;                       // n (n + 1) / 2 candidates when all logits are equal, and room; a power of two
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFar = -1000.f;                   // 2^kFar is 0: -inf logits stay out of 0 * inf
@@ -148,6 +147,7 @@ __device__ __forceinline__ Sums join(Sums a, Sums b, float c) {
 constexpr int kSmall = 96;                        // candidates that are ranked by counting; more are sorted
 
 // The block sorts `count` keys, largest first (bitonic; zeros fill up to a power of two).
+template <int kThreads>
 __device__ __forceinline__ void sort_keys(uint64_t* keys, int count) {
   int size = 64;
   while (size < count) size *= 2;
@@ -164,7 +164,9 @@ __device__ __forceinline__ void sort_keys(uint64_t* keys, int count) {
     }
 }
 
+template <int kThreads>
 struct __align__(16) Shared {
+  static constexpr int kWarps = kThreads / 32, kMaxStretch = kThreads;
   float stretch[kMaxStretch];
   uint64_t cand[kCand];
   uint64_t best[8 * kMaxTop];                     // the cluster's lists, in the first block
@@ -177,12 +179,14 @@ struct __align__(16) Shared {
   int count;
 };
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 2)
+template <typename T, int kThreads>
+__global__ void __launch_bounds__(kThreads, kSmThreads / kThreads)
 token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t* __restrict__ tokens, int V, int n, float c,
                      float inv_temp, float* __restrict__ lp, float* __restrict__ ent, float* __restrict__ stats, float* __restrict__ top_lp,
                      int64_t* __restrict__ top_id) {
-  __shared__ Shared sh;
+  __shared__ Shared<kThreads> sh;
+  constexpr int kWarps = kThreads / 32;
+  constexpr int kMaxStretch = kThreads;            // stretches of a block: 32 of a warp
   constexpr int N = Wide<T>::N;
   pdl_trigger();
   pdl_wait();
@@ -451,7 +455,7 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
       count = sh.count;
     }
     if (count <= kSmall) {
-      if (tid < count) {
+      if (tid < count) {                           // (kSmall < kThreads)
         const uint64_t k = sh.cand[tid];
         int rank = 0;
         for (int j = 0; j < count; ++j) rank += sh.cand[j] > k;
@@ -459,7 +463,7 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
       }
       __syncthreads();
     } else if (count <= kCand) {
-      sort_keys(sh.cand, count);
+      sort_keys<kThreads>(sh.cand, count);
       if (tid < n && tid < count) sh.best[tid] = sh.cand[tid];
       __syncthreads();
     } else {
@@ -498,20 +502,20 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
     __syncthreads();
     cluster.barrier_wait();
     if (part > 0) {
-      Shared* to = cluster.map_shared_rank(&sh, 0);
+      Shared<kThreads>* to = cluster.map_shared_rank(&sh, 0);
       if (tid < n) to->best[part * n + tid] = sh.best[tid];
       if (tid == 0) to->part_sums[part] = sh.sums;
     }
     cluster.barrier_arrive();                      // what was written is there for those who wait
     if (part > 0) return;
     cluster.barrier_wait();
-    const int total = parts * n;                   // at most 512: one key a thread
-    const uint64_t k = tid < total ? sh.best[tid] : 0;
-    if (k) {
+    const int total = parts * n;
+    for (int i = tid; i < total; i += kThreads) {
+      const uint64_t k = sh.best[i];
       int rank = 0;
 #pragma unroll 4
       for (int j = 0; j < total; ++j) rank += sh.best[j] > k;
-      if (rank < n) sh.cand[rank] = k;
+      if (k && rank < n) sh.cand[rank] = k;
     }
     if (warp == kWarps - 1) {
       Sums t = lane == 0 ? sh.sums : lane < parts ? sh.part_sums[lane] : Sums{-INFINITY, 0.f, 0.f};
@@ -545,8 +549,8 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
 // dz_j = 1/temperature [ g_lp d(j = token) + sum_k g_top_k d(j = top_k) - p_j (g_lp + sum_k g_top_k) - g_ent p_j (ln p_j + H) ]
 // One read of the logits, one write of the gradient; the columns of the token and the alternatives are written again
 // after the stretch that holds them.
-constexpr int kGradThreads = 256;
-constexpr int kGradSpan = 16384;                  // bytes of a row that a block handles
+constexpr int kGradThreads = 256, kGradVecs = 4;   // vectors of a thread, all on their way at a time
+constexpr int kGradSpan = kGradThreads * kGradVecs * 16;                    // bytes of a row that a block handles
 
 template <typename T>
 __global__ void __launch_bounds__(kGradThreads)
@@ -554,52 +558,55 @@ token_logprob_grad_kernel(const T* __restrict__ logits, int64_t stride, const in
                           int spans, float c, float inv_temp, const float* __restrict__ ent, const float* __restrict__ stats,
                           const int64_t* __restrict__ top_id, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
                           const float* __restrict__ g_top, T* __restrict__ dz, int64_t dz_stride) {
-  __shared__ float sh_sum;
   constexpr int N = Wide<T>::N;
   pdl_trigger();
   pdl_wait();
-  const int64_t row = blockIdx.x / spans;
-  const int span = (int)(blockIdx.x % spans), tid = threadIdx.x, lane = tid & 31;
+  // last rows first: the forward pass has left them in L2
+  const int64_t row = (gridDim.x - 1 - blockIdx.x) / spans;
+  const int span = (int)((gridDim.x - 1 - blockIdx.x) % spans), tid = threadIdx.x, lane = tid & 31;
   const T* z = logits + row * stride;
   T* d = dz + row * dz_stride;
+  // both rows at the same place inside 16 bytes: vectors; else single elements
+  const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+  const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
+  const int head = same ? min(V, mis ? N - mis : 0) : 0, vecs = same ? (V - head) / N : 0, tail = head + vecs * N;
+  constexpr int kVecs = kGradSpan / 16;
+  const int v0 = span * kVecs + tid;
+  uint4 raw[kGradVecs];
+#pragma unroll
+  for (int i = 0; i < kGradVecs; ++i)
+    if (v0 + i * kGradThreads < vecs) raw[i] = load_raw(z + head + (int64_t)(v0 + i * kGradThreads) * N);
   const int64_t tok = tokens[row];
   const float M = stats[2 * row], ls = stats[2 * row + 1], H = ent[row];
   const bool empty = M == -INFINITY && ls == -INFINITY;                       // log2 of an empty sum
   const float gl = g_lp && tok >= 0 && tok < V ? g_lp[row] : 0.f, ge = g_ent ? g_ent[row] : 0.f;
-  if (tid < 32) {
-    float s = 0.f;
-    if (g_top)
-      for (int i = lane; i < n; i += 32) s += g_top[row * n + i];
-    s = warp_sum(s);
-    if (lane == 0) sh_sum = s;
+  float g_all = 0.f;                               // every warp for itself
+  if (g_top) {
+    for (int i = lane; i < n; i += 32) g_all += g_top[row * n + i];
+    g_all = warp_sum(g_all);
   }
-  __syncthreads();
   // p (A x + B) with x = log2 p
-  const float A = -inv_temp * ge * kLn2, B = -inv_temp * (gl + sh_sum + ge * H);
+  const float A = -inv_temp * ge * kLn2, B = -inv_temp * (gl + g_all + ge * H);
   auto grad = [&](float v) {
     const float x = max_nan(fmaf(v - M, c, -ls), kFar);
     return empty ? 0.f : exp2_approx(x) * fmaf(x, A, B);
   };
-  const int mis = (int)((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
-  const bool same = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(d)) & 15) == 0;
-  // both rows at the same place inside 16 bytes: vectors; else single elements
-  const int head = same ? min(V, mis ? N - mis : 0) : 0, vecs = same ? (V - head) / N : 0, tail = head + vecs * N;
-  constexpr int kVecs = kGradSpan / 16;
-  const int v0 = span * kVecs, v1 = min(v0 + kVecs, vecs);
   int lo, hi;                                      // columns of this block
   if (same) {
-    lo = span == 0 ? 0 : head + v0 * N;
-    hi = span == spans - 1 ? V : min(V, head + (v0 + kVecs) * N);
+    lo = span == 0 ? 0 : head + span * kVecs * N;
+    hi = span == spans - 1 ? V : min(V, head + (span + 1) * kVecs * N);
     if (span == 0 && tid < head) d[tid] = q8::from_float<T>(grad(q8::to_float(z[tid])));
-    for (int v = v0 + tid; v < v1; v += kGradThreads) {
-      float f[N];
-      load16(z + head + (int64_t)v * N, f);
-      uint4 u;
-      T* o = reinterpret_cast<T*>(&u);
 #pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = q8::from_float<T>(grad(f[i]));
-      *reinterpret_cast<uint4*>(d + head + (int64_t)v * N) = u;
-    }
+    for (int i = 0; i < kGradVecs; ++i)
+      if (v0 + i * kGradThreads < vecs) {
+        float f[N];
+        expand<T>(raw[i], f);
+        uint4 u;
+        T* o = reinterpret_cast<T*>(&u);
+#pragma unroll
+        for (int e = 0; e < N; ++e) o[e] = q8::from_float<T>(grad(f[e]));
+        __stcs(reinterpret_cast<uint4*>(d + head + (int64_t)(v0 + i * kGradThreads) * N), u);
+      }
     if (span == spans - 1)
       for (int i = tail + tid; i < V; i += kGradThreads) d[i] = q8::from_float<T>(grad(q8::to_float(z[i])));
   } else {
@@ -607,24 +614,29 @@ token_logprob_grad_kernel(const T* __restrict__ logits, int64_t stride, const in
     hi = span == spans - 1 ? V : min(V, lo + kVecs * N);
     for (int i = lo + tid; i < hi; i += kGradThreads) d[i] = q8::from_float<T>(grad(q8::to_float(z[i])));
   }
+  // thread n: the token; an alternative that is the token is its job
+  const int64_t col = tid < n ? top_id[row * n + tid] : tok;
+  const bool own = tid <= n && !empty && col >= lo && col < hi && !(tid < n && col == tok);
   __syncthreads();
-  if (tid <= n && !empty) {                        // thread n: the token; an alternative that is the token is its job
-    const int64_t col = tid < n ? top_id[row * n + tid] : tok;
-    if (col >= lo && col < hi && !(tid < n && col == tok)) {
-      float add = tid < n ? (g_top ? g_top[row * n + tid] : 0.f) : gl;
-      if (tid == n && g_top)
-        for (int i = 0; i < n; ++i)
-          if (top_id[row * n + i] == tok) add += g_top[row * n + i];
-      d[col] = q8::from_float<T>(fmaf(add, inv_temp, grad(q8::to_float(z[col]))));
-    }
+  if (own) {
+    float add = tid < n ? (g_top ? g_top[row * n + tid] : 0.f) : gl;
+    if (tid == n && g_top)
+      for (int i = 0; i < n; ++i)
+        if (top_id[row * n + i] == tok) add += g_top[row * n + i];
+    d[col] = q8::from_float<T>(fmaf(add, inv_temp, grad(q8::to_float(z[col]))));
   }
 }
 
-// blocks that share a row: as many as the GPU holds at a time (two an SM), each with some to read
+// Threads of a block: 512 (more to read for each of what a block does once); 256 where rows are so short that this is most
+// of the time (300 rows, 512 and 256 threads: 4000 fp32 logits with 20 alternatives 13.7 and 9.9 us, 32 k with 5 16.4 and
+// 15.3 us; 128 rows of 152 k bf16 logits with 8 20.0 and 26.4 us).
+constexpr int kShortRow = 160 << 10;
+// blocks that share a row: as many as the GPU holds at a time, each with some to read
 constexpr int kLeast = 32768;
-int cluster_for(int64_t rows, int64_t row_bytes) {
+int cluster_for(int64_t rows, int64_t row_bytes, int threads) {
+  const int kBlocks = kSmThreads / threads;
   int parts = 1;
-  while (parts < 8 && rows * parts * 2 <= 2 * 148 && row_bytes >= parts * 2 * kLeast) parts *= 2;
+  while (parts < 8 && rows * parts * 2 <= kBlocks * 148 && row_bytes >= parts * 2 * kLeast) parts *= 2;
   return parts;
 }
 
@@ -645,9 +657,11 @@ std::vector<at::Tensor> token_logprob_fwd(const at::Tensor& z, const at::Tensor&
   auto lp = at::empty({R}, f), ent = at::empty({R}, f), stats = at::empty({R, 2}, f), top = at::empty({R, n}, f);
   auto ids = at::empty({R, n}, z.options().dtype(at::kLong));
   if (R == 0) return {lp, ent, top, ids, stats};
-  const int parts = cluster_for(R, V * (int64_t)z.element_size());
+  const int64_t row_bytes = V * (int64_t)z.element_size();
+  const int threads = row_bytes <= kShortRow ? 256 : 512;
+  const int parts = cluster_for(R, row_bytes, threads);
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(R * parts)); cfg.blockDim = dim3(kThreads); cfg.stream = at::cuda::getCurrentCUDAStream();
+  cfg.gridDim = dim3((unsigned)(R * parts)); cfg.blockDim = dim3(threads); cfg.stream = at::cuda::getCurrentCUDAStream();
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = parts; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
@@ -657,7 +671,7 @@ std::vector<at::Tensor> token_logprob_fwd(const at::Tensor& z, const at::Tensor&
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   const float c = (float)(inv_temp * 1.4426950408889634);
 #define LAUNCH(T)                                                                                                        \
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, token_logprob_kernel<T>, (const T*)z.data_ptr(), z.stride(0),                   \
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, threads == 256 ? token_logprob_kernel<T, 256> : token_logprob_kernel<T, 512>, (const T*)z.data_ptr(), z.stride(0),                   \
                                     (const int64_t*)tokens.data_ptr<int64_t>(), (int)V, (int)n, c, (float)inv_temp, lp.data_ptr<float>(),  \
                                     ent.data_ptr<float>(), stats.data_ptr<float>(), top.data_ptr<float>(), ids.data_ptr<int64_t>()))
   if (z.scalar_type() == at::kFloat) LAUNCH(float);
