@@ -39,28 +39,53 @@ struct AppendArgs {
   int64_t pages;
 };
 
-// 8 consecutive elements as fp32; `vec`: the address is 16-byte aligned
+// 8 consecutive elements as they are, and as fp32; `vec`: the address is 16-byte aligned
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, float (&f)[8]) {
+struct __align__(16) Raw {
+  T x[8];
+};
+template <typename T>
+__device__ __forceinline__ Raw<T> load8(const T* p, bool vec) {
+  Raw<T> r;
   if (vec) {
 #pragma unroll
-    for (int i = 0; i < 8; i += 16 / (int)sizeof(T)) {
-      const uint4 u = *reinterpret_cast<const uint4*>(p + i);
-      const T* t = reinterpret_cast<const T*>(&u);
-#pragma unroll
-      for (int j = 0; j < 16 / (int)sizeof(T); ++j) f[i + j] = to_float(t[j]);
-    }
+    for (int i = 0; i < 8; i += 16 / (int)sizeof(T)) *reinterpret_cast<uint4*>(&r.x[i]) = *reinterpret_cast<const uint4*>(p + i);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_float(p[i]);
+    for (int i = 0; i < 8; ++i) r.x[i] = p[i];
   }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void expand(const Raw<T>& r, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = to_float(r.x[i]);
 }
 
-// largest finite magnitude
-__device__ __forceinline__ float finite_max(float m, const float (&f)[8]) {
+// Largest magnitude, NaN left out, infinities not; and the largest finite one, for where there are infinities.  (bf16 and
+// fp16 two at a time: an and and a maximum for two elements.)
+__device__ __forceinline__ float magnitude(const Raw<float>& r) {
+  float m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(r.x[i]));
+  return m;
+}
+__device__ __forceinline__ float magnitude(const Raw<__nv_bfloat16>& r) {
+  const __nv_bfloat162* x = reinterpret_cast<const __nv_bfloat162*>(r.x);
+  const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(x[0]), __habs2(x[1])), __hmax2(__habs2(x[2]), __habs2(x[3])));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+__device__ __forceinline__ float magnitude(const Raw<__half>& r) {
+  const __half2* x = reinterpret_cast<const __half2*>(r.x);
+  const __half2 m = __hmax2(__hmax2(__habs2(x[0]), __habs2(x[1])), __hmax2(__habs2(x[2]), __habs2(x[3])));
+  return fmaxf(__low2float(m), __high2float(m));
+}
+template <typename T>
+__device__ __forceinline__ float finite_magnitude(const Raw<T>& r) {
+  float m = 0.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float a = fabsf(f[i]);
+    const float a = fabsf(to_float(r.x[i]));
     m = a < INFINITY ? fmaxf(m, a) : m;
   }
   return m;
@@ -96,14 +121,15 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
   if (b >= min(a.B, a.T)) return;
   const T* x = static_cast<const T*>(a.x[kv]) + b * a.row[kv] + h * a.head[kv];
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-  float f[2][8], amax = 0.f;                       // D <= 512
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if ((i * 32 + lane) * 8 < a.D) {
-      load8(x + (i * 32 + lane) * 8, vec, f[i]);
-      amax = finite_max(amax, f[i]);
-    }
+  Raw<T> kept;                                     // D <= 256: 8 elements of a lane
+  float amax = 0.f;
+  const bool mine = lane * 8 < a.D;
+  if (mine) {
+    kept = load8(x + lane * 8, vec);
+    amax = magnitude(kept);
+  }
   amax = warp_max(amax);
+  if (!(amax < INFINITY)) amax = warp_max(mine ? finite_magnitude(kept) : 0.f);
   const int pos = a.lens[b] - 1;
   if (pos < 0 || pos / a.bs >= a.width) return;
   const int page = a.tables[(int64_t)b * a.width + pos / a.bs], off = pos % a.bs;
@@ -119,104 +145,103 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
   __syncwarp();
   if (lane == 0) a.scale[kv][ph] = s;
   const float inv = 1.f / s;
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    if ((i * 32 + lane) * 8 < a.D) store8(codes + (int64_t)off * a.D + (i * 32 + lane) * 8, f[i], inv);
+  if (mine) {
+    float f[8];
+    expand(kept, f);
+    store8(codes + (int64_t)off * a.D + lane * 8, f, inv);
+  }
 }
 
 // Any number of tokens per sequence: a block per (page that gets new rows, kv head, K or V).  The rows of a page of 64 x
 // 128 fit the block's registers (kKeep vectors of 8 a thread), so they are read once; longer pages read the rest again,
-// out of L2.
+// out of L2.  Blocks of the same rows run side by side (heads, then K and V): a row's heads lie beside each other.
 constexpr int kKeep = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) append_pages_kernel(const AppendArgs a) {
-  __shared__ int sh_scan[2][kThreads / 32];
   __shared__ int sh_found[4];
   __shared__ float sh_max[kThreads / 32];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int h = blockIdx.x % a.nkv, kv = blockIdx.x / a.nkv & 1, run = blockIdx.x / (2 * a.nkv);
   // which (sequence, page) is this block's: prefix sums of the pages and rows that the sequences add
-  if (tid == 0) sh_found[0] = -1;
-  int base_pages = 0, base_rows = 0;
-  for (int b0 = 0; b0 < a.B; b0 += kThreads) {
-    const int b = b0 + tid;
-    int n = 0, len = 0, cnt = 0;
-    if (b < a.B) {
-      len = a.lens[b];
-      n = max(0, a.news ? a.news[b] : min(1, len));
-      const int from = max(len - n, 0);
-      cnt = (n > 0 && len > 0) ? (len - 1) / a.bs - from / a.bs + 1 : 0;
-    }
-    int ip = cnt, ir = n;
+  if (warp == 0) {
+    if (lane == 0) sh_found[0] = -1;
+    __syncwarp();
+    int pages = 0, rows = 0;                       // before these 32 sequences
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      const int b = b0 + lane;
+      const int len = b < a.B ? a.lens[b] : 0, n = b < a.B ? max(0, a.news[b]) : 0, begin = max(len - n, 0);
+      const int cnt = n > 0 && len > 0 ? (len - 1) / a.bs - begin / a.bs + 1 : 0;
+      int ip = cnt, ir = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int p = __shfl_up_sync(0xffffffffu, ip, o), r = __shfl_up_sync(0xffffffffu, ir, o);
-      if (lane >= o) { ip += p; ir += r; }
+      for (int o = 1; o < 32; o <<= 1) {
+        const int p = __shfl_up_sync(0xffffffffu, ip, o), r = __shfl_up_sync(0xffffffffu, ir, o);
+        if (lane >= o) { ip += p; ir += r; }
+      }
+      const int first = pages + ip - cnt;
+      if (cnt > 0 && first <= run && run < first + cnt) {
+        const int pg = begin / a.bs + (run - first);
+        const int lo = max(begin, pg * a.bs), hi = min(len, (pg + 1) * a.bs);
+        const int row = rows + ir - n + (lo - (len - n));      // row of the page's first new token
+        sh_found[1] = lo - pg * a.bs;
+        sh_found[2] = min(hi - lo, a.T - row);                 // rows that the tensors really hold
+        sh_found[3] = row;
+        if (sh_found[2] > 0 && pg < a.width) sh_found[0] = a.tables[(int64_t)b * a.width + pg];
+      }
+      pages += __shfl_sync(0xffffffffu, ip, 31);
+      rows += __shfl_sync(0xffffffffu, ir, 31);
+      if (pages > run) break;
     }
-    __syncthreads();
-    if (lane == 31) { sh_scan[0][warp] = ip; sh_scan[1][warp] = ir; }
-    __syncthreads();
-    int bp = base_pages, br = base_rows;
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) { bp += sh_scan[0][w]; br += sh_scan[1][w]; }
-      base_pages += sh_scan[0][w]; base_rows += sh_scan[1][w];
-    }
-    const int first = bp + ip - cnt;
-    if (cnt > 0 && first <= (int)blockIdx.x && (int)blockIdx.x < first + cnt) {
-      const int from = max(len - n, 0), pg = from / a.bs + ((int)blockIdx.x - first);
-      const int lo = max(from, pg * a.bs), hi = min(len, (pg + 1) * a.bs);
-      int row = br + ir - n + (lo - (len - n));               // row of the page's first new token
-      sh_found[1] = lo % a.bs;
-      sh_found[2] = min(hi - lo, a.T - row);                   // rows that the tensors really hold
-      sh_found[3] = row;
-      if (sh_found[2] > 0 && pg < a.width) sh_found[0] = a.tables[(int64_t)b * a.width + pg];
-    }
-    __syncthreads();
-    if (base_pages > (int)blockIdx.x) break;
   }
+  __syncthreads();
   const int page = sh_found[0], off = sh_found[1], m = sh_found[2], row = sh_found[3];
   if (page < 0 || page >= a.pages) return;
-  const int h = blockIdx.y, kv = blockIdx.z;
   const T* x = static_cast<const T*>(a.x[kv]) + row * a.row[kv] + h * a.head[kv];
   const bool vec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(a.row[kv] * sizeof(T))) & 15) == 0;
-  const int per = a.D / 8, total = m * per;
-  float f[kKeep][8], amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    const int c = i * kThreads + tid;
-    if (c < total) {
-      load8(x + (c / per) * a.row[kv] + (c % per) * 8, vec, f[i]);
-      amax = finite_max(amax, f[i]);
-    }
-  }
-  for (int c = kKeep * kThreads + tid; c < total; c += kThreads) {
-    float g[8];
-    load8(x + (c / per) * a.row[kv] + (c % per) * 8, vec, g);
-    amax = finite_max(amax, g);
-  }
-  amax = warp_max(amax);
-  if (lane == 0) sh_max[warp] = amax;
+  const int shift = a.D == 64 ? 3 : a.D == 128 ? 4 : 5, total = m << shift;
+  // the thread's vectors, tid + i * kThreads; those of a row lie side by side
+  auto at = [&](int c) { return (c >> shift) * a.row[kv] + (c & ((1 << shift) - 1)) * 8; };
   const int64_t ph = (int64_t)page * a.nkv + h;
   const float old = off > 0 ? a.scale[kv][ph] : 0.f;
-  __syncthreads();
+  Raw<T> kept[kKeep];
+  float amax = 0.f, f[8];
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) amax = fmaxf(amax, sh_max[w]);
+  for (int i = 0; i < kKeep; ++i)
+    if (i * kThreads + tid < total) kept[i] = load8(x + at(i * kThreads + tid), vec);
+  auto largest = [&](auto of) {                    // over the block, by `of` each vector
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < kKeep; ++i)
+      if (i * kThreads + tid < total) m = fmaxf(m, of(kept[i]));
+    for (int c = kKeep * kThreads + tid; c < total; c += kThreads) m = fmaxf(m, of(load8(x + at(c), vec)));
+    m = warp_max(m);
+    if (lane == 0) sh_max[warp] = m;
+    __syncthreads();                               // every thread has read the old scale, too
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, sh_max[w]);
+    return m;
+  };
+  amax = largest([](const Raw<T>& r) { return magnitude(r); });
+  if (!(amax < INFINITY)) {
+    __syncthreads();
+    amax = largest([](const Raw<T>& r) { return finite_magnitude(r); });
+  }
   const float s = fmaxf(scale_for(amax), old), inv = 1.f / s;
   uint8_t* codes = a.codes[kv] + ph * a.bs * a.D;
   if (off > 0 && s > old) regrade(codes, off * a.D, old / s, tid, kThreads);
-  if (tid == 0) a.scale[kv][ph] = s;               // every thread has read the old scale before the barrier above
+  if (tid == 0) a.scale[kv][ph] = s;
   uint8_t* to = codes + (int64_t)off * a.D;
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    const int c = i * kThreads + tid;
-    if (c < total) store8(to + c * 8, f[i], inv);
-  }
+  for (int i = 0; i < kKeep; ++i)
+    if (i * kThreads + tid < total) {
+      expand(kept[i], f);
+      store8(to + (i * kThreads + tid) * 8, f, inv);
+    }
   for (int c = kKeep * kThreads + tid; c < total; c += kThreads) {
-    float g[8];
-    load8(x + (c / per) * a.row[kv] + (c % per) * 8, vec, g);
-    store8(to + c * 8, g, inv);
+    expand(load8(x + at(c), vec), f);
+    store8(to + c * 8, f, inv);
   }
 }
 
@@ -229,7 +254,7 @@ void launch_append(const AppendArgs& a, cudaStream_t st) {
   } else {
     // a sequence with n new tokens adds to at most (n - 1) / bs + 2 pages
     const int64_t runs = std::min<int64_t>(a.T, a.T / a.bs + 2 * (int64_t)a.B);
-    C10_CUDA_CHECK(launch_pdl(append_pages_kernel<T>, dim3((unsigned)runs, a.nkv, 2), dim3(kThreads), 0, st, a));
+    C10_CUDA_CHECK(launch_pdl(append_pages_kernel<T>, dim3((unsigned)(runs * a.nkv * 2)), dim3(kThreads), 0, st, a));
   }
 }
 
