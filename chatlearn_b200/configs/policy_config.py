@@ -38,7 +38,11 @@ class RolloutConfig(BaseModelConfig):
     gpu_memory_utilization: float = 0.8
     enforce_eager: bool = False
     kv_block_size: int = 64
+    # "auto" (the model's dtype) or "fp8_e4m3": keys and values as 8-bit codes with a power-of-two scale per block and kv head
+    kv_cache_dtype: str = "auto"
     max_num_seqs: int = 256
+    # alternatives (token, log-prob) and the entropy to hand back with every generated token (0: none)
+    num_logprobs: int = 0
     # agent tasks: "continuous" = every model turn is its own request in an open engine session (a trajectory's
     # next turn joins the running batch as soon as its tools return); "lockstep" = one batched call per round
     agent_scheduling: str = "continuous"
@@ -64,3 +68,6 @@ class PolicyConfig(RolloutConfig):
         assert self.num_gpu > 0 and self.num_gpu % mp == 0, \
             f"policy.num_gpu={self.num_gpu} must be a multiple of tp*ep={mp}"
         assert 0.0 < self.gpu_memory_utilization <= 1.0
+        assert self.kv_cache_dtype in ("auto", "fp8_e4m3"), \
+            f"policy.kv_cache_dtype is auto or fp8_e4m3, not {self.kv_cache_dtype}"
+        assert 0 <= self.num_logprobs <= 64, "policy.num_logprobs: 0 to 64"

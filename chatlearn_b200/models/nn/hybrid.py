@@ -258,18 +258,18 @@ def gated_attention(arch: ModelArch, p, x, ctx, layer: int):
         q = torch.cat([ops.rope(q[..., :rd].contiguous(), pos, arch.rope_theta), q[..., rd:]], dim=-1)
         k = torch.cat([ops.rope(k[..., :rd].contiguous(), pos, arch.rope_theta), k[..., rd:]], dim=-1)
     scale = 1.0 / math.sqrt(d)
+    from .model import cache_append, cache_attend
     kv = ctx.kv
     if sp is not None:
         # Ulysses: all rows of 1/sp of the heads through attention, then back (the output gate stays with the rows)
         assert kv is None
         q, k, v = sp.seq_to_heads(q.contiguous()), sp.seq_to_heads(k.contiguous(), kv=True), sp.seq_to_heads(v.contiguous(), kv=True)
     if kv is not None:
-        ops.kv_append(k, v.contiguous(), kv.k_cache[layer], kv.v_cache[layer], kv.slot_mapping)
+        cache_append(kv, layer, k, v.contiguous(), ctx)
         if kv.prefill_only:
             o = ops.attention_varlen(q, k, v, ctx.cu_seqlens, ctx.max_seqlen, scale)
         else:
-            o = ops.paged_attention(q, kv.k_cache[layer], kv.v_cache[layer], kv.block_tables,
-                                    kv.seq_lens, kv.q_lens, scale)
+            o = cache_attend(kv, layer, q, scale, ctx)
     elif ctx.cp is not None and ctx.cp.size > 1:
         o = ctx.cp.attention(q.contiguous(), k.contiguous(), v.contiguous(), ctx, scale)    # keys / values gathered
     else:

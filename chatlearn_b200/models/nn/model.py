@@ -138,6 +138,7 @@ class KVCtx:
     q_lens: Optional[torch.Tensor] = None  # [B] new tokens per sequence (None → 1 each)
     prefill_only: bool = False             # all sequences start at position 0 → varlen kernel
     groups: Any = None                     # decode steps: (group members, shared blocks per group, per-sequence first private block): sequences sharing their prompt blocks
+    q8: Any = None                         # per layer ops.Q8KVCache: the cache is held in 8 bits (k_cache / v_cache are its codes)
     lin: Any = None                        # models.nn.hybrid.LinearState: conv / recurrent state of gated delta-net layers
 
 
@@ -164,6 +165,22 @@ class FwdCtx:
     deepstack: Any = None                  # (rows, [features per early layer]): vision taps added after layer i (Qwen3-VL)
     seq_parallel: bool = False             # residual stream and norms hold 1/tp of the rows (Megatron sequence parallelism)
     row_valid: Optional[torch.Tensor] = None   # [rows] bool: False for alignment padding (kept out of the balancing loss)
+
+
+def cache_append(kv: KVCtx, layer: int, k, v, ctx: FwdCtx):
+    """The new rows' keys and values into the layer's cache."""
+    if kv.q8 is not None:
+        ops.kv_append_q8(k, v, kv.q8[layer], kv.block_tables, kv.seq_lens, None if ctx.max_seqlen == 1 else kv.q_lens)
+    else:
+        ops.kv_append(k, v, kv.k_cache[layer], kv.v_cache[layer], kv.slot_mapping)
+
+
+def cache_attend(kv: KVCtx, layer: int, q, scale: float, ctx: FwdCtx):
+    """Attention of the new rows over the layer's cache."""
+    if kv.q8 is not None:
+        return ops.paged_attention_q8(q, kv.q8[layer], kv.block_tables, kv.seq_lens, None if ctx.max_seqlen == 1 else kv.q_lens, scale)
+    return ops.paged_attention(q, kv.k_cache[layer], kv.v_cache[layer], kv.block_tables, kv.seq_lens, kv.q_lens, scale,
+                               groups=kv.groups)
 
 
 def _tp_reduce(x, ctx):
@@ -252,7 +269,7 @@ def attention_block(arch: ModelArch, p: Dict[str, torch.Tensor], x, ctx: FwdCtx,
             # Ulysses: the rotary parts were rotated with this rank's positions; trade rows for heads
             q, k, v = ctx.sp.seq_to_heads(q.contiguous()), ctx.sp.seq_to_heads(k.contiguous()), ctx.sp.seq_to_heads(v)
     else:
-        paged = (ctx.kv is not None and not ctx.kv.prefill_only and ctx.mrope_positions is None and not torch.is_grad_enabled()
+        paged = (ctx.kv is not None and not ctx.kv.prefill_only and ctx.kv.q8 is None and ctx.mrope_positions is None and not torch.is_grad_enabled()
                  and (ctx.sp is None or ctx.sp.size == 1))
         if paged and ctx.planes_ok and p.get("qkv_bias") is None and x.dim() == 2:
             qkv = ops.linear_planes(x, p["qkv"])          # the fused kernel below adds the K slices up itself
@@ -291,12 +308,13 @@ def attention_block(arch: ModelArch, p: Dict[str, torch.Tensor], x, ctx: FwdCtx,
     kv = ctx.kv
     if kv is not None:
         if not arch.use_mla:                 # (the latent row of an MLA layer is already in the cache)
-            ops.kv_append(k, v, kv.k_cache[layer], kv.v_cache[layer], kv.slot_mapping)
+            cache_append(kv, layer, k, v, ctx)
         if kv.prefill_only:
             o = ops.attention_varlen(q, k, v, ctx.cu_seqlens, ctx.max_seqlen, scale)
         else:
-            o = ops.paged_attention(q, kv.k_cache[layer], kv.v_cache[layer], kv.block_tables,
-                                    kv.seq_lens, kv.q_lens, scale, groups=kv.groups)
+            o = cache_attend(kv, layer, q, scale, ctx)
+            if kv.q8 is not None and not partial:
+                return _row_parallel(o.reshape(o.shape[0], -1), p["o_proj"], ctx)
     elif ctx.cp is not None and ctx.cp.size > 1:
         o = ctx.cp.attention(q, k, v, ctx, scale)
     else:

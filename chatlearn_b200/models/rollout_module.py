@@ -101,6 +101,7 @@ class RolloutModule(TorchModule):
             max_num_seqs=int(getattr(ma, "max_num_seqs", 256)),
             max_num_batched_tokens=int(ma.max_num_batched_tokens),
             gpu_memory_utilization=float(ma.gpu_memory_utilization),
+            kv_dtype=torch.float8_e4m3fn if str(getattr(ma, "kv_cache_dtype", "auto")) == "fp8_e4m3" else None,
             max_model_len=int(ma.seq_length), seed=int(ma.seed) + 7919 * self.replica_index,
             lockstep_group=self.ep_group if self._ep > 1 else None,
             use_cuda_graphs=not bool(getattr(ma, "enforce_eager", False)),
@@ -127,7 +128,7 @@ class RolloutModule(TorchModule):
             presence_penalty=getattr(ma, p + "presence_penalty"),
             frequency_penalty=getattr(ma, p + "frequency_penalty"),
             repetition_penalty=getattr(ma, p + "repetition_penalty"), max_tokens=max_tokens,
-            ignore_eos=bool(getattr(ma, "ignore_eos", False)))
+            ignore_eos=bool(getattr(ma, "ignore_eos", False)), logprobs=int(getattr(ma, "num_logprobs", 0)))
 
     def generate(self, data_list: List[Dict], is_eval: bool = False):
         ma = self.module_args
@@ -162,6 +163,10 @@ class RolloutModule(TorchModule):
                 if self.tokenizer is not None else ""
             r["finish_reason"] = q.finish_reason
             r["rollout_logprobs"] = torch.tensor(q.logprobs, dtype=torch.float32)
+            if q.top_logprobs:
+                r["rollout_entropies"] = torch.tensor(q.entropies, dtype=torch.float32)
+                r["rollout_top_ids"] = torch.tensor([[i for i, _ in t] for t in q.top_logprobs], dtype=torch.long)
+                r["rollout_top_logprobs"] = torch.tensor([[l for _, l in t] for t in q.top_logprobs], dtype=torch.float32)
             if "rollout_round" in r:
                 r["rollout_round"] += 1
             out.append(r)

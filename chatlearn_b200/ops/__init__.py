@@ -73,7 +73,9 @@ def _dispatch(name):
     r = getattr(ref, name)
 
     def op(*args, **kwargs):
-        t = next(a for a in args if isinstance(a, torch.Tensor))
+        t = next((a for a in args if isinstance(a, torch.Tensor)), None)
+        if t is None:
+            t = next(a for a in kwargs.values() if isinstance(a, torch.Tensor))
         if _use_native(name, t):
             return _NATIVE[name](*args, **kwargs)
         return r(*args, **kwargs)

@@ -23,6 +23,9 @@ from chatlearn_b200.utils.constant import TAG_KV_CACHE, TAG_WEIGHTS
 from .scheduler import Scheduler, Sequence, StepPlan
 
 
+MAX_LOGPROBS = 64          # alternatives per token that the statistics kernel ranks
+
+
 @dataclass
 class SamplingParams:
     temperature: float = 1.0
@@ -35,6 +38,7 @@ class SamplingParams:
     max_tokens: int = 16
     stop_token_ids: Seq[int] = ()
     ignore_eos: bool = False
+    logprobs: int = 0          # alternatives (and the entropy) to hand back with every generated token
 
     @property
     def has_penalty(self):
@@ -43,7 +47,7 @@ class SamplingParams:
 
     def key(self):
         return (self.temperature, self.top_p, self.top_k, self.min_p, self.presence_penalty,
-                self.frequency_penalty, self.repetition_penalty)
+                self.frequency_penalty, self.repetition_penalty, self.logprobs)
 
 
 class RolloutEngine:
@@ -86,6 +90,15 @@ class RolloutEngine:
         self.max_model_len = max_model_len
         self.util = gpu_memory_utilization
         self.kv_dtype = kv_dtype or model.dtype
+        # float8_e4m3fn: e4m3 codes with a power-of-two scale per block and kv head (ops.Q8KVCache)
+        self.q8 = self.kv_dtype == torch.float8_e4m3fn
+        if self.q8 and self.arch.use_mla:
+            raise ValueError("an 8-bit KV cache holds keys and values per head: not for latent attention")
+        if self.q8 and self.device.type == "cuda" and ops.get_mode() == "native" \
+                and (self.arch.head_dim not in (64, 128, 256) or block_size % 16 or model.dtype != torch.bfloat16):
+            raise ValueError("an 8-bit KV cache on a GPU: bf16 models of head dim 64, 128 or 256, blocks of a multiple of 16 "
+                             f"tokens; got {model.dtype}, {self.arch.head_dim}, {block_size}")
+        self.q8_cache: List[Any] = []
         self._num_blocks_cfg = num_blocks
         self.k_cache: List[torch.Tensor] = []
         self.v_cache: List[torch.Tensor] = []
@@ -120,6 +133,9 @@ class RolloutEngine:
             from chatlearn_b200.models.nn.layout import kv_head_range
             nkv_l = kv_head_range(a, tp, 0)[1]
             per_tok = nkv_l * a.head_dim * 2
+            if self.q8:
+                return ops.Q8KVCache.bytes_per_block(self.block_size, nkv_l, a.head_dim) \
+                    * sum(1 for l in range(a.num_hidden_layers) if not a.layer_is_linear(l))
         esz = torch.empty((), dtype=self.kv_dtype).element_size()
         kv_layers = sum(1 for l in range(a.num_hidden_layers) if not a.layer_is_linear(l))
         return per_tok * esz * self.block_size * kv_layers
@@ -176,6 +192,7 @@ class RolloutEngine:
                 kd, vd = nk_l * a.linear_key_head_dim, nv_l * a.linear_value_head_dim
                 self.k_cache.append(torch.empty(0, device=self.device))
                 self.v_cache.append(torch.empty(0, device=self.device))
+                self.q8_cache.append(None)
                 # slots 0..max_num_seqs are handed out; the last one is scratch for the padded rows of a captured step
                 self.lin_conv.append(torch.zeros(self.max_num_seqs + 2, a.linear_conv_kernel_dim - 1, 2 * kd + vd,
                                                  dtype=self.model.dtype, device=self.device))
@@ -184,6 +201,11 @@ class RolloutEngine:
                 continue
             self.lin_conv.append(None)
             self.lin_rec.append(None)
+            if self.q8:
+                self.q8_cache.append(ops.Q8KVCache.empty(nb + 1, self.block_size, nkv_l, dk, self.device))
+                self.k_cache.append(self.q8_cache[-1].k)
+                self.v_cache.append(self.q8_cache[-1].v)
+                continue
             self.k_cache.append(torch.zeros(nb + 1, self.block_size, nkv_l, dk, dtype=self.kv_dtype,
                                             device=self.device))
             if a.use_mla:
@@ -196,7 +218,7 @@ class RolloutEngine:
 
     def free_kv_cache(self):
         self.invalidate_graphs()
-        self.k_cache, self.v_cache = [], []
+        self.k_cache, self.v_cache, self.q8_cache = [], [], []
         self.lin_conv, self.lin_rec = [], []
         self.num_blocks = 0
 
@@ -274,7 +296,7 @@ class RolloutEngine:
         t = lambda x, dt, slot: xfer.to_device(torch.tensor(x, dtype=dt), dev, slot)  # noqa: E731
         kv = KVCtx(self.k_cache, self.v_cache, t(slots, torch.long, "slots"), xfer.to_device(bt, dev, "bt"),
                    t(seq_lens, torch.int32, "seq_lens"), t(plan.q_lens, torch.int32, "q_lens"), plan.is_prefill,
-                   lin=self._linear_state(plan.seqs))
+                   q8=self.q8_cache if self.q8 else None, lin=self._linear_state(plan.seqs))
         ctx = FwdCtx(positions=t(pos, torch.long, "pos"), cu_seqlens=t(cu, torch.int32, "cu"),
                      max_seqlen=max(plan.q_lens), kv=kv, tp=self.tp, ep=self.ep, tp_symm=self._symm(), fuse_add_norm=True)
         self._embed_patch = None
@@ -329,6 +351,10 @@ class RolloutEngine:
             self._gs = dict(n=n, width=width, in64=in64, tokens=z(torch.long, n), pos=in64[1],
                             slots=in64[2], seq_lens=z(torch.int32, n), bt=z(torch.int32, n, width),
                             u=z(torch.float32, n), ids=z(torch.long, n), lp=z(torch.float32, n),
+                            # rows of (entropy, alternatives' log-probs, their ids), for sampling that asks for them
+                            top=z(torch.float32, n, 1 + 2 * MAX_LOGPROBS),
+                            top_dev=[z(torch.float32, n, 1 + 2 * MAX_LOGPROBS) for _ in range(2)],
+                            top_host=[torch.zeros(n, 1 + 2 * MAX_LOGPROBS, dtype=torch.float32, pin_memory=pin) for _ in range(2)],
                             stage=torch.zeros(6, n, dtype=torch.int64, pin_memory=pin),
                             out_dev=[z(torch.float32, 2, n) for _ in range(2)],
                             out_host=[torch.zeros(2, n, dtype=torch.float32, pin_memory=pin) for _ in range(2)],
@@ -357,7 +383,8 @@ class RolloutEngine:
 
     def _decode_body(self, B: int, sp):
         gs = self._gs
-        kv = KVCtx(self.k_cache, self.v_cache, gs["slots"][:B], gs["bt"][:B], gs["seq_lens"][:B], None, False)
+        kv = KVCtx(self.k_cache, self.v_cache, gs["slots"][:B], gs["bt"][:B], gs["seq_lens"][:B], None, False,
+                   q8=self.q8_cache if self.q8 else None)
         if gs.get("use_groups"):
             kv.groups = (gs["grp_q"][:max(B // 2, 1)], gs["grp_nblk"][:max(B // 2, 1)], gs["blk_start"][:B])
         if self.arch.layer_types is not None:
@@ -369,6 +396,15 @@ class RolloutEngine:
         ids, lp = ops.sample(logits, gs["u"][:B], sp.temperature, sp.top_k, sp.top_p, sp.min_p)
         gs["ids"][:B].copy_(ids)
         gs["lp"][:B].copy_(lp)
+        if sp.logprobs:
+            gs["top"][:B, :1 + 2 * sp.logprobs].copy_(self._alternatives(logits, ids, sp))
+
+    @staticmethod
+    def _alternatives(logits, ids, sp: SamplingParams):
+        """Entropy and likeliest tokens of the distribution the sampled tokens' log-probs refer to, a row of
+        (entropy, log-probs, ids) per token (ids are exact in fp32: vocab < 2^24)."""
+        st = ops.token_logprobs(logits, ids, sp.logprobs, sp.temperature if sp.temperature > 0 else 1.0)
+        return torch.cat([st.entropy[:, None], st.top_logprobs, st.top_ids.float()], 1)
 
     def _graph_decode(self, plan: StepPlan):
         """One decode step for every running sequence through a captured CUDA graph.
@@ -383,7 +419,8 @@ class RolloutEngine:
         scratch_block = self.num_blocks          # one block past the allocator's range
         # plain Python lists, one tensor construction: per-element tensor writes would
         # cost more host time than the whole step takes on the GPU
-        rows = [[0] * Bg, [0] * Bg, [scratch_block * bs] * Bg, [1] * Bg, [0] * Bg, [0] * Bg]
+        # padded rows: one token in the scratch block; of an 8-bit cache none at all (a page belongs to one row of a call)
+        rows = [[0] * Bg, [0] * Bg, [scratch_block * bs] * Bg, [0 if self.q8 else 1] * Bg, [0] * Bg, [0] * Bg]
         owner, blen = gs["bt_owner"], gs["bt_len"]
         for i, s in enumerate(seqs):
             p = s.num_computed                   # position of the token fed now
@@ -457,7 +494,7 @@ class RolloutEngine:
         """Which rows of the decode batch share their first KV blocks (prefix sharing gave the samples of a prompt the
         same physical blocks): the decode attention then reads those blocks once per group.  The tables only change
         when the batch does; they are rebuilt and uploaded then.  Returns whether any group exists."""
-        if self.arch.use_mla or self.arch.layer_types is not None or not seqs:
+        if self.arch.use_mla or self.arch.layer_types is not None or self.q8 or not seqs:
             return False
         rep = self.arch.num_attention_heads // max(self.arch.num_key_value_heads, 1)
         if self.arch.head_dim != 128 or self.block_size != 64 or rep > 4 or os.environ.get("CLB200_GROUPED_DECODE", "1") == "0":
@@ -540,10 +577,16 @@ class RolloutEngine:
         dev_buf[0, :B].copy_(ids)                      # token ids are exact in fp32: vocab < 2^24
         dev_buf[1, :B].copy_(lps)
         host_buf[:, :B].copy_(dev_buf[:, :B], non_blocking=True)
+        n_top = seqs[0].sampling.logprobs              # (one key for the rows of a captured step)
+        if n_top:
+            w = 1 + 2 * n_top
+            gs["top_dev"][par][:B, :w].copy_(gs["top"][:B, :w])
+            gs["top_host"][par][:B, :w].copy_(gs["top_dev"][par][:B, :w], non_blocking=True)
+            xfer.d2h_bytes += B * w * 4
         if gs["out_event"][par] is not None:
             gs["out_event"][par].record()
         xfer.d2h_bytes += 2 * B * 4
-        return {"seqs": list(seqs), "par": par}
+        return {"seqs": list(seqs), "par": par, "n_top": n_top}
 
     def _complete(self, pend, sched: Scheduler, eos_id):
         """Wait for a launched step's tokens, append them and apply the stop conditions."""
@@ -554,7 +597,8 @@ class RolloutEngine:
         both = gs["out_host"][pend["par"]][:, :B].tolist()
         for s in pend["seqs"]:
             s.inflight = 0
-        live = [(s, int(t), lp) for s, t, lp in zip(pend["seqs"], both[0], both[1]) if not s.finished]
+        tops = gs["top_host"][pend["par"]][:B, :1 + 2 * pend["n_top"]].tolist() if pend["n_top"] else [None] * B
+        live = [(s, int(t), lp, top) for s, t, lp, top in zip(pend["seqs"], both[0], both[1], tops) if not s.finished]
         self._apply_tokens(sched, live, eos_id)
 
     def drain(self, sched: Scheduler, eos_id):
@@ -581,7 +625,9 @@ class RolloutEngine:
                 for s in seqs:
                     s.num_computed += 1
                 if not self.pipelined:
-                    self._finish_step(sched, seqs, ids, lps, eos_id)
+                    n_top = seqs[0].sampling.logprobs
+                    self._finish_step(sched, seqs, ids, lps, eos_id,
+                                      xfer.tolist(self._gs["top"][:len(seqs), :1 + 2 * n_top]) if n_top else None)
                     return
                 new = self._start_readback(seqs, ids, lps)
                 if pend is not None:
@@ -626,6 +672,7 @@ class RolloutEngine:
             groups.setdefault(s.sampling.key(), []).append(j)
         ids = torch.empty(len(seqs), dtype=torch.long, device=self.device)
         lps = torch.empty(len(seqs), dtype=torch.float32, device=self.device)
+        tops = [None] * len(seqs)
         u_all = torch.rand(len(seqs), device=self.device, generator=self.gen)
         for key, js in groups.items():
             sp = seqs[js[0]].sampling
@@ -644,22 +691,30 @@ class RolloutEngine:
                                         sp.repetition_penalty, pmask)
             i_, l_ = ops.sample(z, u_all if len(js) == len(seqs) else u_all.index_select(0, jj),
                                 sp.temperature, sp.top_k, sp.top_p, sp.min_p)
+            if sp.logprobs:
+                for j, top in zip(js, xfer.tolist(self._alternatives(z, i_, sp))):
+                    tops[j] = top
             if len(js) == len(seqs):
                 ids, lps = i_, l_
             else:
                 ids[jj], lps[jj] = i_, l_
-        self._finish_step(sched, seqs, ids, lps, eos_id)
+        self._finish_step(sched, seqs, ids, lps, eos_id, tops)
 
-    def _finish_step(self, sched: Scheduler, seqs, ids, lps, eos_id):
+    def _finish_step(self, sched: Scheduler, seqs, ids, lps, eos_id, tops=None):
         """Read the sampled tokens back and apply the stop conditions."""
         # one device -> host read per step (token ids are exact in fp32: vocab < 2^24)
         both = xfer.tolist(torch.stack([ids.float(), lps.float()]))
-        self._apply_tokens(sched, [(s, int(t), lp) for s, t, lp in zip(seqs, both[0], both[1])], eos_id)
+        self._apply_tokens(sched, [(s, int(t), lp, top) for s, t, lp, top in
+                                   zip(seqs, both[0], both[1], tops if tops is not None else [None] * len(seqs))], eos_id)
 
-    def _apply_tokens(self, sched: Scheduler, triples, eos_id):
-        for s, tok, lp in triples:
+    def _apply_tokens(self, sched: Scheduler, tokens, eos_id):
+        for s, tok, lp, top in tokens:
             s.output.append(tok)
             s.logprobs.append(lp)
+            if top is not None:
+                n = (len(top) - 1) // 2
+                s.entropies.append(top[0])
+                s.top_logprobs.append([(int(i), l) for i, l in zip(top[1 + n:], top[1:1 + n])])
             sp = s.sampling
             if not sp.ignore_eos and (tok == eos_id or tok in sp.stop_token_ids):
                 sched.finish(s, "stop")
@@ -773,6 +828,8 @@ class RolloutSession:
     def submit(self, prompt: List[int], sampling: "SamplingParams", max_new_tokens: Optional[int] = None,
                mm: Optional[Dict[str, Any]] = None) -> Sequence:
         eng = self.engine
+        if not 0 <= sampling.logprobs <= min(MAX_LOGPROBS, eng.arch.vocab_size):
+            raise ValueError(f"SamplingParams.logprobs: 0 to {MAX_LOGPROBS} alternatives of {eng.arch.vocab_size}, got {sampling.logprobs}")
         mx = sampling.max_tokens if max_new_tokens is None else max_new_tokens
         mx = max(0, min(mx, eng.max_model_len - len(prompt)))
         s = Sequence(eng._req_counter, list(prompt), mx, sampling)

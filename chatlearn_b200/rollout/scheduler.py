@@ -73,6 +73,9 @@ class Sequence:
     sampling: "object" = None
     output: List[int] = field(default_factory=list)
     logprobs: List[float] = field(default_factory=list)
+    # per generated token, where its sampling asks for alternatives: the likeliest (token, log-prob) and the entropy
+    top_logprobs: List[List[tuple]] = field(default_factory=list)
+    entropies: List[float] = field(default_factory=list)
     blocks: List[int] = field(default_factory=list)
     num_computed: int = 0          # tokens whose KV is in the cache
     finished: bool = False
