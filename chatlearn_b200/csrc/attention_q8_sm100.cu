@@ -244,8 +244,11 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
         }
         uint8_t* box = to[col / 4] + at * 128;
         const int c = col % 4 * 2;
-        *reinterpret_cast<uint4*>(box + ((c ^ (at & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-        *reinterpret_cast<uint4*>(box + (((c + 1) ^ (at & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
+        // the chunks of the second 64 elements in the other order: 8 neighbours then store to 8 different chunks of a row
+        const uint4 lo = make_uint4(h[0], h[1], h[2], h[3]), hi = make_uint4(h[4], h[5], h[6], h[7]);
+        const int odd = col >> 2 & 1;
+        *reinterpret_cast<uint4*>(box + (((c + odd) ^ (at & 7)) << 4)) = odd ? hi : lo;
+        *reinterpret_cast<uint4*>(box + (((c + 1 - odd) ^ (at & 7)) << 4)) = odd ? lo : hi;
       }
     };
     bool ok = true;
