@@ -1,21 +1,27 @@
 // Attention of many new tokens per sequence over the paged 8-bit cache, on the 5th-generation tensor cores.
 //
 // Continuation chunks of a prefill attend over everything cached before them: with hundreds of new tokens per sequence
-// the two products bound the work, not the cache's bytes.  A CTA owns 128 query rows of one sequence and one kv head:
-// 128 / rep tokens times the rep query heads that share the head, so a cached tile is dequantised once for all of them.
-// Warps:
-//   0..3  softmax, thread = query row: first the row itself, rescaled by a power of two to fp16, into shared memory;
+// the two products bound the work, not the cache's bytes.  A CTA owns G groups of 128 query rows of one sequence and one
+// kv head: 128 G / rep tokens times the rep query heads that share the head, so a cached tile is dequantised once for all
+// of them.  Warps, for G = 2 (one CTA to an SM) and G = 1 (two, but for elements of 256):
+//   4 G   softmax, thread = query row: first the row itself, rescaled by a power of two to fp16, into shared memory;
 //         then per tile of 64 keys the scores out of tensor memory, running maximum (lazily applied, as soon as it has
-//         run ahead by 2^8) and sum, P as fp16 into shared memory; at the end O / l to the output
-//   4..7  dequantisation: e4m3 codes from the pages to fp16 tiles (exact) in the 128-byte swizzle, one tile ahead in
-//         registers.  Pages of a multiple of 64 tokens keep their scales out of the tiles (S and P take them).  Of other
-//         pages a tile holds several: K is brought to the largest of its scales (what that loses is 2^-34 of the tile's
-//         largest keys), V becomes bf16 values (exact) and P bf16, as fp16 has not the range for scales far apart.
-//   8     one thread issues S = Q K^T (128x64x16) into one of two S accumulators and O += P V (128xDx16, V as an
-//         MN-major operand straight from its row-major tile)
+//         run ahead by 2^8) and sum, P as fp16 back over the scores; at the end O / l to the output.  Two groups take
+//         turns at the exponentials: one's run beside the other's maxima (both at once had the special-function units
+//         wait on them first and then stand idle: 389 -> 351 us at the case below)
+//   4     dequantisation: e4m3 codes from the pages, copied to shared memory a tile ahead, to fp16 tiles (exact) in the
+//         128-byte swizzle.  Pages of a multiple of 64 tokens keep their scales out of the tiles (S and P take them).  Of
+//         other pages a tile holds several: K is brought to the largest of its scales (what that loses is 2^-34 of the
+//         tile's largest keys), V becomes bf16 values (exact) and P bf16, as fp16 has not the range for scales far apart.
+//   1     one elected thread issues, for each group, S = Q K^T (128x64x16) into one of two accumulators and O += P V
+//         (128xDx16, P from tensor memory, V as an MN-major operand straight from its row-major tile), one tile behind
 // O is kept in units of a V scale that follows the tiles' scales where they are far apart (as in the decode kernel).
 // The queries are causal inside their sequence's new tokens.  Every mbarrier wait is bounded; one that runs out records a
 // status, the CTA drains and frees its tensor memory.
+//
+// 8 sequences of 512 new tokens after 3,584, 32 / 8 heads of 128: 351 us, 740 TFLOP/s of the visible pairs (45 % of a
+// library product's rate); the tensor pipe is 40 % busy while a CTA runs.  What bounds it: a softmax thread's chain of
+// dependent instructions over its tile (2 warps to a scheduler), and 512 CTAs on 148 SMs, of whose fourth wave half is idle.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/empty.h>
@@ -34,23 +40,24 @@ using namespace sm100;
 
 namespace {
 
-constexpr int BM = 128, BN = 64, kStages = 2, kThreads = 288, kInfo = 8;
+constexpr int BM = 128, BN = 64, kStages = 2, kInfo = 8;
 constexpr uint32_t kChunk = BN * 128;             // 64 keys x 64 elements of fp16
 constexpr float kRescale = 8.f;                   // bits that the maximum may run ahead
 constexpr float kShift = 7.f;                     // P times 2^7: at most 2^15, and normal down to 2^-21 of a row's largest
 
-struct TileInfo { float ks, vs; uint32_t seen[2]; };      // scales of the tile, keys that exist
+struct TileInfo { float ks, vs, log2_vs, per_vs; uint32_t seen[2]; };      // scales of the tile, keys that exist
 
-template <int D>
+// G: groups of 128 query rows
+template <int D, int G>
 struct Smem {
-  uint8_t q[D / 64][BM * 128];
+  uint8_t q[G][D / 64][BM * 128];
   uint8_t k[kStages][D / 64][kChunk];
   uint8_t v[kStages][D / 64][kChunk];
-  uint8_t p[BM * 128];
+  uint4 raw[2][BN * D / 16];                        // the codes of the tile to come, each piece read by the thread that copied it
   TileInfo info[kInfo];
   float red[4];
   uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[2], s_empty[2], p_full, pv_done;
+  uint64_t s_full[G][2], p_full[G][2], pv_done[G], turn[2];
   uint32_t tmem_base;
   int seq, tile, row0, len, n;
 };
@@ -73,11 +80,59 @@ __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&r
         "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+  uint32_t y;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(y));
+  return y != 0;
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
+        "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// D += A B with A in tensor memory, two 16-bit elements of a row to a column
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// loads that stay where they are written: the compiler would move them down to the use of their value, and wait there
+__device__ __forceinline__ float load_here(const float* at) {
+  float x;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(x) : "l"(at));
+  return x;
+}
+__device__ __forceinline__ int load_here(const int* at) {
+  int x;
+  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(x) : "l"(at));
+  return x;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\nfma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
@@ -89,15 +144,16 @@ __device__ __forceinline__ uint32_t half2_mul(uint32_t a, __half2 b) {
 }
 
 // SMALL: pages that are no multiple of 64 tokens
-template <int D, bool SMALL>
-__global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(const ChunkArgs a) {
+template <int D, bool SMALL, int G>
+__global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chunk_q8_kernel(const ChunkArgs a) {
   extern __shared__ uint8_t smem_raw[];
-  Smem<D>* sm = reinterpret_cast<Smem<D>*>(smem_raw);
-  constexpr int kTmemCols = D == 256 ? 512 : 256, kOCol = 2 * BN;
+  Smem<D, G>* sm = reinterpret_cast<Smem<D, G>*>(smem_raw);
+  constexpr int kOCol = 2 * BN, kGroupCols = kOCol + D, kTmemCols = G * kGroupCols > 256 ? 512 : 256;
+  static_assert(G * kGroupCols <= 512, "tensor memory has 512 columns");
   pdl_wait();
   pdl_trigger();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y;
-  const int rep = a.nq / a.nkv, tokens = BM / rep;         // tokens of a tile
+  const int rep = a.nq / a.nkv, tokens = G * BM / rep;     // tokens of a tile
 
   // ---- which (sequence, tile) is this CTA's; a sequence's tiles are listed last-first: those with the most keys begin first
   if (warp == 0) {
@@ -147,17 +203,19 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
   const int nblk = (keys + BN - 1) / BN;
 
   if (threadIdx.x == 0) {
-    mbar_init(&sm->q_full, 128);
+    for (int g = 0; g < 2; ++g) mbar_init(&sm->turn[g], 4);
+    mbar_init(&sm->q_full, 128 * G);
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sm->k_full[s], 128); mbar_init(&sm->k_empty[s], 1);
       mbar_init(&sm->v_full[s], 128); mbar_init(&sm->v_empty[s], 1);
     }
-    for (int b = 0; b < 2; ++b) { mbar_init(&sm->s_full[b], 1); mbar_init(&sm->s_empty[b], 4); }
-    mbar_init(&sm->p_full, 128);
-    mbar_init(&sm->pv_done, 1);
+    for (int g = 0; g < G; ++g) {
+      for (int b = 0; b < 2; ++b) { mbar_init(&sm->s_full[g][b], 1); mbar_init(&sm->p_full[g][b], 128); }
+      mbar_init(&sm->pv_done[g], 1);
+    }
     fence_barrier_init();
   }
-  if (warp == 8) {
+  if (warp == 4 * G + 4) {
     tmem_alloc(&sm->tmem_base, kTmemCols);
     tmem_relinquish();
   }
@@ -166,14 +224,13 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
   tc_fence_after_sync();
   const uint32_t tmem_base = sm->tmem_base;
 
-  if (warp >= 4 && warp < 8) {
+  if (warp >= 4 * G && warp < 4 * G + 4) {
     // ------------------------------------------------ dequantisation
     // thread: element chunk `col` (16 codes) of rows tid / CH + i * ROWS
     constexpr int CH = D / 16, ROWS = 128 / CH, N = BN / ROWS;
-    const int tid = threadIdx.x - 128, col = tid % CH, row = tid / CH;
+    const int tid = threadIdx.x - 128 * G, col = tid % CH, row = tid / CH;
     const int* table = a.tables + (int64_t)seq * a.width;
     const int64_t page_bytes = (int64_t)a.bs * D;
-    struct Raw { uint4 x[N]; };
     constexpr int P = SMALL ? N : 1;                // pages of a thread's rows
     struct Ids { int page[P], id[P]; };             // their places in the table and what stands there, loaded two tiles ahead
     auto ids_of = [&](int j) {
@@ -182,7 +239,8 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
       for (int i = 0; i < P; ++i) {
         const int tok = j * BN + (SMALL ? row + i * ROWS : 0);
         x.page[i] = tok / a.bs;
-        x.id[i] = tok < keys ? table[x.page[i]] : -1;
+        x.id[i] = -1;
+        if (tok < keys) x.id[i] = load_here(table + x.page[i]);
       }
       return x;
     };
@@ -197,8 +255,11 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
         const bool ok = (uint32_t)x.id[i] < (uint32_t)a.pages;
         const int ph = ok ? x.id[i] * a.nkv + kvh : 0;
         w.at[i] = ph * page_bytes + (int64_t)(tok - x.page[i] * a.bs) * D + col * 16;
-        w.ks[i] = ok ? a.ks[ph] : 0.f;
-        w.vs[i] = ok ? a.vs[ph] : 0.f;
+        w.ks[i] = w.vs[i] = 0.f;
+        if (ok) {
+          w.ks[i] = load_here(a.ks + ph);
+          w.vs[i] = load_here(a.vs + ph);
+        }
         if constexpr (SMALL) {
           w.ok |= (ok ? 1u : 0u) << i;
         } else if (ok) {
@@ -208,26 +269,30 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
       }
       return w;
     };
-    auto fetch = [&](const uint8_t* from, const Where& w) {
-      Raw r;
+    // the thread's pieces of a tile on their way to shared memory: registers would have to be waited for at the end of the
+    // iteration, where they change names
+    auto fetch = [&](uint4* raw, const uint8_t* from, const Where& w) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        r.x[i] = make_uint4(0, 0, 0, 0);
-        if (w.ok >> i & 1) r.x[i] = __ldg(reinterpret_cast<const uint4*>(from + (SMALL ? w.at[SMALL ? i : 0] : w.at[0] + (row + i * ROWS) * D)));
+        const uint8_t* at = from + (SMALL ? w.at[SMALL ? i : 0] : w.at[0] + (row + i * ROWS) * D);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(raw + i * 128 + tid)), "l"(at), "r"((w.ok >> i & 1) * 16) : "memory");
       }
-      return r;
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
     auto all = [&](bool x) {                        // whether it holds for all 128 threads
       uint32_t y;
       asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.and.pred q, 1, 128, p;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(y) : "r"((uint32_t)x) : "memory");
       return y != 0;
     };
-    auto put = [&](uint8_t (*to)[kChunk], const Raw& r, const float* scale, float ref, auto values) {
+    auto put = [&](uint8_t (*to)[kChunk], const uint4* raw, const float* scale, float ref, auto values) {
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const int at = row + i * ROWS;
         uint32_t h[8];
-        const uint32_t w[4] = {r.x[i].x, r.x[i].y, r.x[i].z, r.x[i].w};
+        uint4 x = raw[i * 128 + tid];
+        if (!SMALL && decltype(values)::value && !(ref > 0.f)) x = make_uint4(0, 0, 0, 0);     // an empty scale: zeros, whatever the codes are
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) e4m3x4_to_half2(w[e], h[2 * e], h[2 * e + 1]);
         if constexpr (SMALL && decltype(values)::value) {            // V: bf16 values
@@ -254,12 +319,11 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
     bool ok = true;
     Where w = {};
     Ids ids = {};
-    Raw rk = {}, rv = {};
     if (nblk > 0) {
       w = where(0, ids_of(0));
       ids = ids_of(1);
-      rk = fetch(a.kc, w);
-      rv = fetch(a.vc, w);
+      fetch(sm->raw[0], a.kc, w);
+      fetch(sm->raw[1], a.vc, w);
     }
     for (int j = 0; j < nblk; ++j) {
       const uint32_t stage = j % kStages, phase = (j / kStages) & 1;
@@ -271,42 +335,49 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
 #pragma unroll
         for (int i = 1; i < N; ++i) ref_k = fmaxf(ref_k, w.ks[i]);
         ref_k = warp_max(ref_k);
-        if (lane == 0) sm->red[warp - 4] = ref_k;
+        if (lane == 0) sm->red[warp - 4 * G] = ref_k;
         asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
         ref_k = fmaxf(fmaxf(sm->red[0], sm->red[1]), fmaxf(sm->red[2], sm->red[3]));
       }
       ok = mbar_wait(&sm->k_empty[stage], phase ^ 1) && ok;
       TileInfo& info = sm->info[j % kInfo];
-      if (tid < 2) info.seen[tid] = 0u;
-      if (tid == 0) { info.ks = ref_k; info.vs = ref_v; }
-      ok = all(ok);                                // the waits of all ran out, or of none: everybody leaves together
-      if (!ok) break;
-      if (col == 0) {                              // keys that exist: a bit for each row
-        uint32_t bits[2] = {0u, 0u};
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (w.ok >> i & 1) bits[(row + i * ROWS) >> 5] |= 1u << ((row + i * ROWS) & 31);
-        atomicOr(&info.seen[0], bits[0]);
-        atomicOr(&info.seen[1], bits[1]);
+      if (tid < 2) info.seen[tid] = SMALL || (w.ok & 1u) ? 0xffffffffu : 0u;
+      if (tid == 0) {
+        info.ks = ref_k;
+        info.vs = ref_v;
+        info.log2_vs = log2f(ref_v);
+        info.per_vs = 1.f / ref_v;
       }
-      put(sm->k[stage], rk, w.ks, ref_k, std::false_type{});
+      if constexpr (SMALL) {
+        ok = all(ok);                              // the waits of all ran out, or of none: everybody leaves together
+        if (!ok) break;
+        if (col == 0 && w.ok != (1u << N) - 1u) {  // keys without a page
+          uint32_t bits[2] = {0xffffffffu, 0xffffffffu};
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (!(w.ok >> i & 1)) bits[(row + i * ROWS) >> 5] &= ~(1u << ((row + i * ROWS) & 31));
+          atomicAnd(&info.seen[0], bits[0]);
+          atomicAnd(&info.seen[1], bits[1]);
+        }
+      } else if (!ok) {
+        break;
+      }
+      put(sm->k[stage], sm->raw[0], w.ks, ref_k, std::false_type{});
       fence_proxy_async();
       mbar_arrive(&sm->k_full[stage]);
-      rk = fetch(a.kc, next);
+      fetch(sm->raw[0], a.kc, next);
       ok = mbar_wait(&sm->v_empty[stage], phase ^ 1);
-      if (!SMALL && !(ref_v > 0.f)) rv = Raw{};    // an empty scale: zeros, whatever the codes are
-      put(sm->v[stage], rv, w.vs, ref_v, std::true_type{});
+      put(sm->v[stage], sm->raw[1], w.vs, ref_v, std::true_type{});
       fence_proxy_async();
       mbar_arrive(&sm->v_full[stage]);
-      rv = fetch(a.vc, next);
+      fetch(sm->raw[1], a.vc, next);
       w = next;
     }
     if (!ok) atomicCAS(&g_q8_status, ST_OK, ST_CONVERT);
-  } else if (warp == 8) {
+  } else if (warp == 4 * G + 4) {
     // ------------------------------------------------ MMA issuer
-    if (lane == 0 && nblk > 0) {
+    if (nblk > 0 && elect_one()) {
       constexpr uint32_t idesc_qk = idesc_of(BM, BN, 0, 0), idesc_pv = idesc_of(BM, D, 1, SMALL);
-      const uint32_t o_tmem = tmem_base + kOCol;
       bool ok = mbar_wait(&sm->q_full, 0);
       tc_fence_after_sync();
       // O += P(i) V(i) is issued one tile behind the scores: the tensor core has the next S = Q K^T to run while the
@@ -314,30 +385,35 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
       auto issue_pv = [&](int i) -> bool {
         const uint32_t st = i % kStages, ph = (i / kStages) & 1;
         if (!mbar_wait(&sm->v_full[st], ph)) return false;
-        if (!mbar_wait(&sm->p_full, i & 1)) return false;
-        tc_fence_after_sync();
-        const uint64_t dp = make_kmajor_sw128_desc(smem_u32(sm->p));
         const uint64_t dv = make_mnmajor_sw128_desc(smem_u32(sm->v[st][0]), kChunk);
+        for (int g = 0; g < G; ++g) {
+          if (!mbar_wait(&sm->p_full[g][i & 1], (i >> 1) & 1)) return false;
+          tc_fence_after_sync();
+          const uint32_t base = tmem_base + g * kGroupCols, p_tmem = base + (i & 1) * BN;
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk)
-          umma_bf16(o_tmem, dp + 2ull * kk, dv + 128ull * kk, idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < BN / 16; ++kk)
+            umma_ts(base + kOCol, p_tmem + 8 * kk, dv + 128ull * kk, idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+          umma_commit(&sm->pv_done[g]);
+        }
         umma_commit(&sm->v_empty[st]);
-        umma_commit(&sm->pv_done);
         return true;
       };
       for (int j = 0; j < nblk && ok; ++j) {
         const uint32_t st = j % kStages, ph = (j / kStages) & 1, b = j & 1;
         if (!mbar_wait(&sm->k_full[st], ph)) { ok = false; break; }
-        if (!mbar_wait(&sm->s_empty[b], ((j >> 1) & 1) ^ 1)) { ok = false; break; }
-        tc_fence_after_sync();
+        for (int g = 0; g < G && ok; ++g) {
+          if (j > 1 && !mbar_wait(&sm->pv_done[g], j & 1)) { ok = false; break; }      // P(j - 2) lies where S(j) goes
+          tc_fence_after_sync();
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t dq = make_kmajor_sw128_desc(smem_u32(sm->q[kk >> 2])) + 2ull * (kk & 3);
-          const uint64_t dk = make_kmajor_sw128_desc(smem_u32(sm->k[st][kk >> 2])) + 2ull * (kk & 3);
-          umma_bf16(tmem_base + b * BN, dq, dk, idesc_qk, kk > 0 ? 1u : 0u);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t dq = make_kmajor_sw128_desc(smem_u32(sm->q[g][kk >> 2])) + 2ull * (kk & 3);
+            const uint64_t dk = make_kmajor_sw128_desc(smem_u32(sm->k[st][kk >> 2])) + 2ull * (kk & 3);
+            umma_bf16(tmem_base + g * kGroupCols + b * BN, dq, dk, idesc_qk, kk > 0 ? 1u : 0u);
+          }
+          umma_commit(&sm->s_full[g][b]);
         }
+        if (!ok) break;
         umma_commit(&sm->k_empty[st]);
-        umma_commit(&sm->s_full[b]);
         if (j > 0 && !issue_pv(j - 1)) { ok = false; break; }
       }
       if (ok) ok = issue_pv(nblk - 1);
@@ -345,9 +421,9 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
     }
   } else {
     // ------------------------------------------------ softmax and epilogue: thread = query row
-    const int row = warp * 32 + lane, tok = row / rep, hr = row - tok * rep;
+    const int g = warp >> 2, row = (warp & 3) * 32 + lane, tok = threadIdx.x / rep, hr = threadIdx.x - tok * rep;
     const bool real = tok < tokens && t0 + tok < n && row0 + t0 + tok < a.T;
-    const int last = real ? first_pos + tok : -1;          // last visible key
+    const int last = real ? min(first_pos + tok, keys - 1) : -1;     // last visible key
     // the row as fp16, its largest in [2^10, 2^11); the sign of the softmax scale goes with it
     const __nv_bfloat16* q = static_cast<const __nv_bfloat16*>(a.q) + (real ? (row0 + t0 + tok) * a.q_row + (int64_t)(kvh * rep + hr) * D : 0);
     float big = 0.f;
@@ -370,17 +446,17 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
       uint32_t h[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) h[e] = half2_bits(to_float(x[2 * e]) * up, to_float(x[2 * e + 1]) * up);
-      *reinterpret_cast<uint4*>(sm->q[c >> 3] + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+      *reinterpret_cast<uint4*>(sm->q[g][c >> 3] + row * 128 + (((c & 7) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
     fence_proxy_async();
     mbar_arrive(&sm->q_full);
 
-    const uint32_t lane_addr = tmem_base + ((uint32_t)(warp * 32) << 16);
-    float m = -INFINITY, l = 0.f, unit = 0.f, per_unit = 0.f;
+    const uint32_t lane_addr = tmem_base + g * kGroupCols + ((uint32_t)((warp & 3) * 32) << 16);
+    float m = -INFINITY, l = 0.f, unit = 0.f, per_unit = 0.f, log2_unit = 0.f;
     bool ok = true;
     for (int j = 0; j < nblk; ++j) {
       const uint32_t b = j & 1;
-      if (!mbar_wait(&sm->s_full[b], (j >> 1) & 1)) { ok = false; break; }
+      if (!mbar_wait(&sm->s_full[g][b], (j >> 1) & 1)) { ok = false; break; }
       tc_fence_after_sync();
       const TileInfo info = sm->info[j % kInfo];
       const int k0 = j * BN;
@@ -392,8 +468,8 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
         see[0] = (room >= 31 ? 0xffffffffu : room < 0 ? 0u : (2u << room) - 1u) & info.seen[0];
         see[1] = (room >= 63 ? 0xffffffffu : room < 32 ? 0u : (2u << (room - 32)) - 1u) & info.seen[1];
       }
-      // the scores are read twice, 32 at a time, once for the maximum and once for P: 64 of them in registers all the
-      // while were too many beside the addresses (a spill of 30 loads a tile)
+      // 32 scores at a time.  With one group they are read twice, for the maximum and for P: two CTAs leave a thread 96
+      // registers, too few for 64 scores beside the addresses (a spill of 30 loads a tile)
       auto scores = [&](int half, uint32_t (&s)[32]) {
         tmem_ld_32x32(lane_addr + b * BN + 32 * half, s);
         tmem_ld_wait();
@@ -403,33 +479,51 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
             if (!(see[half] >> i & 1)) s[i] = 0xff800000u;
         }
       };
+      uint32_t kept[2][G == 2 ? 32 : 1];
       float mx = -INFINITY;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint32_t s[32];
         scores(half, s);
+        if constexpr (G == 2) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[i]));
+          for (int i = 0; i < 32; ++i) kept[half][i] = s[i];
+        }
+        float top[4] = {mx, -INFINITY, -INFINITY, -INFINITY};      // four chains: one is bound by its instructions' latency
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) top[i >> 1 & 3] = max3(top[i >> 1 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
       }
       const float f = fmaxf(sc * info.ks, 1e-37f);          // above 0: masked scores stay -inf at a softmax scale of 0 too
       mx *= f;
-      // P(j-1) must have been consumed before the tile is overwritten, and O must be at rest before it is rescaled
-      if (j > 0 && !mbar_wait(&sm->pv_done, (j - 1) & 1)) { ok = false; break; }
-      float change = 1.f, ratio = info.vs > 0.f ? info.vs * per_unit : 1.f;
-      if (!(ratio <= 1.f && ratio >= 0.0625f)) {
-        change = unit / info.vs;
-        unit = info.vs;
-        per_unit = 1.f / unit;
-        ratio = 1.f;
+      // units of the tile's P V: O's own, where the scales are near enough
+      float change = 1.f, shift = 0.f, back = 1.f;
+      if (info.vs > 0.f) {
+        const float ratio = info.vs * per_unit;
+        if (ratio <= 1.f && ratio >= 0.0625f) {
+          shift = info.log2_vs - log2_unit;
+          back = unit * info.per_vs;
+        } else {
+          change = unit * info.per_vs;
+          unit = info.vs;
+          per_unit = info.per_vs;
+          log2_unit = info.log2_vs;
+        }
       }
-      const bool need = mx > m + kRescale || (m == -INFINITY && mx > m);
-      const float alpha = need ? exp2_approx(m - mx) : 1.f;
-      if (need) { m = mx; l *= alpha; }
-      if (j > 0 && (change != 1.f || __any_sync(0xffffffffu, need))) {
-        tc_fence_after_sync();
+      const bool need = mx > m + kRescale;                  // the first visible key's too
+      const bool rescale = change != 1.f || __any_sync(0xffffffffu, need);
+      // O must be at rest before it is rescaled.  The barrier is in the phase of P(j - 1) V(j - 1) or behind it: S(j) was
+      // issued after P(j - 2) V(j - 2) was done, and P(j) is not given yet.  The last tile waits too, so that the wait after
+      // the loop finds it one phase on.
+      if (j > 0 && (rescale || j == nblk - 1) && !mbar_wait(&sm->pv_done[g], (j - 1) & 1)) { ok = false; break; }
+      if (rescale) {
+        const float alpha = need ? exp2_approx(m - mx) : 1.f;
+        if (need) m = mx;
+        l *= alpha;
         const float by = alpha * change;
+        tc_fence_after_sync();
 #pragma unroll 1
-        for (int cc = 0; cc < D; cc += 32) {
+        for (int cc = 0; cc < (j > 0 ? D : 0); cc += 32) {
           uint32_t o[32];
           tmem_ld_32x32(lane_addr + kOCol + cc, o);
           tmem_ld_wait();
@@ -439,50 +533,50 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
         }
         tmem_st_wait();
       }
-      float off = m == -INFINITY ? 0.f : kShift - m;
-      if (ratio != 1.f) off += log2f(ratio);
-      float sum = 0.f;
-      uint8_t* prow = sm->p + row * 128;
+      const float off = m == -INFINITY ? 0.f : kShift - m + shift;
+      if (G == 2 && (g == 1 || j > 0) && !mbar_wait(&sm->turn[g], (j + g - 1) & 1)) { ok = false; break; }
+      float2 sum2[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        uint32_t s[32];
-        scores(half, s);
-        if (half == 1) {
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm->s_empty[b]);      // the scores are in registers: the buffer may be overwritten
+        uint32_t s[32], w[16];
+        if constexpr (G == 2) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) s[i] = kept[half][i];
+        } else {
+          scores(half, s);
         }
 #pragma unroll
-        for (int ch = 0; ch < 4; ++ch) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p0 = exp2_approx(fmaf(__uint_as_float(s[ch * 8 + 2 * i]), f, off));
-            const float p1 = exp2_approx(fmaf(__uint_as_float(s[ch * 8 + 2 * i + 1]), f, off));
-            sum += p0 + p1;
-            if constexpr (SMALL) {
-              const __nv_bfloat162 x = __floats2bfloat162_rn(p0, p1);
-              w[i] = *reinterpret_cast<const uint32_t*>(&x);
-            } else {
-              w[i] = half2_bits(p0, p1);
-            }
+        for (int i = 0; i < 16; ++i) {
+          const float2 y = fma2({__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, {f, f}, {off, off});
+          const float p0 = exp2_approx(y.x), p1 = exp2_approx(y.y);
+          sum2[i & 1] = add2(sum2[i & 1], {p0, p1});
+          if constexpr (SMALL) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(p0, p1);
+            w[i] = *reinterpret_cast<const uint32_t*>(&x);
+          } else {
+            w[i] = half2_bits(p0, p1);
           }
-          *reinterpret_cast<uint4*>(prow + (((half * 4 + ch) ^ (row & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+        tmem_st_32x16(lane_addr + b * BN + 16 * half, w);      // over scores that are in registers already
       }
-      l += ratio == 1.f ? sum : sum / ratio;
-      fence_proxy_async();          // written through the generic proxy, read through the async one
+      if (G == 2) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm->turn[g ^ 1]);
+      }
+      const float sum = sum2[0].x + sum2[0].y + (sum2[1].x + sum2[1].y);
+      l = fmaf(sum, back, l);
+      tmem_st_wait();
       tc_fence_before_sync();
-      mbar_arrive(&sm->p_full);
+      mbar_arrive(&sm->p_full[g][b]);
     }
-    if (ok && nblk > 0 && !mbar_wait(&sm->pv_done, (nblk - 1) & 1)) ok = false;
+    if (ok && nblk > 0 && !mbar_wait(&sm->pv_done[g], (nblk - 1) & 1)) ok = false;
     if (ok) {
       tc_fence_after_sync();
       const float inv = l == 0.f ? 0.f : unit / l;
       // through the Q tile (no product reads it any more): 16-byte chunk c of row r at chunk c ^ (r % CH), free of bank
       // conflicts row by row and in row segments
       constexpr int CH = D / 8;
-      uint8_t* stage = sm->q[0];
+      uint8_t* stage = sm->q[g][0];
 #pragma unroll 1
       for (int cc = 0; cc < D; cc += 32) {
         uint32_t o[32];
@@ -491,21 +585,21 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
           tmem_ld_wait();
         }
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
+        for (int x = 0; x < 4; ++x) {
           __nv_bfloat16 w[8];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) w[i] = from_float<__nv_bfloat16>(inv == 0.f ? 0.f : __uint_as_float(o[g * 8 + i]) * inv);
-          *reinterpret_cast<uint4*>(stage + row * D * 2 + (((cc / 8 + g) ^ (row & (CH - 1))) << 4)) = *reinterpret_cast<const uint4*>(w);
+          for (int i = 0; i < 8; ++i) w[i] = from_float<__nv_bfloat16>(inv == 0.f ? 0.f : __uint_as_float(o[x * 8 + i]) * inv);
+          *reinterpret_cast<uint4*>(stage + row * D * 2 + (((cc / 8 + x) ^ (row & (CH - 1))) << 4)) = *reinterpret_cast<const uint4*>(w);
         }
       }
       __syncwarp();
       constexpr int RW = 256 / D;                           // rows that the warp writes at a time (D = 256: one)
 #pragma unroll 1
       for (int i = 0; i < 32 / RW; ++i) {
-        const int r = warp * 32 + i * RW + lane / CH, chunk = lane % CH, tk = r / rep;
+        const int r = (warp & 3) * 32 + i * RW + lane / CH, chunk = lane % CH, all = g * BM + r, tk = all / rep;
         if (tk < tokens && t0 + tk < n && row0 + t0 + tk < a.T) {
           const uint4 val = *reinterpret_cast<const uint4*>(stage + r * D * 2 + ((chunk ^ (r & (CH - 1))) << 4));
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + ((int64_t)(row0 + t0 + tk) * a.nq + kvh * rep + (r - tk * rep)) * D + chunk * 8) = val;
+          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + ((int64_t)(row0 + t0 + tk) * a.nq + kvh * rep + (all - tk * rep)) * D + chunk * 8) = val;
         }
       }
     }
@@ -513,25 +607,30 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) chunk_q8_kernel(co
   }
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 4 * G + 4) {
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, kTmemCols);
   }
 }
 
-template <int D, bool SMALL>
+template <int D, bool SMALL, int G>
 void launch(const ChunkArgs& a, int dev, cudaStream_t st) {
   static std::atomic<bool> ready[64] = {};
   if (!ready[dev].load()) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(chunk_q8_kernel<D, SMALL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D>)));
-    C10_CUDA_CHECK(cudaFuncSetAttribute(chunk_q8_kernel<D, SMALL>, cudaFuncAttributePreferredSharedMemoryCarveout,
+    C10_CUDA_CHECK(cudaFuncSetAttribute(chunk_q8_kernel<D, SMALL, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<D, G>)));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(chunk_q8_kernel<D, SMALL, G>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                         (int)cudaSharedmemCarveoutMaxShared));
     ready[dev].store(true);
   }
-  const int tokens = BM / (a.nq / a.nkv);
+  const int tokens = G * BM / (a.nq / a.nkv);
   const int64_t tiles = std::min<int64_t>(a.T / tokens + a.B, a.T / std::max(a.min_new, 1) + a.T / tokens);
   if (tiles > 0)
-    C10_CUDA_CHECK(launch_pdl(chunk_q8_kernel<D, SMALL>, dim3((unsigned)tiles, a.nkv), dim3(kThreads), sizeof(Smem<D>), st, a));
+    C10_CUDA_CHECK(launch_pdl(chunk_q8_kernel<D, SMALL, G>, dim3((unsigned)tiles, a.nkv), dim3(128 * G + 160), sizeof(Smem<D, G>), st, a));
+}
+
+template <int D, bool SMALL>
+void launch_rows(const ChunkArgs& a, bool wide, int dev, cudaStream_t st) {
+  wide ? launch<D, SMALL, 2>(a, dev, st) : launch<D, SMALL, 1>(a, dev, st);
 }
 
 }  // namespace
@@ -541,9 +640,13 @@ bool q8::chunk_supported(int rep) { return rep <= BM; }
 void q8::launch_chunk(const ChunkArgs& a, int D, int dev, cudaStream_t st) {
   TORCH_CHECK(dev >= 0 && dev < 64, "paged_attention_q8: device index out of range");
   const bool small = a.bs % BN != 0;
-  if (D == 64) small ? launch<64, true>(a, dev, st) : launch<64, false>(a, dev, st);
-  else if (D == 128) small ? launch<128, true>(a, dev, st) : launch<128, false>(a, dev, st);
-  else small ? launch<256, true>(a, dev, st) : launch<256, false>(a, dev, st);
+  // two groups of rows where the sequences have more than one on average.  A CTA of two takes 1.5 times as long as the two
+  // of one that an SM holds: 32 sequences of 32 / 48 / 64 / 128 new tokens (4 heads to a kv head: 128 to 512 rows) after
+  // 4,000 take 120 / 225 / 220 / 411 us with one group, 185 / 182 / 187 / 355 us with two; 320 rows 323 and 355 us
+  const bool wide = (int64_t)a.T * (a.nq / a.nkv) * 4 >= (int64_t)a.B * 5 * BM;
+  if (D == 64) small ? launch_rows<64, true>(a, wide, dev, st) : launch_rows<64, false>(a, wide, dev, st);
+  else if (D == 128) small ? launch_rows<128, true>(a, wide, dev, st) : launch_rows<128, false>(a, wide, dev, st);
+  else small ? launch<256, true, 1>(a, dev, st) : launch<256, false, 1>(a, dev, st);
 }
 
 int64_t paged_attention_q8_last_status() {
