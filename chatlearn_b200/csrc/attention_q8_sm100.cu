@@ -573,17 +573,16 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
     if (ok) {
       tc_fence_after_sync();
       const float inv = l == 0.f ? 0.f : unit / l;
-      // through the Q tile (no product reads it any more): 16-byte chunk c of row r at chunk c ^ (r % CH), free of bank
+      // through the Q tile (no product reads it any more; without keys, when other warps may still be writing it, there is
+      // nothing to stage): 16-byte chunk c of row r at chunk c ^ (r % CH), free of bank
       // conflicts row by row and in row segments
       constexpr int CH = D / 8;
       uint8_t* stage = sm->q[g][0];
 #pragma unroll 1
-      for (int cc = 0; cc < D; cc += 32) {
+      for (int cc = 0; cc < (nblk > 0 ? D : 0); cc += 32) {
         uint32_t o[32];
-        if (nblk > 0) {
-          tmem_ld_32x32(lane_addr + kOCol + cc, o);
-          tmem_ld_wait();
-        }
+        tmem_ld_32x32(lane_addr + kOCol + cc, o);
+        tmem_ld_wait();
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           __nv_bfloat16 w[8];
@@ -598,7 +597,8 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       for (int i = 0; i < 32 / RW; ++i) {
         const int r = (warp & 3) * 32 + i * RW + lane / CH, chunk = lane % CH, all = g * BM + r, tk = all / rep;
         if (tk < tokens && t0 + tk < n && row0 + t0 + tk < a.T) {
-          const uint4 val = *reinterpret_cast<const uint4*>(stage + r * D * 2 + ((chunk ^ (r & (CH - 1))) << 4));
+          uint4 val = make_uint4(0, 0, 0, 0);
+          if (nblk > 0) val = *reinterpret_cast<const uint4*>(stage + r * D * 2 + ((chunk ^ (r & (CH - 1))) << 4));
           *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(a.out) + ((int64_t)(row0 + t0 + tk) * a.nq + kvh * rep + (all - tk * rep)) * D + chunk * 8) = val;
         }
       }

@@ -172,6 +172,37 @@ def test_attend_chunks_short_tables_and_rows():
     assert ((got - want).abs() <= oracle.attend_bound(want, around, size, 200, 64, torch.bfloat16, 2.0 ** -8)).all()
 
 
+@pytest.mark.parametrize("nq,nkv,D,bs", [(32, 8, 128, 64), (8, 8, 64, 64), (16, 8, 256, 64)])
+@pytest.mark.parametrize("most", [3, 7, 40, 150])
+def test_attend_many_chunks(nq, nkv, D, bs, most):
+    """New tokens from none to `most` in each of 60 sequences: rows, tiles of one group of rows and of two side by side."""
+    g = torch.Generator().manual_seed(most)
+    news = torch.randint(0, most + 1, (60,), generator=g).tolist()
+    news[7], news[31] = most, 0
+    lens = [n + int(x) for n, x in zip(news, torch.randint(0, 190, (60,), generator=g))]
+    _check_attend(torch.bfloat16, lens, news, nq, nkv, D, bs)
+    from chatlearn_b200.ops import native
+    assert native.C.paged_attention_q8_last_status() == 0
+
+
+@pytest.mark.parametrize("bs", [16, 64])
+@pytest.mark.parametrize("D,nkv", [(128, 4), (64, 8), (256, 2)])
+def test_attend_chunks_at_their_bounds(bs, D, nkv):
+    """Tiles whose sequence is shorter than its new tokens, has no key, no page, or fewer rows than tokens."""
+    got = _check_attend(torch.bfloat16, [30, 0, 100, 300], [160, 20, 20, 130], 4 * nkv, nkv, D, bs)
+    assert not got[:130].any() and not got[160:180].any()
+    _check_attend(torch.bfloat16, [300, 140], [290, 140], 4 * nkv, nkv, D, bs, rows=270)
+    got = _check_attend(torch.bfloat16, [300, 140], [20, 140], 4 * nkv, nkv, D, bs, rows=400)
+    assert not got[160:].any()
+
+    def tweak(cache, table):
+        table[0] = -1
+        table[1, 0] = cache.k.shape[0]
+        table[1, -1] = 1 << 30
+    got = _check_attend(torch.bfloat16, [200, 333], [150, 230], 4 * nkv, nkv, D, bs, tweak=tweak)
+    assert not got[:150].any()
+
+
 def test_attend_rows_behind_the_last_sequence_are_zero():
     got = _check_attend(torch.bfloat16, [30, 50], None, 4, 2, 64, 16, rows=9)
     assert not got[2:].any()
