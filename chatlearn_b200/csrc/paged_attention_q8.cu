@@ -59,8 +59,13 @@ struct Args {
   float scale;                   // softmax scale times log2 e
 };
 
-// sequences with fewer new tokens go row by row; the others in tiles of 128 / rep tokens, which pay from here on
-constexpr int kChunkTokens = 8;
+// Sequences with fewer new tokens go row by row, each row reading its cache; the others in tiles of 128 / rep tokens, which
+// read it once but walk it alone, 64 keys in 1.6 us.  Many sequences fill the GPU with tiles: 32 of 2 / 3 / 4 / 7 new
+// tokens after 4,096 (32 / 8 heads of 128) take 107 / 153 / 197 / 316 us by rows, 129 us in tiles.  Where all new tokens
+// beyond one a sequence are few, the rows of one pass are cheaper than one tile's walk: 2 sequences of 7 after 2,048 take 25
+// us by rows, 54 us in tiles.
+constexpr int kChunkTokens = 3;
+constexpr int64_t kChunkWork = 60000;              // (new tokens - sequences) x kv heads x head_dim from which tiles pay
 
 template <int TILE>
 __device__ __forceinline__ int tiles_of(const Args& a, int r) {
@@ -855,7 +860,7 @@ c10::optional<at::Tensor> paged_attention_q8(const at::Tensor& q, const at::Tens
   const bool bf = q.scalar_type() == at::kBFloat16;
   if (news.has_value()) {
     // (fp16 queries keep to the rows: the tiles' outputs are bf16)
-    const bool chunks = bf && a.T >= kChunkTokens && q8::chunk_supported(a.nq / a.nkv);
+    const bool chunks = bf && (int64_t)(a.T - B) * a.nkv * D >= kChunkWork && q8::chunk_supported(a.nq / a.nkv);
     a.rows = chunks ? (int)std::min<int64_t>(a.T, (int64_t)B * (kChunkTokens - 1)) : a.T;
     row_list = at::empty({3, std::max(a.rows, 1)}, lens.options());
     int* list = row_list.data_ptr<int>();
