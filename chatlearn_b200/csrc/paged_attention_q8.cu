@@ -827,7 +827,7 @@ bool q8::cache_fits(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor
   auto ints = [&](const at::Tensor& x, int64_t dims) { return x.scalar_type() == at::kInt && x.dim() == dims && x.device() == dev && x.is_contiguous(); };
   return dev.is_cuda() && kc.dim() == 4 && codes(kc) && codes(vc) && vc.sizes() == kc.sizes() && kc.size(1) > 0 && kc.size(2) > 0 &&
          kc.size(2) % 16 == 0 && scales(ks) && scales(vs) && ints(tables, 2) && ints(lens, 1) && tables.size(0) == lens.size(0) &&
-         (!news.has_value() || (ints(*news, 1) && news->size(0) == lens.size(0))) && kc.size(0) * kc.size(1) < (int64_t)1 << 31;
+         (!news.has_value() || (ints(*news, 1) && news->size(0) == lens.size(0))) && kc.size(0) > 0 && kc.size(0) * kc.size(1) < (int64_t)1 << 31 && tables.size(1) * kc.size(2) < (int64_t)1 << 30;
 }
 
 // No tensor where the arguments are not as the kernels take them (the caller then says what is wrong, or lays them out).

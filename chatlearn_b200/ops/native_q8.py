@@ -1,7 +1,8 @@
 """The 8-bit key/value cache and the per-token statistics of logits on the sm_100a kernels.
 
 append            csrc/kv_q8.cu  (page maximum, scale growth and the rows of a page in one block)
-attention         csrc/paged_attention_q8.cu  (the tokens of all sequences cut evenly over the SMs)
+attention         csrc/paged_attention_q8.cu  (single tokens: the tokens of all sequences cut evenly over the SMs)
+                  csrc/attention_q8_sm100.cu  (many new tokens a sequence: tensor-core tiles of their rows)
 token statistics  csrc/token_logprob.cu  (log-prob, entropy and alternatives in one pass; gradient in one more)
 
 What the kernels do not take raises: there is no statement of another kind behind these ops.
@@ -64,7 +65,7 @@ def paged_attention_q8(q, cache, block_tables, seq_lens, q_lens=None, scale=None
 
 def token_logprobs(logits, tokens, top_n=0, temperature=1.0):
     run = C.token_logprob_apply if logits.requires_grad and torch.is_grad_enabled() else C.token_logprob_fwd
-    out = run(logits, tokens, top_n, 1.0 / temperature) if temperature > 0 else ()
+    out = run(logits, tokens, top_n, 1.0 / temperature) if 1e-30 <= temperature <= 1e30 else ()
     if not out:
         q8.check_token_logprobs(logits, tokens, top_n, temperature)
         if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):

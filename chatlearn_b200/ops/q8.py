@@ -12,7 +12,9 @@ On a GPU: head dims 64, 128 and 256, pages of a multiple of 16 tokens, any ratio
 kv heads; bf16 and fp16 queries, bf16, fp16 and fp32 new rows.  What the kernels do not take is
 refused.  A page id outside the cache is skipped when appending and masked when attending.  Two
 sequences of one call must not append to the same page (its contents are then undefined, no
-other page is touched).
+other page is touched).  Masked places may hold anything, NaN among it, where no query of the call's
+row of new tokens sees them; a NaN value that a later token of the same call sees may reach the
+earlier ones (zero times NaN), as in the statements.
 """
 from typing import NamedTuple
 
@@ -52,12 +54,16 @@ def _check_tables(what, cache, block_tables, seq_lens, q_lens, rows, device):
     k, v, ks, vs = cache
     if not (k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype == CODE_DTYPE):
         raise ValueError(f"{what}: the cache holds e4m3 codes [pages, kv heads, page tokens, head dim], the same for keys and values")
+    if k.shape[0] == 0:
+        raise ValueError(f"{what}: a cache without pages")
     if not (ks.shape == vs.shape == k.shape[:2] and ks.dtype == vs.dtype == torch.float32):
         raise ValueError(f"{what}: one fp32 scale per page and kv head")
     if not (k.is_contiguous() and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError(f"{what}: the cache's tensors are contiguous")
     if block_tables.dim() != 2 or seq_lens.dim() != 1 or block_tables.shape[0] != seq_lens.shape[0]:
         raise ValueError(f"{what}: block_tables [B, width] and seq_lens [B]")
+    if block_tables.shape[1] * k.shape[2] >= 2 ** 30:
+        raise ValueError(f"{what}: tables of {block_tables.shape[1]} pages of {k.shape[2]} tokens, 2^30 tokens and more")
     if q_lens is not None:
         if q_lens.shape != seq_lens.shape:
             raise ValueError(f"{what}: q_lens [B] like seq_lens")
@@ -114,5 +120,5 @@ def check_token_logprobs(logits, tokens, top_n, temperature):
         raise ValueError(f"{what}: {top_n} alternatives out of a vocabulary of {logits.shape[1]}")
     if logits.shape[1] == 0:
         raise ValueError(f"{what}: an empty vocabulary")
-    if not temperature > 0.0:
-        raise ValueError(f"{what}: the temperature is positive, got {temperature}")
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"{what}: the temperature is positive (1e-30 to 1e30), got {temperature}")

@@ -254,6 +254,17 @@ def test_engine_hands_back_alternatives():
         assert (torch.tensor([[l for _, l in t] for t in s.top_logprobs]) - want.top_logprobs).abs().max() < 1e-4
 
 
+def test_refuses_empty_caches_wide_tables_and_far_temperatures():
+    x, lens = torch.randn(1, 2, 16), _i([20])
+    with pytest.raises(ValueError, match="without pages"):
+        ops.paged_attention_q8(x, ops.Q8KVCache.empty(0, 16, 2, 16), _i([[0, 1]]), lens)
+    with pytest.raises(ValueError, match="tokens and more"):
+        ops.paged_attention_q8(x, ops.Q8KVCache.empty(1, 1024, 2, 16), _i([[0]]).expand(1, 2 ** 20), lens)
+    for t in (0.0, -1.0, 1e-31, 1e31, float("inf"), float("nan")):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.token_logprobs(torch.randn(2, 5), torch.tensor([0, 1]), 2, t)
+
+
 def test_engine_refuses():
     from chatlearn_b200.rollout import RolloutEngine, SamplingParams
     with pytest.raises(ValueError, match="latent"):

@@ -243,6 +243,49 @@ def test_attend_nan_key_reaches_only_its_rows():
     assert got[0, :2].isnan().all() and not got[0, 2:].isnan().any() and not got[1].isnan().any()
 
 
+@pytest.mark.parametrize("nq,nkv,D,bs", [(32, 8, 128, 64), (8, 4, 64, 16), (16, 4, 256, 32), (32, 4, 64, 128), (16, 4, 128, 48)])
+@pytest.mark.parametrize("news", [None, [5, 0, 130, 64, 2], [300, 9, 1, 40, 3]])
+def test_attend_never_reads_what_no_row_sees(nq, nkv, D, bs, news):
+    """NaN codes in every slot behind the lengths and in every page without tokens, NaN scales where there are no tokens."""
+    lens = [321, 9, 130, 64, 3]
+
+    def tweak(cache, table):
+        used = torch.zeros(cache.k.shape[0], bs, dtype=torch.bool)
+        for b, L in enumerate(lens):
+            for t in range(L):
+                used[int(table[b, t // bs]), t % bs] = True
+        for codes, scale in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)):
+            codes.view(torch.uint8).masked_fill_(~used[:, None, :, None].to(DEV), 0x7f)
+            scale.masked_fill_(~used.any(1)[:, None].to(DEV), float("nan"))
+    _check_attend(torch.bfloat16, lens, news, nq, nkv, D, bs, tweak=tweak, width=-(-321 // bs) + 2)
+
+
+def test_attend_two_streams_and_a_graph():
+    """Two calls at once on two streams, and a captured call beside an eager one: nothing is shared between them."""
+    cache, table = oracle.make_cache([500, 300], 4, 128, 64, device=DEV)
+    lens, news = _i32([500, 300]), _i32([200, 100])
+    q = torch.randn(300, 16, 128, device=DEV, dtype=torch.bfloat16)
+    want_rows, want = ops.paged_attention_q8(q[:2], cache, table, lens), ops.paged_attention_q8(q, cache, table, lens, news)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for s, out, n in zip(streams, got, (None, news)):
+            with torch.cuda.stream(s):
+                out.append(ops.paged_attention_q8(q[:2] if n is None else q, cache, table, lens, n))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want_rows) for x in got[0]) and all(torch.equal(x, want) for x in got[1])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a, b = ops.paged_attention_q8(q[:2], cache, table, lens), ops.paged_attention_q8(q, cache, table, lens, news)
+    for _ in range(3):
+        a.fill_(7), b.fill_(7)
+        graph.replay()
+        assert torch.equal(ops.paged_attention_q8(q, cache, table, lens, news), want)
+        torch.cuda.synchronize()
+        assert torch.equal(a, want_rows) and torch.equal(b, want)
+
+
 def test_attend_is_deterministic_and_takes_strided_queries():
     cache, table = oracle.make_cache([3000, 10, 900], 2, 128, 64, device=DEV)
     base = torch.randn(3, 3, 8, 128, device=DEV, dtype=torch.bfloat16)
