@@ -110,7 +110,8 @@ __device__ __forceinline__ void regrade(uint8_t* codes, int n, float ratio, int 
 }
 
 // One token per sequence: a warp per (sequence, kv head, K or V).  The chain length -> table -> scale of dependent
-// loads is all there is to wait for; the row itself is loaded beside it.
+// loads is all there is to wait for; the row itself is loaded beside it.  128 sequences (8 kv heads of 128): 3.0 us, 5.3
+// from the caller's side.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs a) {
   pdl_trigger();
@@ -155,6 +156,8 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
 // Any number of tokens per sequence: a block per (page that gets new rows, kv head, K or V).  The rows of a page of 64 x
 // 128 fit the block's registers (kKeep vectors of 8 a thread), so they are read once; longer pages read the rest again,
 // out of L2.  Blocks of the same rows run side by side (heads, then K and V): a row's heads lie beside each other.
+// 16 prompts of 900 to 1,152 tokens (100 MB in bf16 rows and codes): 25.6 us, 3.9 TB/s.  Bound by the chain in each block:
+// find the page, load, block maximum, store; 4,400 blocks of 256 threads are 3.7 waves of them.
 constexpr int kKeep = 4;
 
 template <typename T>

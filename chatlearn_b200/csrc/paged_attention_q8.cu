@@ -15,6 +15,12 @@
 // alone: its own cp.async ring, running maximum and sum, no barrier until its block's share is done.  A unit that lies
 // inside a warp's stretch is finished by the warp; parts of divided units meet at the end of the block, and a second
 // kernel joins what a cut between blocks divides.  The cuts go by the lengths alone, so results do not depend on timing.
+//
+// Measured, 32 / 8 heads of 128: 128 sequences of 128 to 2,600 tokens (344 MB) 71 us, 4.8 TB/s; 4 of 30 to 65 thousand (331
+// MB) 70 us; one of 750 9.7 us.  About 10 us stand still (lengths -> tables -> tiles -> parts -> join), the rest runs at 5.4
+// TB/s, which is what two blocks an SM with 96 KB each on their way read (7 TB/s take some 256 KB, more than an SM has);
+// shorter tiles, more or fewer stages or blocks did not change it.  (Of the cuts tried, more shares than resident blocks
+// cost more in parts than they even out.)
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/empty.h>
@@ -781,14 +787,25 @@ q8_rows_kernel(const int* __restrict__ lens, const int* __restrict__ news, int B
 
 template <typename T, int D>
 void launch_q8(Args a, const at::Tensor& q, cudaStream_t st) {
+  // stages of a ring: as much on its way at D = 64, where a tile has half the bytes (64 x 4096 tokens of 8 kv heads: 75 us
+  // with 3, 64 us with 5); more than 3 cost the second resident block elsewhere
   constexpr int ST = D == 64 ? 5 : 3;
   const int rep = a.nq / a.nkv;
-  a.unit_rows = rep <= 8 ? 8 : 16;
+  // More than 8 query heads to a kv head: 16 of them to a unit read the cache once, 8 twice, but faster (at head dim 256 16
+  // rows do not fit the registers).  One kv head in two of B sequences of L tokens, 16 heads each, us with 8 / 16 rows:
+  //   B x L      1 x 1024     8 x 4096     32 x 4096    64 x 4096
+  //   D = 64     14.4 / 13.8  15.8 / 17.3  26.3 / 23.3
+  //   D = 128    10.9 / 14.0  19.1 / 23.9  33.6 / 33.6  56.4 / 49.7
+  //   D = 256    15.0 / 21.3  28.3 / 39.1  56.0 / 66.7
+  // so 16 at D = 64, and at D = 128 where the tables have room for 64 MB (32 x 4096 above)
+  constexpr bool kBoth = D < 256;
+  a.unit_rows = kBoth && rep > 8 && (D == 64 || (int64_t)a.rows * a.nkv * a.width * a.bs * 2 * D >= 64 << 20) ? 16 : 8;
   const int row_tiles = (rep + a.unit_rows - 1) / a.unit_rows;
   constexpr int kMostPG = tile_tokens(D) / 16;
   const int pg = a.bs % tile_tokens(D) ? kMostPG : 1;
-  void (*kernel)(const Args) = a.unit_rows == 8 ? (pg == 1 ? paged_q8_kernel<T, D, ST, 1, 1> : paged_q8_kernel<T, D, ST, 1, kMostPG>)
-                                                : (pg == 1 ? paged_q8_kernel<T, D, ST, 2, 1> : paged_q8_kernel<T, D, ST, 2, kMostPG>);
+  void (*kernel)(const Args) = pg == 1 ? paged_q8_kernel<T, D, ST, 1, 1> : paged_q8_kernel<T, D, ST, 1, kMostPG>;
+  if constexpr (kBoth)
+    if (a.unit_rows == 16) kernel = pg == 1 ? paged_q8_kernel<T, D, ST, 2, 1> : paged_q8_kernel<T, D, ST, 2, kMostPG>;
   constexpr size_t smem = sizeof(WarpRing<D, ST>) * kWarps;
   static_assert(sizeof(WarpRing<D, ST>) >= 16 * D * sizeof(float), "a part fits the ring");
   static std::atomic<int> residents[64][4] = {};   // blocks that a device holds, per kernel
@@ -827,7 +844,8 @@ bool q8::cache_fits(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor
   auto ints = [&](const at::Tensor& x, int64_t dims) { return x.scalar_type() == at::kInt && x.dim() == dims && x.device() == dev && x.is_contiguous(); };
   return dev.is_cuda() && kc.dim() == 4 && codes(kc) && codes(vc) && vc.sizes() == kc.sizes() && kc.size(1) > 0 && kc.size(2) > 0 &&
          kc.size(2) % 16 == 0 && scales(ks) && scales(vs) && ints(tables, 2) && ints(lens, 1) && tables.size(0) == lens.size(0) &&
-         (!news.has_value() || (ints(*news, 1) && news->size(0) == lens.size(0))) && kc.size(0) > 0 && kc.size(0) * kc.size(1) < (int64_t)1 << 31 && tables.size(1) * kc.size(2) < (int64_t)1 << 30;
+         (!news.has_value() || (ints(*news, 1) && news->size(0) == lens.size(0))) && kc.size(0) > 0 &&
+         kc.size(0) * kc.size(1) < (int64_t)1 << 31 && tables.size(1) * kc.size(2) < (int64_t)1 << 30;
 }
 
 // No tensor where the arguments are not as the kernels take them (the caller then says what is wrong, or lays them out).

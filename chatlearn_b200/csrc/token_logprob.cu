@@ -13,6 +13,10 @@
 // logits no more than n have to be looked at.  Order: larger logit first, then lower index.
 //
 // A row is read by a cluster of 1 to 8 blocks, which write their sums and lists into the first block's shared memory.
+//
+// Reading the logits bounds it; exponentials (one a logit) take half of that time, the selection at the end 3 us (8
+// alternatives) that nothing hides.  128 rows of 152 k fp32 logits with 8: 20.4 us, 3.8 TB/s; 1,024 rows of bf16 with 2, and
+// the gradient: 201 us, 623 MB without the second read of the logits, 4.6 TB/s with it.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/empty.h>
@@ -548,7 +552,7 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
 
 // dz_j = 1/temperature [ g_lp d(j = token) + sum_k g_top_k d(j = top_k) - p_j (g_lp + sum_k g_top_k) - g_ent p_j (ln p_j + H) ]
 // One read of the logits, one write of the gradient; the columns of the token and the alternatives are written again
-// after the stretch that holds them.
+// after the stretch that holds them.  Bound by the two passes' bytes: 1,024 x 152 k bf16 115 us, 5.4 TB/s.
 constexpr int kGradThreads = 256, kGradVecs = 4;   // vectors of a thread, all on their way at a time
 constexpr int kGradSpan = kGradThreads * kGradVecs * 16;                    // bytes of a row that a block handles
 
@@ -631,7 +635,8 @@ token_logprob_grad_kernel(const T* __restrict__ logits, int64_t stride, const in
 // of the time (300 rows, 512 and 256 threads: 4000 fp32 logits with 20 alternatives 13.7 and 9.9 us, 32 k with 5 16.4 and
 // 15.3 us; 128 rows of 152 k bf16 logits with 8 20.0 and 26.4 us).
 constexpr int kShortRow = 160 << 10;
-// blocks that share a row: as many as the GPU holds at a time, each with some to read
+// blocks that share a row: as many as the GPU holds at a time, each with some to read (1 / 16 / 64 rows of 152 k fp32 logits
+// with 8 alternatives: 15.0 / 16.7 / 24.3 us with one block a row, 11.3 / 11.0 / 13.9 us with clusters)
 constexpr int kLeast = 32768;
 int cluster_for(int64_t rows, int64_t row_bytes, int threads) {
   const int kBlocks = kSmThreads / threads;
