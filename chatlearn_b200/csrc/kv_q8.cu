@@ -156,14 +156,15 @@ __global__ void __launch_bounds__(kThreads) append_step_kernel(const AppendArgs 
 // Any number of tokens per sequence: a block per (page that gets new rows, kv head, K or V).  The rows of a page of 64 x
 // 128 fit the block's registers (kKeep vectors of 8 a thread), so they are read once; longer pages read the rest again,
 // out of L2.  Blocks of the same rows run side by side (heads, then K and V): a row's heads lie beside each other.
-// 16 prompts of 900 to 1,152 tokens (100 MB in bf16 rows and codes): 25.6 us, 3.9 TB/s.  Bound by the chain in each block:
-// find the page, load, block maximum, store; 4,400 blocks of 256 threads are 3.7 waves of them.
-constexpr int kKeep = 4;
+// 16 prompts of 900 to 1,152 tokens (100 MB in bf16 rows and codes): 22.4 us, 4.5 TB/s.  Bound by the chain in each block:
+// find the page, load (rows and page id beside each other), block maximum, store.  So many small blocks: 128 threads, 8
+// blocks an SM 22.4 us; 64 threads, 10 blocks 23.6; 256 threads, 6 or 5 blocks 24.3 and 27.3; 512 threads, 4 blocks 33.
+constexpr int kPageThreads = 128, kKeep = 8;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) append_pages_kernel(const AppendArgs a) {
-  __shared__ int sh_found[4];
-  __shared__ float sh_max[kThreads / 32];
+__global__ void __launch_bounds__(kPageThreads, sizeof(T) == 4 ? 5 : 8) append_pages_kernel(const AppendArgs a) {
+  __shared__ int sh_found[5];
+  __shared__ float sh_max[kPageThreads / 32];
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -191,7 +192,8 @@ __global__ void __launch_bounds__(kThreads) append_pages_kernel(const AppendArgs
         sh_found[1] = lo - pg * a.bs;
         sh_found[2] = min(hi - lo, a.T - row);                 // rows that the tensors really hold
         sh_found[3] = row;
-        if (sh_found[2] > 0 && pg < a.width) sh_found[0] = a.tables[(int64_t)b * a.width + pg];
+        sh_found[4] = pg;
+        if (sh_found[2] > 0 && pg < a.width) sh_found[0] = b;
       }
       pages += __shfl_sync(0xffffffffu, ip, 31);
       rows += __shfl_sync(0xffffffffu, ir, 31);
@@ -199,31 +201,33 @@ __global__ void __launch_bounds__(kThreads) append_pages_kernel(const AppendArgs
     }
   }
   __syncthreads();
-  const int page = sh_found[0], off = sh_found[1], m = sh_found[2], row = sh_found[3];
-  if (page < 0 || page >= a.pages) return;
+  const int seq = sh_found[0], off = sh_found[1], m = sh_found[2], row = sh_found[3];
+  if (seq < 0) return;
+  const int page = a.tables[(int64_t)seq * a.width + sh_found[4]];       // on its way while the rows are
   const T* x = static_cast<const T*>(a.x[kv]) + row * a.row[kv] + h * a.head[kv];
   const bool vec = ((reinterpret_cast<uintptr_t>(x) | (uintptr_t)(a.row[kv] * sizeof(T))) & 15) == 0;
   const int shift = a.D == 64 ? 3 : a.D == 128 ? 4 : 5, total = m << shift;
-  // the thread's vectors, tid + i * kThreads; those of a row lie side by side
+  // the thread's vectors, tid + i * kPageThreads; those of a row lie side by side
   auto at = [&](int c) { return (c >> shift) * a.row[kv] + (c & ((1 << shift) - 1)) * 8; };
-  const int64_t ph = (int64_t)page * a.nkv + h;
-  const float old = off > 0 ? a.scale[kv][ph] : 0.f;
   Raw<T> kept[kKeep];
   float amax = 0.f, f[8];
 #pragma unroll
   for (int i = 0; i < kKeep; ++i)
-    if (i * kThreads + tid < total) kept[i] = load8(x + at(i * kThreads + tid), vec);
+    if (i * kPageThreads + tid < total) kept[i] = load8(x + at(i * kPageThreads + tid), vec);
+  if (page < 0 || page >= a.pages) return;
+  const int64_t ph = (int64_t)page * a.nkv + h;
+  const float old = off > 0 ? a.scale[kv][ph] : 0.f;
   auto largest = [&](auto of) {                    // over the block, by `of` each vector
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < kKeep; ++i)
-      if (i * kThreads + tid < total) m = fmaxf(m, of(kept[i]));
-    for (int c = kKeep * kThreads + tid; c < total; c += kThreads) m = fmaxf(m, of(load8(x + at(c), vec)));
+      if (i * kPageThreads + tid < total) m = fmaxf(m, of(kept[i]));
+    for (int c = kKeep * kPageThreads + tid; c < total; c += kPageThreads) m = fmaxf(m, of(load8(x + at(c), vec)));
     m = warp_max(m);
     if (lane == 0) sh_max[warp] = m;
     __syncthreads();                               // every thread has read the old scale, too
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) m = fmaxf(m, sh_max[w]);
+    for (int w = 0; w < kPageThreads / 32; ++w) m = fmaxf(m, sh_max[w]);
     return m;
   };
   amax = largest([](const Raw<T>& r) { return magnitude(r); });
@@ -233,16 +237,16 @@ __global__ void __launch_bounds__(kThreads) append_pages_kernel(const AppendArgs
   }
   const float s = fmaxf(scale_for(amax), old), inv = 1.f / s;
   uint8_t* codes = a.codes[kv] + ph * a.bs * a.D;
-  if (off > 0 && s > old) regrade(codes, off * a.D, old / s, tid, kThreads);
+  if (off > 0 && s > old) regrade(codes, off * a.D, old / s, tid, kPageThreads);
   if (tid == 0) a.scale[kv][ph] = s;
   uint8_t* to = codes + (int64_t)off * a.D;
 #pragma unroll
   for (int i = 0; i < kKeep; ++i)
-    if (i * kThreads + tid < total) {
+    if (i * kPageThreads + tid < total) {
       expand(kept[i], f);
-      store8(to + (i * kThreads + tid) * 8, f, inv);
+      store8(to + (i * kPageThreads + tid) * 8, f, inv);
     }
-  for (int c = kKeep * kThreads + tid; c < total; c += kThreads) {
+  for (int c = kKeep * kPageThreads + tid; c < total; c += kPageThreads) {
     expand(load8(x + at(c), vec), f);
     store8(to + c * 8, f, inv);
   }
@@ -257,7 +261,7 @@ void launch_append(const AppendArgs& a, cudaStream_t st) {
   } else {
     // a sequence with n new tokens adds to at most (n - 1) / bs + 2 pages
     const int64_t runs = std::min<int64_t>(a.T, a.T / a.bs + 2 * (int64_t)a.B);
-    C10_CUDA_CHECK(launch_pdl(append_pages_kernel<T>, dim3((unsigned)(runs * a.nkv * 2)), dim3(kThreads), 0, st, a));
+    C10_CUDA_CHECK(launch_pdl(append_pages_kernel<T>, dim3((unsigned)(runs * a.nkv * 2)), dim3(kPageThreads), 0, st, a));
   }
 }
 
