@@ -109,12 +109,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // loads that stay where they are written: the compiler would move them down to the use of their value, and wait there
 __device__ __forceinline__ float load_here(const float* at) {
   float x;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(x) : "l"(at));
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(x) : "l"(at));
   return x;
 }
 __device__ __forceinline__ int load_here(const int* at) {
   int x;
-  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(x) : "l"(at));
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(x) : "l"(at));
   return x;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -373,6 +373,7 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       fetch(sm->raw[1], a.vc, next);
       w = next;
     }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
     if (!ok) atomicCAS(&g_q8_status, ST_OK, ST_CONVERT);
   } else if (warp == 4 * G + 4) {
     // ------------------------------------------------ MMA issuer
