@@ -172,7 +172,7 @@ def test_attend_chunks_short_tables_and_rows():
     assert ((got - want).abs() <= oracle.attend_bound(want, around, size, 200, 64, torch.bfloat16, 2.0 ** -8)).all()
 
 
-@pytest.mark.parametrize("nq,nkv,D,bs", [(32, 8, 128, 64), (8, 8, 64, 64), (16, 8, 256, 64)])
+@pytest.mark.parametrize("nq,nkv,D,bs", [(32, 8, 128, 64), (8, 8, 64, 64), (16, 8, 256, 64), (200, 2, 64, 64), (128, 1, 128, 128), (130, 2, 256, 64)])
 @pytest.mark.parametrize("most", [3, 7, 40, 150])
 def test_attend_many_chunks(nq, nkv, D, bs, most):
     """New tokens from none to `most` in each of 60 sequences: rows, tiles of one group of rows and of two side by side."""
