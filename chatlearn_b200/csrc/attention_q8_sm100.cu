@@ -12,7 +12,9 @@
 //   4     dequantisation: e4m3 codes from the pages, copied to shared memory a tile ahead, to fp16 tiles (exact) in the
 //         128-byte swizzle.  Pages of a multiple of 64 tokens keep their scales out of the tiles (S and P take them).  Of
 //         other pages a tile holds several: K is brought to the largest of its scales (what that loses is 2^-34 of the
-//         tile's largest keys), V becomes bf16 values (exact) and P bf16, as fp16 has not the range for scales far apart.
+//         tile's largest keys); V too where its scales are within 2^8 (exact: its smallest code is then 2^-17), else V
+//         becomes bf16 values (exact) and P bf16 (8 bits), as fp16 has not the range for scales far apart.
+//         (Always bf16 was 248 us where this takes 273, 8 x 256 tokens on pages of 16, with eight times P's rounding.)
 //   1     one elected thread issues, for each group, S = Q K^T (128x64x16) into one of two accumulators and O += P V
 //         (128xDx16, P from tensor memory, V as an MN-major operand straight from its row-major tile), one tile behind
 // O is kept in units of a V scale that follows the tiles' scales where they are far apart (as in the decode kernel).
@@ -45,7 +47,7 @@ constexpr uint32_t kChunk = BN * 128;             // 64 keys x 64 elements of fp
 constexpr float kRescale = 8.f;                   // bits that the maximum may run ahead
 constexpr float kShift = 7.f;                     // P times 2^7: at most 2^15, and normal down to 2^-21 of a row's largest
 
-struct TileInfo { float ks, vs, log2_vs, per_vs; uint32_t seen[2]; };      // scales of the tile, keys that exist
+struct TileInfo { float ks, vs, log2_vs, per_vs; uint32_t seen[2], bf; };      // scales of the tile, keys that exist, P and V in bf16
 
 // G: groups of 128 query rows
 template <int D, int G>
@@ -55,7 +57,7 @@ struct Smem {
   uint8_t v[kStages][D / 64][kChunk];
   uint4 raw[2][BN * D / 16];                        // the codes of the tile to come, each piece read by the thread that copied it
   TileInfo info[kInfo];
-  float red[4];
+  float red[3][4];
   uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[G][2], p_full[G][2], pv_done[G], turn[2];
   uint32_t tmem_base;
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       asm volatile("{\n.reg .pred p, q;\nsetp.ne.u32 p, %1, 0;\nbarrier.cta.red.and.pred q, 1, 128, p;\nselp.u32 %0, 1, 0, q;\n}" : "=r"(y) : "r"((uint32_t)x) : "memory");
       return y != 0;
     };
-    auto put = [&](uint8_t (*to)[kChunk], const uint4* raw, const float* scale, float ref, auto values) {
+    auto put = [&](uint8_t (*to)[kChunk], const uint4* raw, const float* scale, float ref, bool bf, auto values) {
       asm volatile("cp.async.wait_group 1;" ::: "memory");
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -295,14 +297,14 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) e4m3x4_to_half2(w[e], h[2 * e], h[2 * e + 1]);
-        if constexpr (SMALL && decltype(values)::value) {            // V: bf16 values
+        if (SMALL && decltype(values)::value && bf) {                // V: bf16 values
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
             const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * scale[i], f.y * scale[i]);
             h[e] = *reinterpret_cast<const uint32_t*>(&b);
           }
-        } else if constexpr (SMALL) {                                // K: codes under the tile's largest scale
+        } else if constexpr (SMALL) {                                // codes under the tile's largest scale
           const __half2 f = __float2half2_rn(ref > 0.f ? scale[i] / ref : 0.f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) h[e] = half2_mul(h[e], f);
@@ -330,14 +332,32 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       const Where next = where(j + 1, ids);
       ids = ids_of(j + 2);
       float ref_k = w.ks[0];
-      const float ref_v = SMALL ? 1.f : w.vs[0];
+      float ref_v = w.vs[0];
+      bool bf = false;
       if constexpr (SMALL) {
+        float low = INFINITY;                      // smallest V scale of the tile
 #pragma unroll
-        for (int i = 1; i < N; ++i) ref_k = fmaxf(ref_k, w.ks[i]);
-        ref_k = warp_max(ref_k);
-        if (lane == 0) sm->red[warp - 4 * G] = ref_k;
+        for (int i = 0; i < N; ++i) {
+          ref_k = fmaxf(ref_k, w.ks[i]);
+          ref_v = fmaxf(ref_v, w.vs[i]);
+          if (w.vs[i] > 0.f) low = fminf(low, w.vs[i]);
+        }
+        // (order of numbers from 0 on: that of their bits)
+        ref_k = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(ref_k, 0.f))));
+        ref_v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(ref_v, 0.f))));
+        low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
+        if (lane == 0) {
+          sm->red[0][warp - 4 * G] = ref_k;
+          sm->red[1][warp - 4 * G] = ref_v;
+          sm->red[2][warp - 4 * G] = low;
+        }
         asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
-        ref_k = fmaxf(fmaxf(sm->red[0], sm->red[1]), fmaxf(sm->red[2], sm->red[3]));
+        const float (&r)[3][4] = sm->red;
+        ref_k = fmaxf(fmaxf(r[0][0], r[0][1]), fmaxf(r[0][2], r[0][3]));
+        ref_v = fmaxf(fmaxf(r[1][0], r[1][1]), fmaxf(r[1][2], r[1][3]));
+        low = fminf(fminf(r[2][0], r[2][1]), fminf(r[2][2], r[2][3]));
+        bf = low < ref_v * 0x1p-8f;
+        if (bf) ref_v = 1.f;
       }
       ok = mbar_wait(&sm->k_empty[stage], phase ^ 1) && ok;
       TileInfo& info = sm->info[j % kInfo];
@@ -347,6 +367,7 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
         info.vs = ref_v;
         info.log2_vs = log2f(ref_v);
         info.per_vs = 1.f / ref_v;
+        info.bf = bf;
       }
       if constexpr (SMALL) {
         ok = all(ok);                              // the waits of all ran out, or of none: everybody leaves together
@@ -362,12 +383,12 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       } else if (!ok) {
         break;
       }
-      put(sm->k[stage], sm->raw[0], w.ks, ref_k, std::false_type{});
+      put(sm->k[stage], sm->raw[0], w.ks, ref_k, false, std::false_type{});
       fence_proxy_async();
       mbar_arrive(&sm->k_full[stage]);
       fetch(sm->raw[0], a.kc, next);
       ok = mbar_wait(&sm->v_empty[stage], phase ^ 1);
-      put(sm->v[stage], sm->raw[1], w.vs, ref_v, std::true_type{});
+      put(sm->v[stage], sm->raw[1], w.vs, ref_v, bf, std::true_type{});
       fence_proxy_async();
       mbar_arrive(&sm->v_full[stage]);
       fetch(sm->raw[1], a.vc, next);
@@ -378,7 +399,7 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
   } else if (warp == 4 * G + 4) {
     // ------------------------------------------------ MMA issuer
     if (nblk > 0 && elect_one()) {
-      constexpr uint32_t idesc_qk = idesc_of(BM, BN, 0, 0), idesc_pv = idesc_of(BM, D, 1, SMALL);
+      constexpr uint32_t idesc_qk = idesc_of(BM, BN, 0, 0), idesc_pv_half = idesc_of(BM, D, 1, 0), idesc_pv_bf = idesc_of(BM, D, 1, 1);
       bool ok = mbar_wait(&sm->q_full, 0);
       tc_fence_after_sync();
       // O += P(i) V(i) is issued one tile behind the scores: the tensor core has the next S = Q K^T to run while the
@@ -386,6 +407,7 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       auto issue_pv = [&](int i) -> bool {
         const uint32_t st = i % kStages, ph = (i / kStages) & 1;
         if (!mbar_wait(&sm->v_full[st], ph)) return false;
+        const uint32_t idesc_pv = SMALL && sm->info[i % kInfo].bf ? idesc_pv_bf : idesc_pv_half;
         const uint64_t dv = make_mnmajor_sw128_desc(smem_u32(sm->v[st][0]), kChunk);
         for (int g = 0; g < G; ++g) {
           if (!mbar_wait(&sm->p_full[g][i & 1], (i >> 1) & 1)) return false;
@@ -551,12 +573,18 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
           const float2 y = fma2({__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, {f, f}, {off, off});
           const float p0 = exp2_approx(y.x), p1 = exp2_approx(y.y);
           sum2[i & 1] = add2(sum2[i & 1], {p0, p1});
-          if constexpr (SMALL) {
-            const __nv_bfloat162 x = __floats2bfloat162_rn(p0, p1);
+          s[2 * i] = __float_as_uint(p0);
+          s[2 * i + 1] = __float_as_uint(p1);
+        }
+        if (SMALL && info.bf) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
             w[i] = *reinterpret_cast<const uint32_t*>(&x);
-          } else {
-            w[i] = half2_bits(p0, p1);
           }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) w[i] = half2_bits(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
         }
         tmem_st_32x16(lane_addr + b * BN + 16 * half, w);      // over scores that are in registers already
       }
