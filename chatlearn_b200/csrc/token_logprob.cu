@@ -597,8 +597,9 @@ token_logprob_grad_kernel(const T* __restrict__ logits, int64_t stride, const in
   };
   int lo, hi;                                      // columns of this block
   if (same) {
-    lo = span == 0 ? 0 : head + span * kVecs * N;
-    hi = span == spans - 1 ? V : min(V, head + (span + 1) * kVecs * N);
+    // what lies behind the last whole vector is the last span's, though an earlier one may reach over it
+    lo = span == 0 ? 0 : min(tail, head + span * kVecs * N);
+    hi = span == spans - 1 ? V : min(tail, head + (span + 1) * kVecs * N);
     if (span == 0 && tid < head) d[tid] = q8::from_float<T>(grad(q8::to_float(z[tid])));
 #pragma unroll
     for (int i = 0; i < kGradVecs; ++i)
