@@ -17,8 +17,10 @@ constexpr int kWarp = 32;
 // tensor-memory allocation, descriptor prefetch) and block in pdl_wait() until the predecessor has completed and
 // its writes are visible.  pdl_trigger() tells the hardware that the successor may start; a grid's successor
 // starts once every CTA of the grid has triggered or exited.  Both are no-ops in a kernel launched the ordinary
-// way, and a successor launched the ordinary way waits for full completion as always.  Rule for every kernel
-// launched through launch_pdl: pdl_wait() comes before its first access to global memory.
+// way, and a successor launched the ordinary way waits for full completion as always.  Rules for every kernel
+// launched through launch_pdl: pdl_wait() comes before its first access to global memory, and every CTA reaches it
+// before it ends, those without work too: the successor's wait is for this grid alone, so that a grid which ends
+// without waiting would let the successor start on what an earlier kernel is still writing.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

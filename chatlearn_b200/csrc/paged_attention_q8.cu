@@ -691,7 +691,8 @@ paged_q8_kernel(const Args a) {
 
 // Joins the parts of the units that the cuts between blocks divide: block (c, r) looks after query head r of the unit that
 // the cut in front of share c + 1 divides, if it is the first cut inside its unit.  Where the cut lies is found while the
-// attention kernel still runs (it lets this one start only after the lengths are there).  Few and short loops: a handful
+// attention kernel still runs, ahead of the wait: from the lengths alone, which are there, because every block of the
+// attention kernel triggers this one behind its own wait for the kernels that wrote them.  Few and short loops: a handful
 // of warps run through here once, and waiting for code to arrive is a good part of what that takes.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) paged_q8_join_kernel(const Args a) {
@@ -701,17 +702,18 @@ __global__ void __launch_bounds__(kThreads) paged_q8_join_kernel(const Args a) {
   const int c = blockIdx.x + 1, r = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Place place = locate<tile_tokens(D)>(a, per_row, c, true);
   const int64_t pos = place.pos;
-  if (pos >= place.total) return;
-  const int tiles = tiles_of<tile_tokens(D)>(a, place.row);
+  bool mine = pos < place.total;
+  const int tiles = mine ? tiles_of<tile_tokens(D)>(a, place.row) : 1;
   const int unit = (int)((uint32_t)(pos - place.base) / (uint32_t)tiles);
   const int64_t start = place.base + (int64_t)unit * tiles, stop = start + tiles;
   const int head = unit / row_tiles, rt = unit - head * row_tiles;
-  if (pos == start || place.begin(c - 1) > start || r >= min(a.unit_rows, rep - rt * a.unit_rows)) return;
+  mine = mine && pos != start && place.begin(c - 1) <= start && r < min(a.unit_rows, rep - rt * a.unit_rows);
   // parts: the end of share c - 1 and the shares from c on that begin before `stop`
   int last = c + (int)((uint32_t)(stop - 1 - pos) / (uint32_t)min(place.share + 1, (int64_t)1 << 31));      // no share is longer
-  while (last + 1 < place.shares && place.begin(last + 1) < stop) ++last;
+  while (mine && last + 1 < place.shares && place.begin(last + 1) < stop) ++last;
   const int parts = last - c + 2;
-  pdl_wait();
+  pdl_wait();                                      // blocks without a cut wait too: this grid's end says that the outputs are there
+  if (!mine) return;
   auto slot = [&](int x) { return (x == 0 ? 2 * (c - 1) + 1 : 2 * (c - 1 + x)) * a.unit_rows + r; };
   float big = -INFINITY;
   for (int x = lane; x < parts; x += 32) big = fmaxf(big, a.part_ml[slot(x) * 2]);
