@@ -347,9 +347,9 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
         if (lane >= 16 && tail + lane - 16 < V) take_one(q8::to_float(z[tail + lane - 16]), tail + lane - 16);
       }
     };
-    // what reaches it
+    // what reaches it (where nothing does: NaN too, whose vectors have NaN for a maximum)
     auto look = [&](const uint4& u, int v) {
-      if (raw_max<T>(u) >= bound) {
+      if (!(raw_max<T>(u) < bound)) {
         float f[N];
         expand<T>(u, f);
 #pragma unroll
@@ -400,7 +400,7 @@ token_logprob_kernel(const T* __restrict__ logits, int64_t stride, const int64_t
           uint4 u[kUnroll];
           fetch(b0 + warp + i * kWarps, u);
           const float m = warp_max_f32(fmaxf(fmaxf(raw_max<T>(u[0]), raw_max<T>(u[1])), fmaxf(raw_max<T>(u[2]), raw_max<T>(u[3]))));
-          if (lane == 0) sh.stretch[warp + i * kWarps] = m;
+          if (lane == 0) sh.stretch[warp + i * kWarps] = fmaxf(m, -INFINITY);        // of nothing but NaN: -inf
         }
       } else if (lane < nth) {
         sh.stretch[warp + lane * kWarps] = maxima;

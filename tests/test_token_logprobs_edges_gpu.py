@@ -1,8 +1,11 @@
 """Token statistics on a GPU at the places where blocks, vectors and lists of candidates end."""
+import math
+
 import pytest
 import torch
 
 from chatlearn_b200 import ops
+from chatlearn_b200.ops import reference as ref
 from tests.test_token_logprobs_gpu import _check
 
 pytestmark = pytest.mark.gpu
@@ -29,3 +32,47 @@ def test_gradient_of_the_last_columns(dtype, V, pad):
         dz, = torch.autograd.grad(out.logprob.sum() + out.top_logprobs.sum(), leaf)
         first = dz if first is None else first
         assert torch.equal(dz, first)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,V", [(1, 151936), (3, 40001), (3, 997), (400, 4099), (310, 100003)])
+@pytest.mark.parametrize("n", [1, 8, 64])
+def test_nan_ranks_as_minus_infinity(dtype, R, V, n):
+    """Rows of nothing but NaN, and rows with fewer other logits than alternatives: ids as the statement has them, with
+    a cluster to a row and with one block."""
+    g = torch.Generator().manual_seed(R + V)
+    z = (torch.randn(R, V, generator=g) * 2).to(dtype)
+    rows = [z[r] for r in (0, R // 2, R - 1)]
+    rows[0].fill_(math.nan)
+    if R > 1:
+        rows[1][3:].fill_(math.nan)                                  # three ordinary logits, at the front
+        rows[2].fill_(math.nan)
+        rows[2][[V // 3, V - 1]] = torch.tensor([1.0, 2.0], dtype=dtype)
+    if R > 3:
+        z[1, :V // 2] = math.nan                                     # half a row
+        z[2, ::2] = math.nan                                         # every other one
+        z[3] = -math.inf
+        z[3, V // 2:] = math.nan                                     # equal ranks: by index
+    tok = torch.randint(0, V, (R,), generator=g)
+    got = ops.token_logprobs(z.to(DEV), tok.to(DEV), n)
+    want = ref.token_logprobs(z, tok, n)
+    assert torch.equal(got.top_ids.cpu(), want.top_ids)
+    nan = z.isnan().any(1)
+    assert got.logprob.cpu()[nan].isnan().all() and got.entropy.cpu()[nan].isnan().all() and got.top_logprobs.cpu()[nan].isnan().all()
+    assert torch.isfinite(got.logprob.cpu()[~nan]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("R,V", [(400, 8000), (4, 8000), (4, 60001), (400, 60001)])
+def test_equal_logits_beside_nan(dtype, R, V):
+    """Thousands of logits reach the n-th largest, and whole stretches between them are NaN."""
+    z = torch.zeros(R, V, dtype=dtype)
+    z[0, :V // 4] = math.nan
+    z[1, 600:2700] = math.nan
+    z[1, V - 5] = 3.0
+    z[2, 1:] = math.nan
+    z[3] = math.nan
+    tok = torch.zeros(R, dtype=torch.long)
+    for n in (2, 64):
+        got, want = ops.token_logprobs(z.to(DEV), tok.to(DEV), n), ref.token_logprobs(z, tok, n)
+        assert torch.equal(got.top_ids.cpu(), want.top_ids)
