@@ -10,10 +10,11 @@
 //         turns at the exponentials: one's run beside the other's maxima (both at once had the special-function units
 //         wait on them first and then stand idle: 389 -> 351 us at the case below)
 //   4     dequantisation: e4m3 codes from the pages, copied to shared memory a tile ahead, to fp16 tiles (exact) in the
-//         128-byte swizzle.  Pages of a multiple of 64 tokens keep their scales out of the tiles (S and P take them).  Of
-//         other pages a tile holds several: K is brought to the largest of its scales (what that loses is 2^-34 of the
-//         tile's largest keys); V too where its scales are within 2^8 (exact: its smallest code is then 2^-17), else V
-//         becomes bf16 values (exact) and P bf16 (8 bits), as fp16 has not the range for scales far apart.
+//         128-byte swizzle.  K's scales stay out of the tiles: S takes them, one for each 16 keys where pages end inside a
+//         tile, so that scales of any distance leave each other's keys alone.  V's too (P takes it) where a page covers
+//         the tile.  Of other pages V is brought to the largest of its scales where they are within 2^8 (exact: its
+//         smallest code is then 2^-17), else V becomes bf16 values (exact) and P bf16 (8 bits), as fp16 has not the range
+//         for scales far apart.
 //         (Always bf16 was 248 us where this takes 273, 8 x 256 tokens on pages of 16, with eight times P's rounding.)
 //   1     one elected thread issues, for each group, S = Q K^T (128x64x16) into one of two accumulators and O += P V
 //         (128xDx16, P from tensor memory, V as an MN-major operand straight from its row-major tile), one tile behind
@@ -47,7 +48,8 @@ constexpr uint32_t kChunk = BN * 128;             // 64 keys x 64 elements of fp
 constexpr float kRescale = 8.f;                   // bits that the maximum may run ahead
 constexpr float kShift = 7.f;                     // P times 2^7: at most 2^15, and normal down to 2^-21 of a row's largest
 
-struct TileInfo { float ks, vs, log2_vs, per_vs; uint32_t seen[2], bf; };      // scales of the tile, keys that exist, P and V in bf16
+// K's scale of each 16 keys (pages of a multiple of 64: the first one's is the tile's), V's scale, keys that exist, P and V in bf16
+struct TileInfo { float ks[4], vs, log2_vs, per_vs; uint32_t seen[2], bf; };
 
 // G: groups of 128 query rows
 template <int D, int G>
@@ -57,7 +59,7 @@ struct Smem {
   uint8_t v[kStages][D / 64][kChunk];
   uint4 raw[2][BN * D / 16];                        // the codes of the tile to come, each piece read by the thread that copied it
   TileInfo info[kInfo];
-  float red[3][4];
+  float red[2][4];
   uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[G][2], p_full[G][2], pv_done[G], turn[2];
   uint32_t tmem_base;
@@ -297,14 +299,14 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) e4m3x4_to_half2(w[e], h[2 * e], h[2 * e + 1]);
-        if (SMALL && decltype(values)::value && bf) {                // V: bf16 values
+        if (SMALL && decltype(values)::value && bf) {                // bf16 values
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[e]));
             const __nv_bfloat162 b = __floats2bfloat162_rn(f.x * scale[i], f.y * scale[i]);
             h[e] = *reinterpret_cast<const uint32_t*>(&b);
           }
-        } else if constexpr (SMALL) {                                // codes under the tile's largest scale
+        } else if constexpr (SMALL && decltype(values)::value) {     // codes under the tile's largest scale
           const __half2 f = __float2half2_rn(ref > 0.f ? scale[i] / ref : 0.f);
 #pragma unroll
           for (int e = 0; e < 8; ++e) h[e] = half2_mul(h[e], f);
@@ -331,39 +333,41 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       const uint32_t stage = j % kStages, phase = (j / kStages) & 1;
       const Where next = where(j + 1, ids);
       ids = ids_of(j + 2);
-      float ref_k = w.ks[0];
       float ref_v = w.vs[0];
       bool bf = false;
       if constexpr (SMALL) {
         float low = INFINITY;                      // smallest V scale of the tile
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          ref_k = fmaxf(ref_k, w.ks[i]);
           ref_v = fmaxf(ref_v, w.vs[i]);
           if (w.vs[i] > 0.f) low = fminf(low, w.vs[i]);
         }
         // (order of numbers from 0 on: that of their bits)
-        ref_k = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(ref_k, 0.f))));
         ref_v = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(ref_v, 0.f))));
         low = __uint_as_float(__reduce_min_sync(0xffffffffu, __float_as_uint(low)));
         if (lane == 0) {
-          sm->red[0][warp - 4 * G] = ref_k;
-          sm->red[1][warp - 4 * G] = ref_v;
-          sm->red[2][warp - 4 * G] = low;
+          sm->red[0][warp - 4 * G] = ref_v;
+          sm->red[1][warp - 4 * G] = low;
         }
         asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
-        const float (&r)[3][4] = sm->red;
-        ref_k = fmaxf(fmaxf(r[0][0], r[0][1]), fmaxf(r[0][2], r[0][3]));
-        ref_v = fmaxf(fmaxf(r[1][0], r[1][1]), fmaxf(r[1][2], r[1][3]));
-        low = fminf(fminf(r[2][0], r[2][1]), fminf(r[2][2], r[2][3]));
+        const float (&r)[2][4] = sm->red;
+        ref_v = fmaxf(fmaxf(r[0][0], r[0][1]), fmaxf(r[0][2], r[0][3]));
+        low = fminf(fminf(r[1][0], r[1][1]), fminf(r[1][2], r[1][3]));
         bf = low < ref_v * 0x1p-8f;
         if (bf) ref_v = 1.f;
       }
       ok = mbar_wait(&sm->k_empty[stage], phase ^ 1) && ok;
       TileInfo& info = sm->info[j % kInfo];
       if (tid < 2) info.seen[tid] = SMALL || (w.ok & 1u) ? 0xffffffffu : 0u;
+      if constexpr (SMALL) {
+        if (col == 0)
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if ((row + i * ROWS) % 16 == 0) info.ks[(row + i * ROWS) / 16] = w.ks[i];
+      } else if (tid == 0) {
+        info.ks[0] = w.ks[0];
+      }
       if (tid == 0) {
-        info.ks = ref_k;
         info.vs = ref_v;
         info.log2_vs = log2f(ref_v);
         info.per_vs = 1.f / ref_v;
@@ -383,7 +387,7 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       } else if (!ok) {
         break;
       }
-      put(sm->k[stage], sm->raw[0], w.ks, ref_k, false, std::false_type{});
+      put(sm->k[stage], sm->raw[0], w.ks, 1.f, false, std::false_type{});
       fence_proxy_async();
       mbar_arrive(&sm->k_full[stage]);
       fetch(sm->raw[0], a.kc, next);
@@ -502,6 +506,10 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
             if (!(see[half] >> i & 1)) s[i] = 0xff800000u;
         }
       };
+      constexpr int NF = SMALL ? 4 : 1;
+      float f[NF];
+#pragma unroll
+      for (int x = 0; x < NF; ++x) f[x] = fmaxf(sc * info.ks[x], 1e-37f);        // above 0: masked scores stay -inf at a softmax scale of 0 too
       uint32_t kept[2][G == 2 ? 32 : 1];
       float mx = -INFINITY;
 #pragma unroll
@@ -512,13 +520,15 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
 #pragma unroll
           for (int i = 0; i < 32; ++i) kept[half][i] = s[i];
         }
-        float top[4] = {mx, -INFINITY, -INFINITY, -INFINITY};      // four chains: one is bound by its instructions' latency
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // four chains: one is bound by its instructions' latency
+        // (chains 0 and 1: the first 16 keys, 2 and 3: the others)
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) top[i >> 1 & 3] = max3(top[i >> 1 & 3], __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-        mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        for (int i = 0; i < 32; i += 2) {
+          float& t = top[i >> 4 << 1 | (i >> 1 & 1)];
+          t = max3(t, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
+        }
+        mx = max3(mx, fmaxf(top[0], top[1]) * f[NF == 4 ? 2 * half : 0], fmaxf(top[2], top[3]) * f[NF == 4 ? 2 * half + 1 : 0]);
       }
-      const float f = fmaxf(sc * info.ks, 1e-37f);          // above 0: masked scores stay -inf at a softmax scale of 0 too
-      mx *= f;
       // units of the tile's P V: O's own, where the scales are near enough
       float change = 1.f, shift = 0.f, back = 1.f;
       if (info.vs > 0.f) {
@@ -570,7 +580,8 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float2 y = fma2({__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, {f, f}, {off, off});
+          const float by = f[NF == 4 ? 2 * half + (i >> 3) : 0];
+          const float2 y = fma2({__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, {by, by}, {off, off});
           const float p0 = exp2_approx(y.x), p1 = exp2_approx(y.y);
           sum2[i & 1] = add2(sum2[i & 1], {p0, p1});
           s[2 * i] = __float_as_uint(p0);

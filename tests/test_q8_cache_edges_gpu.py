@@ -44,3 +44,21 @@ def test_the_next_kernel_sees_the_output(lens, news, width):
             got = ops.linear(out, w)
             assert torch.equal(got, want)
     assert ops.launch_counts["gemm_bf16_nt"] == before["gemm_bf16_nt"] + 50
+
+
+@pytest.mark.parametrize("D,nkv,bs", [(128, 4, 16), (64, 8, 48), (256, 2, 32)])
+@pytest.mark.parametrize("apart", [14, 26, 40])
+def test_small_keys_beside_a_large_page(D, nkv, bs, apart):
+    """Pages inside a tile of 64 keys whose K scales are far apart, the large one behind the earlier rows: those see
+    their own keys as if it were not there.  Queries as large as their keys are small."""
+    L, n, big = 300, 280, 160                      # the page of token `big` is large: rows of earlier tokens do not see it
+    cache, table = oracle.make_cache([L], nkv, D, bs, device=DEV)
+    at = big // bs * bs
+    plain = [t.clone() for t in cache]
+    cache.k_scale[table[0, big // bs].long()] = 2.0 ** (apart - 7)
+    q = (torch.randn(n, 4 * nkv, D, generator=torch.Generator().manual_seed(0)) * 0.5).bfloat16().to(DEV)
+    got = ops.paged_attention_q8(q, cache, table, _i32([L]), _i32([n]))
+    rows = at - (L - n)                            # new tokens in front of the page
+    want, around, size = oracle.attend(q[:rows], ops.Q8KVCache(*plain), table, _i32([at]), _i32([rows]))
+    off, tol = (got[:rows].cpu().double() - want).abs(), oracle.attend_bound(want, around, size, L, D, torch.bfloat16)
+    assert rows > 64 and (off <= tol).all(), f"worst {(off / tol.clamp_min(1e-30)).max():.3g} times the bound"
