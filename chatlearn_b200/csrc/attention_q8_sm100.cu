@@ -48,8 +48,7 @@ constexpr uint32_t kChunk = BN * 128;             // 64 keys x 64 elements of fp
 constexpr float kRescale = 8.f;                   // bits that the maximum may run ahead
 constexpr float kShift = 7.f;                     // P times 2^7: at most 2^15, and normal down to 2^-21 of a row's largest
 
-// K's scale of each 16 keys (pages of a multiple of 64: the first one's is the tile's), V's scale, keys that exist, P and V in bf16
-struct TileInfo { float ks[4], vs, log2_vs, per_vs; uint32_t seen[2], bf; };
+struct TileInfo { float ks, vs, log2_vs, per_vs; uint32_t seen[2], bf; };      // scales of the tile, keys that exist, P and V in bf16
 
 // G: groups of 128 query rows
 template <int D, int G>
@@ -59,6 +58,7 @@ struct Smem {
   uint8_t v[kStages][D / 64][kChunk];
   uint4 raw[2][BN * D / 16];                        // the codes of the tile to come, each piece read by the thread that copied it
   TileInfo info[kInfo];
+  float4 ks[kInfo];                                 // K's scale of each 16 keys, where pages end inside a tile
   float red[2][4];
   uint64_t q_full, k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[G][2], p_full[G][2], pv_done[G], turn[2];
@@ -363,11 +363,10 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
         if (col == 0)
 #pragma unroll
           for (int i = 0; i < N; ++i)
-            if ((row + i * ROWS) % 16 == 0) info.ks[(row + i * ROWS) / 16] = w.ks[i];
-      } else if (tid == 0) {
-        info.ks[0] = w.ks[0];
+            if ((row + i * ROWS) % 16 == 0) reinterpret_cast<float*>(&sm->ks[j % kInfo])[(row + i * ROWS) / 16] = w.ks[i];
       }
       if (tid == 0) {
+        info.ks = w.ks[0];
         info.vs = ref_v;
         info.log2_vs = log2f(ref_v);
         info.per_vs = 1.f / ref_v;
@@ -507,9 +506,11 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
         }
       };
       constexpr int NF = SMALL ? 4 : 1;
-      float f[NF];
-#pragma unroll
-      for (int x = 0; x < NF; ++x) f[x] = fmaxf(sc * info.ks[x], 1e-37f);        // above 0: masked scores stay -inf at a softmax scale of 0 too
+      float f[NF];                                          // scales of the scores; above 0: masked ones stay -inf at a softmax scale of 0 too
+      if constexpr (SMALL) {
+        const float4 ks = sm->ks[j % kInfo];
+        f[0] = fmaxf(sc * ks.x, 1e-37f); f[1] = fmaxf(sc * ks.y, 1e-37f); f[2] = fmaxf(sc * ks.z, 1e-37f); f[3] = fmaxf(sc * ks.w, 1e-37f);
+      }
       uint32_t kept[2][G == 2 ? 32 : 1];
       float mx = -INFINITY;
 #pragma unroll
@@ -520,14 +521,19 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
 #pragma unroll
           for (int i = 0; i < 32; ++i) kept[half][i] = s[i];
         }
-        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};      // four chains: one is bound by its instructions' latency
-        // (chains 0 and 1: the first 16 keys, 2 and 3: the others)
+        // four chains: one is bound by its instructions' latency (SMALL: 0 and 1 the first 16 keys, 2 and 3 the others)
+        float top[4] = {SMALL ? -INFINITY : mx, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float& t = top[i >> 4 << 1 | (i >> 1 & 1)];
+          float& t = top[SMALL ? i >> 4 << 1 | (i >> 1 & 1) : i >> 1 & 3];
           t = max3(t, __uint_as_float(s[i]), __uint_as_float(s[i + 1]));
         }
-        mx = max3(mx, fmaxf(top[0], top[1]) * f[NF == 4 ? 2 * half : 0], fmaxf(top[2], top[3]) * f[NF == 4 ? 2 * half + 1 : 0]);
+        if constexpr (SMALL) mx = max3(mx, fmaxf(top[0], top[1]) * f[2 * half], fmaxf(top[2], top[3]) * f[2 * half + 1]);
+        else mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      }
+      if constexpr (!SMALL) {
+        f[0] = fmaxf(sc * info.ks, 1e-37f);
+        mx *= f[0];
       }
       // units of the tile's P V: O's own, where the scales are near enough
       float change = 1.f, shift = 0.f, back = 1.f;
