@@ -47,6 +47,9 @@ constexpr int BM = 128, BN = 64, kStages = 2, kInfo = 8;
 constexpr uint32_t kChunk = BN * 128;             // 64 keys x 64 elements of fp16
 constexpr float kRescale = 8.f;                   // bits that the maximum may run ahead
 constexpr float kShift = 7.f;                     // P times 2^7: at most 2^15, and normal down to 2^-21 of a row's largest
+// Scores (in bits) from which a score's product is rounded before the maximum is taken off.  The exact product inside a
+// fused multiply-add is off the rounded maximum by up to half a step of it: 2^-4 at 2^20, more than P has room for from 2^24 on
+constexpr float kFarScore = 0x1p20f;
 
 struct TileInfo { float ks, vs, log2_vs, per_vs; uint32_t seen[2], bf; };      // scales of the tile, keys that exist, P and V in bf16
 
@@ -479,10 +482,11 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
 
     const uint32_t lane_addr = tmem_base + g * kGroupCols + ((uint32_t)((warp & 3) * 32) << 16);
     float m = -INFINITY, l = 0.f, unit = 0.f, per_unit = 0.f, log2_unit = 0.f;
-    bool ok = true;
-    for (int j = 0; j < nblk; ++j) {
+    bool ok = true, far = false;                            // far: a row of the warp has a maximum of kFarScore or more
+    // a tile; false: it has to be done again, as the maximum turned out to be far (or a wait ran out)
+    auto take = [&](int j, auto from_far) {
       const uint32_t b = j & 1;
-      if (!mbar_wait(&sm->s_full[g][b], (j >> 1) & 1)) { ok = false; break; }
+      if (!mbar_wait(&sm->s_full[g][b], (j >> 1) & 1)) return ok = false;
       tc_fence_after_sync();
       const TileInfo info = sm->info[j % kInfo];
       const int k0 = j * BN;
@@ -554,10 +558,11 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       // O must be at rest before it is rescaled.  The barrier is in the phase of P(j - 1) V(j - 1) or behind it: S(j) was
       // issued after P(j - 2) V(j - 2) was done, and P(j) is not given yet.  The last tile waits too, so that the wait after
       // the loop finds it one phase on.
-      if (j > 0 && (rescale || j == nblk - 1) && !mbar_wait(&sm->pv_done[g], (j - 1) & 1)) { ok = false; break; }
+      if (j > 0 && (rescale || j == nblk - 1) && !mbar_wait(&sm->pv_done[g], (j - 1) & 1)) return ok = false;
       if (rescale) {
         const float alpha = need ? exp2_approx(m - mx) : 1.f;
         if (need) m = mx;
+        far = __any_sync(0xffffffffu, fabsf(m) >= kFarScore && m != -INFINITY);
         l *= alpha;
         const float by = alpha * change;
         tc_fence_after_sync();
@@ -571,9 +576,10 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
           tmem_st_32x32(lane_addr + kOCol + cc, o);
         }
         tmem_st_wait();
+        if (far && !decltype(from_far)::value) return false;
       }
-      const float off = m == -INFINITY ? 0.f : kShift - m + shift;
-      if (G == 2 && (g == 1 || j > 0) && !mbar_wait(&sm->turn[g], (j + g - 1) & 1)) { ok = false; break; }
+      const float base = m == -INFINITY ? 0.f : m, off = m == -INFINITY ? 0.f : kShift - m + shift;
+      if (G == 2 && (g == 1 || j > 0) && !mbar_wait(&sm->turn[g], (j + g - 1) & 1)) return ok = false;
       float2 sum2[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -586,8 +592,12 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
         }
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float by = f[NF == 4 ? 2 * half + (i >> 3) : 0];
-          const float2 y = fma2({__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])}, {by, by}, {off, off});
+          const float by = f[NF == 4 ? 2 * half + (i >> 3) : 0], s0 = __uint_as_float(s[2 * i]), s1 = __uint_as_float(s[2 * i + 1]);
+          float2 y;
+          if constexpr (decltype(from_far)::value)
+            y = {__fadd_rn(__fmul_rn(s0, by), -base) + (kShift + shift), __fadd_rn(__fmul_rn(s1, by), -base) + (kShift + shift)};
+          else
+            y = fma2({s0, s1}, {by, by}, {off, off});
           const float p0 = exp2_approx(y.x), p1 = exp2_approx(y.y);
           sum2[i & 1] = add2(sum2[i & 1], {p0, p1});
           s[2 * i] = __float_as_uint(p0);
@@ -614,7 +624,9 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       tmem_st_wait();
       tc_fence_before_sync();
       mbar_arrive(&sm->p_full[g][b]);
-    }
+      return true;
+    };
+    for (int j = 0; j < nblk && ok;) j += far ? take(j, std::true_type{}) : take(j, std::false_type{});
     if (ok && nblk > 0 && !mbar_wait(&sm->pv_done[g], (nblk - 1) & 1)) ok = false;
     if (ok) {
       tc_fence_after_sync();

@@ -44,6 +44,9 @@ constexpr int kThreads = 128, kWarps = 4;
 __host__ __device__ constexpr int tile_tokens(int D) { return D >= 256 ? 16 : 32; }
 // probabilities are carried times 2^10: fp16 keeps 11 bits of them down to 2^-24 of the largest
 constexpr float kProbShift = 10.f;
+// scores (in bits) from which a score's product is rounded before the maximum is taken off: the exact product in a fused
+// multiply-add is off the rounded maximum by up to half a step of it, 2^-4 here, but 2^6 and more from 2^30 on
+constexpr float kFarScore = 0x1p20f;
 
 struct Args {
   const void* q;                 // [T, nq, D], row stride q_row
@@ -398,6 +401,7 @@ paged_q8_kernel(const Args a) {
       shift[h][0] = shift[h][1] = 0.f;
     }
     float unit_v = 0.f, per_unit = 0.f;            // o is kept in units of this V scale; 1 / unit_v
+    bool far = false;                              // of the whole warp
 
     for (int i = 0; i < n; ++i) {
       __pipeline_wait_prior(ST - 2);
@@ -481,10 +485,27 @@ paged_q8_kernel(const Args a) {
               const float top = fmaxf(m[h][y], mx[h][y]);
               const float alpha = top == m[h][y] ? 1.f : exp2_approx(m[h][y] - top);
               m[h][y] = top;
+              far |= fabsf(top) >= kFarScore && top != -INFINITY;
               shift[h][y] = top == -INFINITY ? 0.f : kProbShift - top;
               l[h][y] *= alpha;
 #pragma unroll
               for (int j = 0; j < NT; ++j) { o[h][j][y] *= alpha; o[h][j][2 + y] *= alpha; }
+            }
+          far = __any_sync(0xffffffffu, far);
+        }
+        if (far) {                                 // scores become their distances to the maximum
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              if (m[h][y] == -INFINITY) continue;
+#pragma unroll
+              for (int x = 0; x < PIECES; ++x) {
+                s[h][x][y] = __fadd_rn(__fmul_rn(s[h][x][y], f[h][y][x * PG / PIECES]), -m[h][y]);
+                s[h][x][2 + y] = __fadd_rn(__fmul_rn(s[h][x][2 + y], f[h][y][x * PG / PIECES]), -m[h][y]);
+              }
+#pragma unroll
+              for (int x = 0; x < PG; ++x) f[h][y][x] = 1.f;
             }
         }
 #pragma unroll
@@ -493,8 +514,9 @@ paged_q8_kernel(const Args a) {
           for (int y = 0; y < 2; ++y)
 #pragma unroll
             for (int x = 0; x < PIECES; ++x) {
-              s[h][x][y] = exp2_approx(fmaf(s[h][x][y], f[h][y][x * PG / PIECES], shift[h][y]));
-              s[h][x][2 + y] = exp2_approx(fmaf(s[h][x][2 + y], f[h][y][x * PG / PIECES], shift[h][y]));
+              const float off = far && m[h][y] != -INFINITY ? kProbShift : shift[h][y];
+              s[h][x][y] = exp2_approx(fmaf(s[h][x][y], f[h][y][x * PG / PIECES], off));
+              s[h][x][2 + y] = exp2_approx(fmaf(s[h][x][2 + y], f[h][y][x * PG / PIECES], off));
               l[h][y] += s[h][x][y] + s[h][x][2 + y];
             }
         // ---- O^T += V^T P^T, 16 tokens at a time: lane g holds the elements of its piece of V's rows

@@ -62,3 +62,30 @@ def test_small_keys_beside_a_large_page(D, nkv, bs, apart):
     want, around, size = oracle.attend(q[:rows], ops.Q8KVCache(*plain), table, _i32([at]), _i32([rows]))
     off, tol = (got[:rows].cpu().double() - want).abs(), oracle.attend_bound(want, around, size, L, D, torch.bfloat16)
     assert rows > 64 and (off <= tol).all(), f"worst {(off / tol.clamp_min(1e-30)).max():.3g} times the bound"
+
+
+@pytest.mark.parametrize("nq,nkv,D,bs", [(32, 8, 128, 64), (16, 4, 128, 16), (32, 4, 64, 64), (16, 2, 256, 32), (64, 8, 64, 48), (32, 2, 128, 64)])
+@pytest.mark.parametrize("power", [18, 24, 30, 45, 70])
+@pytest.mark.parametrize("chunk", [False, True])
+def test_scores_far_from_zero(nq, nkv, D, bs, power, chunk):
+    """Scores of 2^18 to 2^70 whose largest is twice the next: all weight is on that key, whose value comes back as it is.
+    (One element of q and of each key: the scores are exact, but for the softmax scale.)"""
+    L = 200
+    cache, table = oracle.make_cache([L], nkv, D, bs, device=DEV)
+    # token 0 is the one: every row of new tokens sees it
+    cache.k.view(torch.uint8).zero_()
+    codes = torch.full((cache.k.shape[0], nkv, bs), 8.0)
+    codes[int(table[0, 0]), :, 0] = 16.0
+    cache.k[..., 5] = codes.to(DEV).to(cache.k.dtype)
+    cache.k_scale.fill_(2.0 ** (power // 2))
+    n = 180 if chunk else 1
+    q = torch.zeros(n, nq, D, device=DEV, dtype=torch.bfloat16)
+    q[..., 5] = 1.5 * 2.0 ** (power - power // 2)
+    got = ops.paged_attention_q8(q, cache, table, _i32([L]), _i32([n]) if chunk else None)
+    v = cache.dequantize()[1][int(table[0, 0]), :, 0]                          # [nkv, D], exact in bf16
+    assert torch.equal(got.float(), v.repeat_interleave(nq // nkv, 0)[None].expand(n, -1, -1))
+    # all but that key at the same score: where it is out of sight, the mean
+    cache.k[..., 5] = torch.full_like(codes, 8.0).to(DEV).to(cache.k.dtype)
+    got = ops.paged_attention_q8(q, cache, table, _i32([L]), _i32([n]) if chunk else None).cpu().double()
+    want, around, _ = oracle.attend(q, cache, table, _i32([L]), _i32([n]) if chunk else None)
+    assert ((got - want).abs() <= oracle.attend_bound(want, around, 0.0, L, D, torch.bfloat16)).all()
