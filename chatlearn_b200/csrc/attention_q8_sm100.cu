@@ -13,9 +13,9 @@
 //         128-byte swizzle.  K's scales stay out of the tiles: S takes them, one for each 16 keys where pages end inside a
 //         tile, so that scales of any distance leave each other's keys alone.  V's too (P takes it) where a page covers
 //         the tile.  Of other pages V is brought to the largest of its scales where they are within 2^8 (exact: its
-//         smallest code is then 2^-17), else V becomes bf16 values (exact) and P bf16 (8 bits), as fp16 has not the range
-//         for scales far apart.
-//         (Always bf16 was 248 us where this takes 273, 8 x 256 tokens on pages of 16, with eight times P's rounding.)
+//         smallest code is then 2^-17), else V becomes bf16 values (exact) and P two bf16, the second what the first's
+//         rounding leaves (17 bits in all), as fp16 has not the range for scales far apart.
+//         (8 x 256 tokens on pages of 16: 277 us, where every tile's scales are far apart 316)
 //   1     one elected thread issues, for each group, S = Q K^T (128x64x16) into one of two accumulators and O += P V
 //         (128xDx16, P from tensor memory, V as an MN-major operand straight from its row-major tile), one tile behind
 // O is kept in units of a V scale that follows the tiles' scales where they are far apart (as in the decode kernel).
@@ -413,15 +413,19 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
       auto issue_pv = [&](int i) -> bool {
         const uint32_t st = i % kStages, ph = (i / kStages) & 1;
         if (!mbar_wait(&sm->v_full[st], ph)) return false;
-        const uint32_t idesc_pv = SMALL && sm->info[i % kInfo].bf ? idesc_pv_bf : idesc_pv_half;
+        const bool bf = SMALL && sm->info[i % kInfo].bf;
+        const uint32_t idesc_pv = bf ? idesc_pv_bf : idesc_pv_half;
         const uint64_t dv = make_mnmajor_sw128_desc(smem_u32(sm->v[st][0]), kChunk);
         for (int g = 0; g < G; ++g) {
           if (!mbar_wait(&sm->p_full[g][i & 1], (i >> 1) & 1)) return false;
           tc_fence_after_sync();
           const uint32_t base = tmem_base + g * kGroupCols, p_tmem = base + (i & 1) * BN;
 #pragma unroll
-          for (int kk = 0; kk < BN / 16; ++kk)
-            umma_ts(base + kOCol, p_tmem + 8 * kk, dv + 128ull * kk, idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+          for (int kk = 0; kk < BN / 16; ++kk) {
+            const uint32_t p = p_tmem + (bf ? 32 * (kk >> 1) + 8 * (kk & 1) : 8 * kk);
+            umma_ts(base + kOCol, p, dv + 128ull * kk, idesc_pv, (i > 0 || kk > 0) ? 1u : 0u);
+            if (bf) umma_ts(base + kOCol, p + 16, dv + 128ull * kk, idesc_pv, 1u);
+          }
           umma_commit(&sm->pv_done[g]);
         }
         umma_commit(&sm->v_empty[st]);
@@ -603,17 +607,24 @@ __global__ void __launch_bounds__(128 * G + 160, D == 256 || G == 2 ? 1 : 2) chu
           s[2 * i] = __float_as_uint(p0);
           s[2 * i + 1] = __float_as_uint(p1);
         }
-        if (SMALL && info.bf) {
+        // over scores that are in registers already
+        if (SMALL && info.bf) {                             // P and what its rounding leaves, side by side
+          uint32_t rest[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const __nv_bfloat162 x = __floats2bfloat162_rn(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+            const float p0 = __uint_as_float(s[2 * i]), p1 = __uint_as_float(s[2 * i + 1]);
+            const __nv_bfloat162 x = __floats2bfloat162_rn(p0, p1);
+            const __nv_bfloat162 y = __floats2bfloat162_rn(p0 - __low2float(x), p1 - __high2float(x));
             w[i] = *reinterpret_cast<const uint32_t*>(&x);
+            rest[i] = *reinterpret_cast<const uint32_t*>(&y);
           }
+          tmem_st_32x16(lane_addr + b * BN + 32 * half, w);
+          tmem_st_32x16(lane_addr + b * BN + 32 * half + 16, rest);
         } else {
 #pragma unroll
           for (int i = 0; i < 16; ++i) w[i] = half2_bits(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1]));
+          tmem_st_32x16(lane_addr + b * BN + 16 * half, w);
         }
-        tmem_st_32x16(lane_addr + b * BN + 16 * half, w);      // over scores that are in registers already
       }
       if (G == 2) {
         __syncwarp();

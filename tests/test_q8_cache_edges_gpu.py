@@ -89,3 +89,22 @@ def test_scores_far_from_zero(nq, nkv, D, bs, power, chunk):
     got = ops.paged_attention_q8(q, cache, table, _i32([L]), _i32([n]) if chunk else None).cpu().double()
     want, around, _ = oracle.attend(q, cache, table, _i32([L]), _i32([n]) if chunk else None)
     assert ((got - want).abs() <= oracle.attend_bound(want, around, 0.0, L, D, torch.bfloat16)).all()
+
+
+@pytest.mark.parametrize("D,nkv,bs", [(128, 4, 16), (64, 8, 48), (256, 2, 32), (64, 8, 16)])
+@pytest.mark.parametrize("apart", [0, 8, 9, 30])
+@pytest.mark.parametrize("lens,news", [([300], [300]), ([130, 400, 77], [130, 100, 70])])
+def test_probabilities_on_small_pages(D, nkv, bs, apart, lens, news):
+    """Tiles of several pages hold probabilities to 2^-11 or better, whatever their V scales are (2^8 apart: the last
+    that fp16 takes; 2^9: the first that it does not)."""
+    cache, table = oracle.make_cache(lens, nkv, D, bs, device=DEV)
+    if apart:
+        cache.v_scale.fill_(2.0 ** -7)
+        cache.v_scale[table[:, 1::2].long()] = 2.0 ** (apart - 7)
+    g = torch.Generator().manual_seed(1)
+    q = (torch.randn(sum(news), 4 * nkv, D, generator=g) * 0.25).bfloat16().to(DEV)
+    lens_t, news_t = _i32(lens), _i32(news)
+    got = ops.paged_attention_q8(q, cache, table, lens_t, news_t).cpu().double()
+    want, around, size = oracle.attend(q, cache, table, lens_t, news_t)
+    off, tol = (got - want).abs(), oracle.attend_bound(want, around, size, max(lens), D, torch.bfloat16, 2.0 ** -11)
+    assert (off <= tol).all(), f"worst {(off / tol.clamp_min(1e-30)).max():.3g} times the bound"
