@@ -12,6 +12,19 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+const char* const kOnce = "token_logprobs is differentiable once";
+
+// The gradient where a graph of it is asked for: a node that refuses to be differentiated, so that nobody takes a gradient
+// that depends on the logits for a constant.
+struct TokenLogprobGrad : torch::autograd::Function<TokenLogprobGrad> {
+  static at::Tensor forward(AutogradContext*, const at::Tensor& z, const at::Tensor& tokens, const at::Tensor& ent, const at::Tensor& stats,
+                            const at::Tensor& ids, const c10::optional<at::Tensor>& g_lp, const c10::optional<at::Tensor>& g_ent,
+                            const c10::optional<at::Tensor>& g_top, double inv_temp) {
+    return token_logprob_bwd(z, tokens, ent, stats, ids, g_lp, g_ent, g_top, inv_temp);
+  }
+  static variable_list backward(AutogradContext*, variable_list) { TORCH_CHECK(false, kOnce); }
+};
+
 struct TokenLogprob : torch::autograd::Function<TokenLogprob> {
   static variable_list forward(AutogradContext* ctx, const at::Tensor& z, const at::Tensor& tokens, int64_t n, double inv_temp) {
     auto out = token_logprob_fwd(z, tokens, n, inv_temp);
@@ -30,12 +43,15 @@ struct TokenLogprob : torch::autograd::Function<TokenLogprob> {
       return t.to(at::kFloat).contiguous();
     };
     const auto lp = plain(g[0]), ent = plain(g[1]), top = plain(g[2]);
+    const double inv_temp = ctx->saved_data["inv_temp"].toDouble();
     at::Tensor dz;
     if (lp || ent || top) {
-      TORCH_CHECK(!at::GradMode::is_enabled() || !((lp && lp->requires_grad()) || (ent && ent->requires_grad()) || (top && top->requires_grad())),
-                  "token_logprobs is differentiable once");
-      at::AutoDispatchBelowADInplaceOrView below;
-      dz = token_logprob_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], lp, ent, top, ctx->saved_data["inv_temp"].toDouble());
+      if (at::GradMode::is_enabled()) {
+        dz = TokenLogprobGrad::apply(saved[0], saved[1], saved[2], saved[3], saved[4], lp, ent, top, inv_temp);
+      } else {
+        at::AutoDispatchBelowADInplaceOrView below;
+        dz = token_logprob_bwd(saved[0], saved[1], saved[2], saved[3], saved[4], lp, ent, top, inv_temp);
+      }
     }
     return {dz, at::Tensor(), at::Tensor(), at::Tensor()};
   }

@@ -76,3 +76,25 @@ def test_equal_logits_beside_nan(dtype, R, V):
     for n in (2, 64):
         got, want = ops.token_logprobs(z.to(DEV), tok.to(DEV), n), ref.token_logprobs(z, tok, n)
         assert torch.equal(got.top_ids.cpu(), want.top_ids)
+
+
+@pytest.mark.parametrize("which", ["logprob", "entropy", "top_logprobs"])
+def test_second_derivatives_are_refused(which):
+    """A gradient whose graph is asked for is no constant, with constant incoming gradients either."""
+    z = torch.randn(3, 500, device=DEV, requires_grad=True)
+    w = torch.randn(3, 500, device=DEV, requires_grad=True)
+    tok = torch.tensor([1, 2, 3], device=DEV)
+    plain, = torch.autograd.grad(getattr(ops.token_logprobs(z, tok, 4), which).sum(), z)
+    dz, = torch.autograd.grad(getattr(ops.token_logprobs(z, tok, 4), which).sum(), z, create_graph=True)
+    assert torch.equal(dz, plain) and dz.requires_grad
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        (dz.square().sum() + w.sum()).backward()
+    # incoming gradients that need one themselves
+    weight = torch.ones(3, device=DEV, requires_grad=True)
+    dz, = torch.autograd.grad((ops.token_logprobs(z, tok, 4).logprob * weight).sum(), z, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        dz.sum().backward()
+    # a graph of what lies in front of the operator stays open
+    loss = ops.token_logprobs(w * w, tok, 4).logprob.sum()
+    first, = torch.autograd.grad(loss, w, create_graph=True)
+    assert first.shape == w.shape
