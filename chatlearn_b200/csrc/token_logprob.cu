@@ -655,7 +655,8 @@ std::vector<at::Tensor> token_logprob_fwd(const at::Tensor& z, const at::Tensor&
   const bool fits = z.is_cuda() && z.dim() == 2 && (type == at::kBFloat16 || type == at::kHalf || type == at::kFloat) && z.size(1) > 0 &&
                     (z.size(1) == 1 || z.stride(1) == 1) && z.size(0) < (int64_t)1 << 28 && z.size(1) < (int64_t)1 << 30 && n >= 0 &&
                     n <= std::min<int64_t>(kMaxTop, z.size(1)) && inv_temp > 0.0 && tokens.scalar_type() == at::kLong && tokens.dim() == 1 &&
-                    tokens.size(0) == z.size(0) && tokens.is_contiguous() && tokens.device() == z.device();
+                    tokens.size(0) == z.size(0) && tokens.is_contiguous() && tokens.device() == z.device() &&
+                    !z._fw_grad(0).defined();
   if (!fits) return {};
   const c10::cuda::CUDAGuard guard(z.device());
   const int64_t R = z.size(0), V = z.size(1);

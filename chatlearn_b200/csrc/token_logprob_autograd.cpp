@@ -61,5 +61,6 @@ struct TokenLogprob : torch::autograd::Function<TokenLogprob> {
 
 // {log-prob, entropy, alternatives' log-probs, their ids}; empty where the arguments are not as the kernel takes them
 std::vector<at::Tensor> token_logprob_apply(const at::Tensor& z, const at::Tensor& tokens, int64_t n, double inv_temp) {
+  if (z._fw_grad(0).defined()) return {};          // forward mode: for the caller to refuse
   return TokenLogprob::apply(z, tokens, n, inv_temp);
 }

@@ -68,6 +68,8 @@ def token_logprobs(logits, tokens, top_n=0, temperature=1.0):
     out = run(logits, tokens, top_n, 1.0 / temperature) if 1e-30 <= temperature <= 1e30 else ()
     if not out:
         q8.check_token_logprobs(logits, tokens, top_n, temperature)
+        if torch.autograd.forward_ad.unpack_dual(logits).tangent is not None:
+            raise RuntimeError("token_logprobs: no forward-mode derivative on a GPU")
         if logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
             raise TypeError(f"token_logprobs: fp32, bf16 or fp16 logits, got {logits.dtype}")
         if top_n > MAX_TOP:

@@ -98,3 +98,18 @@ def test_second_derivatives_are_refused(which):
     loss = ops.token_logprobs(w * w, tok, 4).logprob.sum()
     first, = torch.autograd.grad(loss, w, create_graph=True)
     assert first.shape == w.shape
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(grad):
+    """A tangent on the logits is not dropped."""
+    import torch.autograd.forward_ad as fwad
+    z, tok = torch.randn(3, 500, device=DEV), torch.tensor([1, 2, 3], device=DEV)
+    with fwad.dual_level():
+        dual = fwad.make_dual(z.requires_grad_(grad), torch.ones_like(z))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.token_logprobs(dual, tok, 4)
+        with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():
+            ops.token_logprobs(dual, tok, 4)
+        ops.token_logprobs(z.detach(), tok, 4)
+    assert ops.token_logprobs(z, tok, 4).logprob.requires_grad == grad
