@@ -78,7 +78,8 @@ class PartialRolloutManager(BaseModule):
                 "input_ids": r["all_tokens"].tolist(),
                 "max_generate_token_length": kept["max_generate_token_length"],
             })
-            for k in ("rollout_logprobs", "finish_reason", "all_token_length"):
+            for k in ("rollout_logprobs", "rollout_entropies", "rollout_top_ids", "rollout_top_logprobs", "finish_reason",
+                      "all_token_length"):
                 if k in r:
                     kept[k] = r[k]
             if self.is_finished(kept):

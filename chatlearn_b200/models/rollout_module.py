@@ -19,6 +19,14 @@ from chatlearn_b200.synchronizer.parameter_sync import layout_of_model
 from chatlearn_b200.utils.constant import TAG_KV_CACHE, TAG_WEIGHTS
 
 
+def token_statistics(entropies, top_logprobs, n: int) -> Dict[str, torch.Tensor]:
+    """What the engine hands back per generated token, as a sample carries it: entropies [T] and the ``n`` likeliest
+    tokens with their log-probs [T, n]."""
+    return {"rollout_entropies": torch.tensor(entropies, dtype=torch.float32),
+            "rollout_top_ids": torch.tensor([[i for i, _ in t] for t in top_logprobs], dtype=torch.long).view(-1, n),
+            "rollout_top_logprobs": torch.tensor([[l for _, l in t] for t in top_logprobs], dtype=torch.float32).view(-1, n)}
+
+
 class RolloutModule(TorchModule):
     def __init__(self, name: str, args=None, replica_id: int = 0):
         super().__init__(name, args, replica_id)
@@ -163,10 +171,10 @@ class RolloutModule(TorchModule):
                 if self.tokenizer is not None else ""
             r["finish_reason"] = q.finish_reason
             r["rollout_logprobs"] = torch.tensor(q.logprobs, dtype=torch.float32)
-            if q.top_logprobs:
-                r["rollout_entropies"] = torch.tensor(q.entropies, dtype=torch.float32)
-                r["rollout_top_ids"] = torch.tensor([[i for i, _ in t] for t in q.top_logprobs], dtype=torch.long)
-                r["rollout_top_logprobs"] = torch.tensor([[l for _, l in t] for t in q.top_logprobs], dtype=torch.float32)
+            if q.sampling.logprobs:
+                new = token_statistics(q.entropies, q.top_logprobs, q.sampling.logprobs)
+                # (one row per response token: those of earlier partial rounds stay in front)
+                r.update({k: torch.cat([s[k], v]) if len(resp) > len(q.output) and k in s else v for k, v in new.items()})
             if "rollout_round" in r:
                 r["rollout_round"] += 1
             out.append(r)

@@ -1,0 +1,88 @@
+"""Entropies and alternatives of generated tokens on their way from the engine to a sample: partial rounds, agents."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from chatlearn_b200 import ops
+from chatlearn_b200.models.nn import CausalLM, packed_ctx
+from chatlearn_b200.models.nn.arch import PRESETS
+
+KEYS = ("rollout_entropies", "rollout_top_ids", "rollout_top_logprobs")
+
+
+def _rollout(cls, num_logprobs, **kw):
+    """A rollout role on the CPU around a tiny engine, without the runtime."""
+    from chatlearn_b200.rollout import RolloutEngine
+    role = cls.__new__(cls)
+    arch = PRESETS["tiny_qwen3"]()
+    model = CausalLM(arch, dtype=torch.float32).init_weights(2)
+    role.engine = RolloutEngine(model, block_size=8, num_blocks=128, max_num_seqs=16, max_model_len=128)
+    role.arch, role.tokenizer = arch, None
+    role._module_args = SimpleNamespace(vllm_input_ids_key="input_ids", max_response_tokens_length=8, seq_length=128, temperature=0.7,
+                                        top_p=1.0, top_k=-1, min_p=0.0, presence_penalty=0.0, frequency_penalty=0.0,
+                                        repetition_penalty=1.0, ignore_eos=True, num_logprobs=num_logprobs, **kw)
+    return role
+
+
+def _scored(role, tokens, n_prompt, n):
+    """The same statistics from one pass over the whole sequence."""
+    toks = torch.as_tensor(tokens)
+    ctx, _ = packed_ctx([toks.numel()], "cpu")
+    with torch.no_grad():
+        hidden = role.engine.model.hidden_states(toks, ctx)
+        z = torch.nn.functional.linear(hidden, role.engine.model.lm_head_weight()).double()[n_prompt - 1:-1]
+    return ops.token_logprobs(z, toks[n_prompt:], n, 0.7)
+
+
+def _check(role, r, n):
+    T = int(r["response_token_length"])
+    assert r["rollout_entropies"].shape == (T,) and r["rollout_top_ids"].shape == r["rollout_top_logprobs"].shape == (T, n)
+    want = _scored(role, r["all_tokens"], int(r["prompt_token_length"]), n)
+    # fp32 logits of a two-layer model, steps against one pass: 1e-4 is over 2^9 roundings of values near 1
+    assert (r["rollout_entropies"] - want.entropy).abs().max() < 1e-4
+    assert (r["rollout_top_logprobs"] - want.top_logprobs).abs().max() < 1e-4
+    assert torch.equal(r["rollout_top_ids"], want.top_ids)
+    return want
+
+
+def _partial_rounds(role, prompts):
+    """Two rounds of 4 tokens each through the manager; the samples that are handed to training."""
+    from chatlearn_b200.algorithm.grpo_utils.partial_rollout_manager import PartialRolloutManager
+    man = PartialRolloutManager.__new__(PartialRolloutManager)
+    man._module_args = SimpleNamespace(max_rollout_round=2, rollout_ratio=[0.5, 0.5], mini_response_per_prompt=0, seed=1)
+    man.global_args = SimpleNamespace(models=SimpleNamespace(policy=SimpleNamespace(max_response_tokens_length=8, num_inference_per_prompt=1)))
+    man._metric_list = []
+    man.setup()
+    batch = [{"uid": i, "prompt_uid": str(i), "input_ids": list(p), "prompt_token_ids": list(p)} for i, p in enumerate(prompts)]
+    done = []
+    for _ in range(2):
+        man.before_episode()
+        rows = man.get_sample_for_rollout(batch)
+        done += man.post_process_rollout_results(role.postprocess_func(rows, role.generate(rows)))
+        batch = []
+    return sorted(done, key=lambda r: r["uid"])
+
+
+@pytest.mark.parametrize("n", [0, 3])
+def test_statistics_of_partial_rounds(n):
+    """A sample that was carried on has them for every token of its response, those of the first round in front."""
+    from chatlearn_b200.models.rollout_module import RolloutModule
+    role = _rollout(RolloutModule, n)
+    done = _partial_rounds(role, [[5, 6, 7, 8], [9, 10, 11]])
+    assert len(done) == 2
+    for r in done:
+        assert int(r["response_token_length"]) == 8
+        if n:
+            _check(role, r, n)
+        else:
+            assert not any(k in r for k in KEYS)
+
+
+def test_statistics_of_responses_without_tokens():
+    """A prompt that fills the model's length still has the keys that its batch has."""
+    from chatlearn_b200.models.rollout_module import RolloutModule
+    role = _rollout(RolloutModule, 2)
+    rows = [{"input_ids": [3, 4, 5]}, {"input_ids": list(range(128))}]
+    out = role.postprocess_func(rows, role.generate(rows))
+    assert [tuple(r[k].shape) for r in out for k in KEYS] == [(8,), (8, 2), (8, 2), (0,), (0, 2), (0, 2)]
