@@ -170,11 +170,12 @@ class RolloutModule(TorchModule):
             r["str_outputs"] = self.tokenizer.decode(resp, skip_special_tokens=True) \
                 if self.tokenizer is not None else ""
             r["finish_reason"] = q.finish_reason
-            r["rollout_logprobs"] = torch.tensor(q.logprobs, dtype=torch.float32)
+            new = {"rollout_logprobs": torch.tensor(q.logprobs, dtype=torch.float32)}
             if q.sampling.logprobs:
-                new = token_statistics(q.entropies, q.top_logprobs, q.sampling.logprobs)
-                # (one row per response token: those of earlier partial rounds stay in front)
-                r.update({k: torch.cat([s[k], v]) if len(resp) > len(q.output) and k in s else v for k, v in new.items()})
+                new.update(token_statistics(q.entropies, q.top_logprobs, q.sampling.logprobs))
+            # one row per response token: those of earlier partial rounds stay in front
+            before = len(resp) - len(q.output)
+            r.update({k: torch.cat([s[k], v]) if before > 0 and k in s and len(s[k]) == before else v for k, v in new.items()})
             if "rollout_round" in r:
                 r["rollout_round"] += 1
             out.append(r)

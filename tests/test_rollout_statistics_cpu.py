@@ -86,3 +86,12 @@ def test_statistics_of_responses_without_tokens():
     rows = [{"input_ids": [3, 4, 5]}, {"input_ids": list(range(128))}]
     out = role.postprocess_func(rows, role.generate(rows))
     assert [tuple(r[k].shape) for r in out for k in KEYS] == [(8,), (8, 2), (8, 2), (0,), (0, 2), (0, 2)]
+
+
+def test_log_probs_of_partial_rounds():
+    """Log-probs belong to the response's tokens from its first one on: what the trainer compares them with."""
+    from chatlearn_b200.models.rollout_module import RolloutModule
+    role = _rollout(RolloutModule, 0)
+    for r in _partial_rounds(role, [[5, 6, 7, 8], [9, 10, 11]]):
+        want = _scored(role, r["all_tokens"], int(r["prompt_token_length"]), 0)
+        assert r["rollout_logprobs"].shape == (8,) and (r["rollout_logprobs"] - want.logprob).abs().max() < 1e-4
