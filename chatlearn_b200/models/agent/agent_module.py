@@ -17,7 +17,7 @@ from typing import Dict, List, Type
 
 import torch
 
-from chatlearn_b200.models.rollout_module import RolloutModule
+from chatlearn_b200.models.rollout_module import RolloutModule, token_statistics
 from chatlearn_b200.rollout.engine import SamplingParams
 from .base_agent_graph import AgentGraphOutput, BaseAgentGraph
 from .chat_model import LLMRequest, LLMResponse
@@ -67,7 +67,13 @@ class AgentModule(RolloutModule):
             sps.append(sp)
         mm = [r.mm for r in reqs] if self.engine.vision is not None and any(r.mm is not None for r in reqs) else None
         seqs = self.engine.generate([r.token_ids for r in reqs], sps, max_new_tokens=budgets, mm_inputs=mm)
-        return [LLMResponse(list(q.output), list(q.logprobs), q.finish_reason) for q in seqs]
+        return [self._response(q) for q in seqs]
+
+    @staticmethod
+    def _response(q) -> LLMResponse:
+        top = q.sampling.logprobs > 0
+        return LLMResponse(list(q.output), list(q.logprobs), q.finish_reason, list(q.entropies) if top else None,
+                           list(q.top_logprobs) if top else None)
 
     def _sync_objects(self, objs):
         """Broadcast from the replica's first tensor-parallel rank."""
@@ -115,7 +121,7 @@ class AgentModule(RolloutModule):
                 if not lead:
                     continue
                 try:
-                    fresh.append((i, gens[i].send(LLMResponse(list(q.output), list(q.logprobs), q.finish_reason))))
+                    fresh.append((i, gens[i].send(self._response(q))))
                 except StopIteration as e:
                     done[i] = e.value
         sess.close()
@@ -182,6 +188,10 @@ class AgentModule(RolloutModule):
             })
             if o.response_logprobs is not None:
                 r["rollout_logprobs"] = torch.tensor(o.response_logprobs, dtype=torch.float32)
+            if o.response_top_logprobs is not None:
+                # tokens that a tool wrote have no alternatives: id -1, log-prob 0
+                n = max([int(getattr(self.module_args, "num_logprobs", 0))] + [len(t) for t in o.response_top_logprobs])
+                r.update(token_statistics(o.response_entropies, [list(t) + [(-1, 0.0)] * (n - len(t)) for t in o.response_top_logprobs], n))
             res.append(r)
         return res
 

@@ -39,6 +39,9 @@ class AgentGraphOutput:
     visual_time_steps: Any = None        # per image / video: temporal position step (videos), None (images)
     attention_mask: Any = None
     extra_fields: Dict[str, Any] = field(default_factory=dict)
+    # aligned with response_logprobs, where the sampling asks for alternatives
+    response_entropies: Optional[List[float]] = None
+    response_top_logprobs: Optional[List[List[tuple]]] = None
 
 
 class CompiledGraph:
@@ -151,4 +154,5 @@ class BaseAgentGraph:
             loss_mask=mask, response_logprobs=meta.get("logprobs"), num_turns=last + 1,
             pixel_values=mm.get("pixel_values"), image_grid_thw=mm.get("image_grid_thw"),
             visual_time_steps=mm.get("visual_time_steps"),
-            attention_mask=mm.get("attention_mask"))
+            attention_mask=mm.get("attention_mask"),
+            response_entropies=meta.get("entropies"), response_top_logprobs=meta.get("top_logprobs"))

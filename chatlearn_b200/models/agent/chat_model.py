@@ -90,6 +90,13 @@ class LLMResponse:
     output_ids: List[int]
     logprobs: Optional[List[float]] = None
     finish_reason: Optional[str] = None
+    # where the sampling asks for alternatives, per generated token: entropy, likeliest (token, log-prob)
+    entropies: Optional[List[float]] = None
+    top_logprobs: Optional[List[List[tuple]]] = None
+
+
+# statistics of the response's tokens besides their log-probs, and what stands for tokens that have none (a tool's)
+_PER_TOKEN = (("entropies", 0.0), ("top_logprobs", ()))
 
 
 def tool_schema(fn: Callable) -> Dict[str, Any]:
@@ -188,6 +195,9 @@ class ChatModel:
             pre["mm"] = prev["multimodel_batch_feature"]
         if "logprobs" in prev:        # aligned with the response tokens; tool tokens carry 0
             pre["logprobs"] = list(prev["logprobs"]) + [0.0] * len(tail)
+        for key, none in _PER_TOKEN:
+            if key in prev:
+                pre[key] = list(prev[key]) + [none] * len(tail)
         return pre
 
     # ---- generated ids -> AI message -------------------------------------------
@@ -215,6 +225,10 @@ class ChatModel:
             meta["multimodel_batch_feature"] = pre["mm"]
         if resp.logprobs is not None:
             meta["logprobs"] = list(pre.get("logprobs", [])) + list(resp.logprobs)
+            for key, none in _PER_TOKEN:
+                new = getattr(resp, key)
+                if new is not None or key in pre:        # (a turn without them among others)
+                    meta[key] = list(pre.get(key, [none] * len(pre.get("logprobs", [])))) + (list(new) if new is not None else [none] * len(out))
         return Message(content=content, type="ai", tool_calls=good[: self.max_parallel_calls],
                        invalid_tool_calls=bad[: self.max_parallel_calls], response_metadata=meta)
 

@@ -95,3 +95,60 @@ def test_log_probs_of_partial_rounds():
     for r in _partial_rounds(role, [[5, 6, 7, 8], [9, 10, 11]]):
         want = _scored(role, r["all_tokens"], int(r["prompt_token_length"]), 0)
         assert r["rollout_logprobs"].shape == (8,) and (r["rollout_logprobs"] - want.logprob).abs().max() < 1e-4
+
+
+def test_statistics_of_an_agents_turns():
+    """Two turns with a tool's answer between them: one entry per response token, none for the tool's."""
+    from chatlearn_b200.data.tokenizer import ByteTokenizer
+    from chatlearn_b200.models.agent.agent_module import AgentModule
+    from chatlearn_b200.models.agent.chat_model import LLMResponse
+    from chatlearn_b200.models.agent.examples.math_code_agent_graph import MathCodeAgentGraph
+    tok = ByteTokenizer(512)
+    turns = [tok.encode('<tool_call>{"name": "execute_python", "arguments": {"code": "print(6*7)"}}</tool_call>'), tok.encode("The answer is 42")]
+    role = AgentModule.__new__(AgentModule)
+    role._module_args = SimpleNamespace(num_logprobs=2)
+    for with_stats in ((True, True), (False, True), (True, False), (False, False)):
+        gen = MathCodeAgentGraph("mathcode_agent", cfg={"max_ai_message_turn": 3}, tokenizer=tok).run(
+            messages=[{"role": "user", "content": "6*7?"}], sampling_params={}, ground_truth="42")
+        req, n0 = next(gen), 0
+        with pytest.raises(StopIteration) as end:
+            for ids, has in zip(turns, with_stats):
+                n0 = n0 or len(req.token_ids)
+                stats = ([0.25] * len(ids), [[(5, -0.5), (6, -1.5)]] * len(ids)) if has else (None, None)
+                req = gen.send(LLMResponse(ids, [-0.5] * len(ids), "stop", *stats))
+        r, = role.postprocess_func([end.value.value], [{}])
+        if not any(with_stats):
+            assert not any(k in r for k in KEYS)
+            continue
+        T = int(r["response_token_length"])
+        assert r["rollout_logprobs"].shape == r["rollout_entropies"].shape == (T,)
+        tool = T - len(turns[0]) - len(turns[1])
+        has = torch.tensor([with_stats[0]] * len(turns[0]) + [False] * tool + [with_stats[1]] * len(turns[1]))
+        assert tool > 0 and torch.equal(r["rollout_entropies"], torch.where(has, 0.25, 0.0))
+        assert torch.equal(r["rollout_top_ids"], torch.where(has[:, None], torch.tensor([5, 6]), -1))
+        assert torch.equal(r["rollout_top_logprobs"], torch.where(has[:, None], torch.tensor([-0.5, -1.5]), 0.0))
+
+
+@pytest.mark.parametrize("schedule", ["continuous", "lockstep"])
+def test_statistics_reach_the_agents(schedule):
+    """Both ways of answering a graph's requests hand over what the engine has."""
+    from chatlearn_b200.models.agent.agent_module import AgentModule
+    from chatlearn_b200.models.agent.base_agent_graph import AgentGraphOutput, BaseAgentGraph
+    from chatlearn_b200.models.agent.chat_model import LLMRequest
+
+    class OneTurn(BaseAgentGraph):
+        def run(self, sampling_params, prompt_ids=None, **query):
+            a = yield LLMRequest(list(prompt_ids), {"max_new_tokens": 5}, None)
+            return AgentGraphOutput("", list(prompt_ids), list(prompt_ids) + list(a.output_ids), [0] * len(prompt_ids) + [1] * 5,
+                                    a.logprobs, response_entropies=a.entropies, response_top_logprobs=a.top_logprobs)
+
+    for n in (0, 3):
+        role = _rollout(AgentModule, n, agent_scheduling=schedule)
+        role.tp_group = None
+        role.agent_factory = {"one": OneTurn("one", llm=role)}
+        data = [{"agent_name": "one", "prompt_ids": p} for p in ([5, 6, 7], [8, 9])]
+        for r in role.postprocess_func(role.run_trajectories(data), data):
+            if n:
+                _check(role, r, n)
+            else:
+                assert not any(k in r for k in KEYS)
