@@ -286,8 +286,8 @@ def attention_block(arch: ModelArch, p: Dict[str, torch.Tensor], x, ctx: FwdCtx,
             o = ops.paged_attention(q, kvc.k_cache[layer], kvc.v_cache[layer], kvc.block_tables, kvc.seq_lens,
                                     kvc.q_lens, 1.0 / math.sqrt(d), groups=kvc.groups)
             if partial:
-                return ctx.tp_symm.gemm_partial(o.reshape(o.shape[0], -1), p["o_proj"])
-            return _row_parallel(o.reshape(o.shape[0], -1), p["o_proj"], ctx)
+                return ctx.tp_symm.gemm_partial(o.flatten(1), p["o_proj"])
+            return _row_parallel(o.flatten(1), p["o_proj"], ctx)
         q = qkv[:, :nh_l * d].view(T, nh_l, d)
         k = qkv[:, nh_l * d:(nh_l + nkv_l) * d].view(T, nkv_l, d)
         v = qkv[:, (nh_l + nkv_l) * d:].view(T, nkv_l, d)
@@ -314,7 +314,7 @@ def attention_block(arch: ModelArch, p: Dict[str, torch.Tensor], x, ctx: FwdCtx,
         else:
             o = cache_attend(kv, layer, q, scale, ctx)
             if kv.q8 is not None and not partial:
-                return _row_parallel(o.reshape(o.shape[0], -1), p["o_proj"], ctx)
+                return _row_parallel(o.flatten(1), p["o_proj"], ctx)
     elif ctx.cp is not None and ctx.cp.size > 1:
         o = ctx.cp.attention(q, k, v, ctx, scale)
     else:
@@ -322,8 +322,8 @@ def attention_block(arch: ModelArch, p: Dict[str, torch.Tensor], x, ctx: FwdCtx,
     if ctx.sp is not None and ctx.sp.size > 1:
         o = ctx.sp.heads_to_seq(o)
     if partial:
-        return ctx.tp_symm.gemm_partial(o.reshape(o.shape[0], -1), p["o_proj"])
-    out = ops.linear(o.reshape(o.shape[0], -1), p["o_proj"])
+        return ctx.tp_symm.gemm_partial(o.flatten(1), p["o_proj"])
+    out = ops.linear(o.flatten(1), p["o_proj"])
     return _tp_reduce(out, ctx)
 
 
