@@ -733,7 +733,7 @@ class RolloutEngine:
         dev = self.device
         z = lambda dt: torch.zeros(0, dtype=dt, device=dev)  # noqa: E731
         kv = KVCtx(self.k_cache, self.v_cache, z(torch.long), torch.zeros(0, 1, dtype=torch.int32, device=dev),
-                   z(torch.int32), z(torch.int32), True, lin=self._linear_state([]))
+                   z(torch.int32), z(torch.int32), True, q8=self.q8_cache if self.q8 else None, lin=self._linear_state([]))
         ctx = FwdCtx(positions=z(torch.long), cu_seqlens=torch.zeros(1, dtype=torch.int32, device=dev),
                      max_seqlen=0, kv=kv, tp=self.tp, ep=self.ep, tp_symm=self._symm(), fuse_add_norm=True)
         self.model.hidden_states(z(torch.long), ctx)

@@ -6,7 +6,7 @@ from chatlearn_b200.models.nn import CausalLM
 from chatlearn_b200.models.nn.arch import PRESETS
 
 
-@pytest.mark.parametrize("kv_dtype", [None])
+@pytest.mark.parametrize("kv_dtype", [None, torch.float8_e4m3fn])
 @pytest.mark.parametrize("preset", ["tiny_qwen3", "tiny_moe", "tiny_qwen3_next", "tiny_llama", "tiny_mla_moe"])
 def test_idle_step(preset, kv_dtype):
     """No token: every layer runs on none, and the caches stay as they are."""

@@ -5,7 +5,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("kv_dtype", [None])
+@pytest.mark.parametrize("kv_dtype", [None, torch.float8_e4m3fn])
 @pytest.mark.parametrize("experts", [0, 8])
 def test_idle_step(kv_dtype, experts):
     from chatlearn_b200.models.nn import CausalLM, ModelArch
