@@ -20,6 +20,9 @@ def main():
     ap.add_argument("--context", type=int, default=1024)
     ap.add_argument("--steps", type=int, default=32)
     ap.add_argument("--layers", type=int, default=0, help="override the number of layers (0 = model default)")
+    ap.add_argument("--samples", type=int, default=1, help="samples per prompt: they share their prompt's cache blocks")
+    ap.add_argument("--kv-cache-dtype", choices=("auto", "fp8_e4m3"), default="auto")
+    ap.add_argument("--num-logprobs", type=int, default=0, help="alternatives and entropy of every token")
     ap.add_argument("--profile", action="store_true")
     ap.add_argument("--tp", type=int, default=1, help="tensor-parallel size (launch with torchrun --nproc-per-node TP)")
     args = ap.parse_args()
@@ -45,14 +48,16 @@ def main():
     model = CausalLM(arch, dtype=torch.bfloat16, device=dev, tp=args.tp, tp_rank=tp_rank).init_weights(0)
     max_len = args.context + args.steps * 3 + 64
     eng = RolloutEngine(model, tp_group=tp_group, block_size=64, max_num_seqs=args.batch, max_num_batched_tokens=16384,
-                        gpu_memory_utilization=0.8, max_model_len=max_len)
+                        gpu_memory_utilization=0.8, max_model_len=max_len,
+                        kv_dtype=torch.float8_e4m3fn if args.kv_cache_dtype == "fp8_e4m3" else None)
     eng.alloc_kv_cache()
     sched = Scheduler(eng.num_blocks, eng.block_size, args.batch, 16384)
-    sp = SamplingParams(temperature=1.0, max_tokens=args.steps * 3 + 8, ignore_eos=True)
+    sp = SamplingParams(temperature=1.0, max_tokens=args.steps * 3 + 8, ignore_eos=True, logprobs=args.num_logprobs)
     g = torch.Generator().manual_seed(0)
     for i in range(args.batch):
-        sched.add(Sequence(i, torch.randint(0, arch.vocab_size - 1, (args.context,), generator=g).tolist(),
-                           sp.max_tokens, sp))
+        if i % args.samples == 0:
+            prompt = torch.randint(0, arch.vocab_size - 1, (args.context,), generator=g).tolist()
+        sched.add(Sequence(i, list(prompt), sp.max_tokens, sp))
     # warm-up outside the timed prefill (library probes, kernel attribute set-up)
     eng.generate([[1, 2, 3, 4]], SamplingParams(temperature=1.0, max_tokens=2, ignore_eos=True))
     # prefill
@@ -82,6 +87,7 @@ def main():
     weights_gb = model.num_params() * 2 / 1e9
     kv_gb = args.batch * args.context * eng.kv_bytes_per_block() / eng.block_size / 1e9
     out = {"model": args.model, "layers": arch.num_hidden_layers, "batch": args.batch, "context": args.context,
+           "kv_cache_dtype": args.kv_cache_dtype, "samples": args.samples, "num_logprobs": args.num_logprobs,
            "prefill_s": round(prefill_s, 3), "prefill_tok_per_s": round(args.batch * args.context / prefill_s, 1),
            "decode_graph_ms": round(graph_ms, 3), "decode_graph_wall_ms": round(graph_wall, 3),
            "decode_eager_ms": round(eager_ms, 3), "decode_eager_wall_ms": round(eager_wall, 3),

@@ -14,7 +14,7 @@
 //         tile, so that scales of any distance leave each other's keys alone.  V's too (P takes it) where a page covers
 //         the tile.  Of other pages V is brought to the largest of its scales where they are within 2^8 (exact: its
 //         smallest code is then 2^-17), else V becomes bf16 values (exact) and P two bf16, the second what the first's
-//         rounding leaves (17 bits in all), as fp16 has not the range for scales far apart.
+//         rounding leaves (16 bits in all), as fp16 has not the range for scales far apart.
 //         (8 x 256 tokens on pages of 16: 277 us, where every tile's scales are far apart 316)
 //   1     one elected thread issues, for each group, S = Q K^T (128x64x16) into one of two accumulators and O += P V
 //         (128xDx16, P from tensor memory, V as an MN-major operand straight from its row-major tile), one tile behind
@@ -22,8 +22,10 @@
 // The queries are causal inside their sequence's new tokens.  Every mbarrier wait is bounded; one that runs out records a
 // status, the CTA drains and frees its tensor memory.
 //
-// 8 sequences of 512 new tokens after 3,584, 32 / 8 heads of 128: 351 us, 740 TFLOP/s of the visible pairs (45 % of a
-// library product's rate); the tensor pipe is 40 % busy while a CTA runs.  What bounds it: a softmax thread's chain of
+// P is rounded to fp16 (or two bf16) once, as the matrix instruction takes it: 2^-11 of each probability; the sum is fp32.
+//
+// 8 sequences of 512 new tokens after 3,300 to 3,800, 32 / 8 heads of 128: 363 us, 700 TFLOP/s of the visible pairs (42 % of
+// a library product's rate); the tensor pipe is 40 % busy while a CTA runs.  What bounds it: a softmax thread's chain of
 // dependent instructions over its tile (2 warps to a scheduler), and 512 CTAs on 148 SMs, of whose fourth wave half is idle.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>

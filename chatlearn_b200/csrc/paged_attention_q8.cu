@@ -7,6 +7,8 @@
 // cached byte is read once per unit and dequantised once.  Codes become halves by one conversion (exact: e4m3 is a
 // subset of fp16); the scales are powers of two and stay out of the products: s_k joins the softmax scale, s_v the
 // probabilities.  (Products of e4m3 operands are no way around the conversions: mma.sync carries them out in halves.)
+// The probabilities are rounded to fp16 once, as the product beside exact codes takes them (2^-11 of each); their sum is
+// taken in fp32 before.
 // Queries are rescaled per row by a power of two to 2^10..2^11, so that their fp16 form loses nothing that counts (bf16
 // has 8 significant bits, fp16 11; what falls below 2^-24 of a row's largest is lost).
 //
@@ -16,11 +18,13 @@
 // inside a warp's stretch is finished by the warp; parts of divided units meet at the end of the block, and a second
 // kernel joins what a cut between blocks divides.  The cuts go by the lengths alone, so results do not depend on timing.
 //
-// Measured, 32 / 8 heads of 128: 128 sequences of 128 to 2,600 tokens (344 MB) 71 us, 4.8 TB/s; 4 of 30 to 65 thousand (331
-// MB) 70 us; one of 750 9.7 us.  About 10 us stand still (lengths -> tables -> tiles -> parts -> join), the rest runs at 5.4
-// TB/s, which is what two blocks an SM with 96 KB each on their way read (7 TB/s take some 256 KB, more than an SM has);
-// shorter tiles, more or fewer stages or blocks did not change it.  (Of the cuts tried, more shares than resident blocks
-// cost more in parts than they even out.)
+// Measured, 32 / 8 heads of 128, from box to box: 128 sequences of 128 to 2,600 tokens (344 MB) 71 to 82 us, 4.2 to 4.8 TB/s;
+// 4 of 30 to 65 thousand (331 MB) 70 to 78 us; one of 750 9.9 us.  About 10 us stand still (lengths -> tables -> tiles ->
+// parts -> join).  The rest is a warp's own chain over a tile, which has to end before its stage is filled again: with two
+// warps to a scheduler (162 registers, 98 KB of ring a block) an instruction is issued in 35 % of the cycles, DRAM is 57 %
+// busy, no pipe above 34 % (the conversions'), and the warps wait for the instruction before (1.7 of 5 cycles), for the
+// copies (0.8) and for shared memory (0.7).  Shorter tiles, more or fewer stages or blocks did not change it.  (Of the cuts
+// tried, more shares than resident blocks cost more in parts than they even out.)
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/empty.h>

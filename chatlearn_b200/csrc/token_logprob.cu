@@ -14,9 +14,11 @@
 //
 // A row is read by a cluster of 1 to 8 blocks, which write their sums and lists into the first block's shared memory.
 //
-// Reading the logits bounds it; exponentials (one a logit) take half of that time, the selection at the end 3 us (8
-// alternatives) that nothing hides.  128 rows of 152 k fp32 logits with 8: 20.4 us, 3.8 TB/s; 1,024 rows of bf16 with 2, and
-// the gradient: 201 us, 623 MB without the second read of the logits, 4.6 TB/s with it.
+// 128 rows of 152 k fp32 logits with 8 alternatives: 20.3 us, 3.8 TB/s; of bf16 logits 20.0 us, half the bytes.  What
+// bounds it there is not the bytes alone: instructions are issued in 48 % of the cycles for either type, waits are for the
+// loads (fp32), at the barriers of the selection (3 us that nothing hides) and for busy pipes (bf16; exponentials one a
+// logit, conversions, packed fp32 sums).  1,024 rows of bf16 with 16, and the gradient: 200 us, 623 MB without the second
+// read of the logits, 4.7 TB/s with it.
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/ops/empty.h>

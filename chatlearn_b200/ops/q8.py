@@ -10,7 +10,9 @@ sequence are ignored.
 
 On a GPU: head dims 64, 128 and 256, pages of a multiple of 16 tokens, any ratio of query to
 kv heads; bf16 and fp16 queries, bf16, fp16 and fp32 new rows.  What the kernels do not take is
-refused.  A page id outside the cache is skipped when appending and masked when attending.  Two
+refused.  Many new tokens of a sequence go through tensor-core tiles that read its cache once where
+the queries are bf16; fp16 queries go row by row, each reading what it sees: for single tokens that is
+the same, for long chunks it is slow.  A page id outside the cache is skipped when appending and masked when attending.  Two
 sequences of one call must not append to the same page (its contents are then undefined, no
 other page is touched).  Masked places may hold anything, NaN among it, where no query of the call's
 row of new tokens sees them; a NaN value that a later token of the same call sees may reach the

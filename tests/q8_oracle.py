@@ -61,8 +61,8 @@ def attend(q, cache, table, lens, news=None, scale=None):
 
 def attend_bound(out, around, size, L, D, dtype, prob=2.0 ** -11):
     """How far a result may be off.  The output is rounded once (half a step).  Probabilities are rounded to fp16 for
-    the product (2^-11 of each; to bf16, 2^-8, by the kernel that takes long chunks, where its tiles of 64 keys hold
-    several pages: ``prob``).  A score is a sum of D exact products in fp32 (truncating adds: 2^-23 each) times
+    the product (2^-11 of each: ``prob``; the kernel that takes long chunks rounds them to two bf16, 2^-16, where its
+    tiles of 64 keys hold pages whose V scales are far apart).  A score is a sum of D exact products in fp32 (truncating adds: 2^-23 each) times
     rounded factors (4 roundings): (D + 8) 2^-23 of sum |q k|; fp16 queries lose 2^-11 of elements below 2^-24 of their
     row's largest: 2^-33 sum |q k|, inside that.  The exponential adds 2^-22, and the maximum it is relative to as much again.
     Numerator and denominator each carry the score's error.  The sums over L tokens: 2^-23 per add."""

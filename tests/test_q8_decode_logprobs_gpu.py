@@ -42,8 +42,8 @@ def test_decode_steps_on_the_8_bit_cache(head_dim):
     s is the spread of a row's logits.  A hidden state is rounded to bf16 some 14 times a layer, 28 times in all, each with
     a standard deviation of 2^-9 / sqrt 3 of itself; two runs, five deviations: 5 sqrt(2 * 28) 2^-9 / sqrt 3 = 0.042 s.
     The second layer's keys and values, apart by some 2^-7 then, fall on neighbouring codes (2^-3.5 apart) once in 2^3.5:
-    sqrt(2^-3.5) 2^-3.5 = 2^-5.3 in the mean, five deviations: 0.13 s more.  e4m3 itself rounds keys and values by 2^-5.3 in the mean, which is what an attention output is off by at most in the mean,
-    and so a layer's share of the hidden state; two layers, five deviations: 5 sqrt 2 2^-5.3 = 0.18 s more."""
+    sqrt(2^-3.5) 2^-3.5 = 2^-5.3 in the mean, five deviations: 0.13 s more.  e4m3 itself rounds keys and values by
+    2^-5.3 in the mean, which is what an attention output is off by at most in the mean, and so a layer's share of the hidden state; two layers, five deviations: 5 sqrt 2 2^-5.3 = 0.18 s more."""
     arch, model = _model(head_dim)
     g = torch.Generator().manual_seed(4)
     prompts = [torch.randint(0, arch.vocab_size - 1, (n,), generator=g).tolist() for n in (333, 150, 90, 64)]
